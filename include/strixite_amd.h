@@ -265,6 +265,94 @@ int sx_mtp_accept(const sx_logit_cand *cands, const uint32_t *nan, int64_t kc, c
                   const double *u, double temperature, int64_t top_k, double top_p, int64_t n_valid, int32_t *out,
                   sx_stream stream);
 
+/* ---- a verify layer's attention half: norm with FP8 output, FP8 linear, attention of drafted tokens over a paged
+ * cache, append to that cache. No reference counterparts (its attention, kernels/attention.hpp, reads a contiguous
+ * BF16 cache and one chain of tokens; its norm, kernels/norm.hpp, has no 8-bit output). ---- */
+/* r = x + residual (rounded to act, stored to residual_out), y = r / sqrt(mean(r^2) + eps) * (weight + w_add).
+ * x [M, K] with row stride ldx; residual (nullable: r = x), residual_out, y (nullable) [M, K] and weight [K] in act; q
+ * (nullable) [M, K] e4m3 codes of y with scale [M, K / 128] FP32 = amax(|y|) / 448 of each run of 128 features: the
+ * activations sx_linear_fp8 takes. A run of zeros has scale 0 and codes 0; a run that holds NaN comes out NaN.
+ * K a multiple of 128, up to 32768. y may be x or the residual, residual_out the residual or x, row for row. */
+int sx_add_rms_norm_fp8(const void *x, int64_t ldx, const void *residual, const void *weight, int64_t M, int64_t K,
+                        float eps, float w_add, void *residual_out, void *y, uint8_t *q, float *scale, int act,
+                        sx_stream stream);
+
+/* An FP8 weight: q [N, K] e4m3 (OCP) row-major, 16-byte aligned; scale [ceil(N / 128), K / 128] FP32, one for each
+ * 128 x 128 tile; w = code * scale. K a multiple of 128. */
+typedef struct sx_fp8_view {
+    const uint8_t *q;
+    const float *scale;
+    int64_t N, K;
+} sx_fp8_view;
+/* y[M, N] (out_act) = x * w^T with x [M, K] e4m3 codes (16-byte aligned) and x_scale [M, K / 128] FP32. Products of a
+ * block of 128 are exact, sums FP32, one rounding at the store. */
+int sx_linear_fp8(const uint8_t *x, const float *x_scale, const sx_fp8_view *w, void *y, int64_t M, int out_act,
+                  sx_stream stream);
+
+/* BF16 rows of heads: element [t, h, d] at p[t * token + h * head + d] (with layers: + l * layer). Strides in
+ * elements, multiples of 8; p 16-byte aligned. A slice of a packed query / key / value projection is one. */
+typedef struct sx_head_rows {
+    void *p;
+    int64_t token, head, layer;
+} sx_head_rows;
+enum sx_kv_dtype { SX_KV_BF16 = 0, SX_KV_E4M3 = 1 };
+/* A paged cache of keys and values: position p of sequence b is row p % page_size of page table[b, p / page_size],
+ * at k[layer * k_layer + page * k_page + row * k_token + head * k_head + d] (strides in elements, multiples of 16
+ * bytes, any order; v alike). page_size a power of two, 16 to 65536. table [batch, pages_per_seq] with row stride
+ * table_ld and lens [batch] (cached tokens) are device int32. E4M3: value = code * k_scale (v_scale). */
+typedef struct sx_kv_cache {
+    void *k, *v;
+    int32_t dtype;
+    float k_scale, v_scale;
+    int64_t pages, page_size, heads, dim, layers;
+    int64_t k_page, k_token, k_head, k_layer;
+    int64_t v_page, v_token, v_head, v_layer;
+    const int32_t *table;
+    int64_t table_ld, pages_per_seq;
+    const int32_t *lens;
+    int64_t batch;
+} sx_kv_cache;
+/* Attention of drafted tokens: sequence b's are rows starts[b] .. starts[b + 1] - 1 (device int32 [batch + 1]) of q
+ * [T, Hq, dim], k_new and v_new [T, heads, dim]; none to max_new (1..256) of them, T bounds them all. Token t sees
+ * every cached token of its sequence and, of the drafted ones, number j of the sequence where bit j % 64 of
+ * mask[t * mask_ld + j / 64] is set (its ancestors and itself for a tree; a chain: all up to itself). out = softmax(
+ * scale * q k^T) v per query head h over key head h / (Hq / heads); a row that sees nothing is zero. A drafted token
+ * that a row does not see does not touch it, NaN and infinities included. lse (nullable) [T, Hq] FP32: the natural
+ * logarithm of each row's sum of exp(score). Rows behind starts[batch] are left as they are. dim 64, 128 or 256; Hq a
+ * multiple of heads; batch up to 1024. ws: sx_tree_attention_workspace_bytes bytes, 16-byte aligned, its contents
+ * never read before they are written; one per stream. A sequence with impossible words (a length its table does not
+ * hold, a run of tokens that is negative, over max_new or outside T) or a page outside the cache is not read: its
+ * rows come out NaN (none, where the run itself is impossible) and err (nullable) is {1, the length or page, the
+ * sequence}. */
+int sx_tree_attention_workspace_bytes(int64_t B, int64_t Hq, int64_t Hkv, int64_t D, int64_t max_new, size_t *bytes);
+int sx_tree_attention(const sx_head_rows *q, const sx_head_rows *k_new, const sx_head_rows *v_new, int64_t T, int64_t Hq,
+                      const sx_kv_cache *cache, const int32_t *starts, int64_t max_new, const uint64_t *mask,
+                      int64_t mask_ld, float scale, const sx_head_rows *out, float *lse, void *ws, size_t ws_bytes,
+                      uint32_t *err, sx_stream stream);
+/* The accepted tokens into every layer of the cache: for i < count[b] (device int32 [batch], up to max_count), drafted
+ * row starts[b] + path[b * path_ld + i] (path null: starts[b] + i) goes to position lens[b] + i. BF16 rows are copied,
+ * E4M3 takes the nearest code of x / scale, saturating at 448. lens is only read; lens_out (nullable, apart from lens)
+ * gets lens + count. The pages for the new positions are the caller's to provide, each to one sequence. A sequence
+ * with an impossible word (a run of tokens as above, a count over max_count or the table, a path entry outside the
+ * sequence's drafted tokens, a page outside the cache) keeps its length and gets nothing; err (nullable) is then {1,
+ * the count, path entry or page, the sequence}. */
+int sx_kv_append(const sx_head_rows *k_new, const sx_head_rows *v_new, int64_t T, const sx_kv_cache *cache,
+                 const int32_t *starts, const int32_t *count, int64_t max_count, const int32_t *path, int64_t path_ld,
+                 int32_t *lens_out, uint32_t *err, sx_stream stream);
+
+/* ---- routing by scores (no reference counterpart; sx_moe_router is the reference's) ----
+ * s = sigmoid(logit) or the softmax over the E experts, c = s + bias[e] (bias nullable, FP32). With groups > 1 (equal
+ * runs of E / groups experts) only the top_groups groups with the largest sum of their group_best (1 or 2) best c stay
+ * in the choice. ids: the k largest c, larger first; every tie, of groups too, goes to the lower index. coef = s of
+ * the chosen ones (without the bias), divided by their sum if renorm (a sum of zero leaves them zero), times factor.
+ * Scores and choices are FP64, coef rounded once. Shared slot, errors (a non-finite logit or bias; err nullable) and layouts
+ * as sx_moe_router's; factor does not touch the shared slot. groups <= 64, k in 1..min(E, 32), E in 1..1024. */
+enum sx_score { SX_SCORE_SIGMOID = 0, SX_SCORE_SOFTMAX = 1 };
+int sx_moe_router_scored(const void *logits, int64_t ld, int64_t M, int64_t E, int64_t k, int score, const float *bias,
+                         int64_t groups, int64_t top_groups, int64_t group_best, int renorm, float factor,
+                         const void *shared_logit, int64_t shared_ld, int32_t shared_id, int32_t *ids, float *coef,
+                         int act, uint32_t *err, sx_stream stream);
+
 /* ---- strixw weight files: formats/strixw.hpp (the reader, StrixwFile :86-112) and runtime/strixw_loader.hpp (the
  * upload, StrixwDevice :22-52) ----
  * A file is a 128-byte header (magic "STRIXWT\0", format version 1..4, index and data-region offsets, file size, the

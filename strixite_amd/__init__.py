@@ -12,6 +12,8 @@ LIB_PATH = os.path.join(HERE, "libstrixite_amd.so")
 SX_OK, SX_EINVAL, SX_EHIP, SX_EUNSUPPORTED = 0, 1, 2, 3
 ACT_F32, ACT_BF16 = 0, 1
 MOE_F32, MOE_WMMA_BF16, MOE_WMMA_F16 = 0, 1, 2
+KV_BF16, KV_E4M3 = 0, 1
+SCORE_SIGMOID, SCORE_SOFTMAX = 0, 1
 
 
 class SxError(RuntimeError):
@@ -40,6 +42,28 @@ class MtpPick(ctypes.Structure):
                 ("emb", ctypes.c_ulonglong)]
 
 
+class Fp8View(ctypes.Structure):
+    """sx_fp8_view: an e4m3 weight [N, K] with one FP32 scale for each 128 x 128 tile."""
+    _fields_ = [("q", ctypes.c_void_p), ("scale", ctypes.c_void_p), ("N", ctypes.c_int64), ("K", ctypes.c_int64)]
+
+
+class HeadRows(ctypes.Structure):
+    """sx_head_rows: BF16 rows of heads, strides in elements."""
+    _fields_ = [("p", ctypes.c_void_p), ("token", ctypes.c_int64), ("head", ctypes.c_int64), ("layer", ctypes.c_int64)]
+
+
+class KvCacheC(ctypes.Structure):
+    """sx_kv_cache: a paged cache of keys and values."""
+    _fields_ = [("k", ctypes.c_void_p), ("v", ctypes.c_void_p), ("dtype", ctypes.c_int32), ("k_scale", ctypes.c_float),
+                ("v_scale", ctypes.c_float), ("pages", ctypes.c_int64), ("page_size", ctypes.c_int64),
+                ("heads", ctypes.c_int64), ("dim", ctypes.c_int64), ("layers", ctypes.c_int64),
+                ("k_page", ctypes.c_int64), ("k_token", ctypes.c_int64), ("k_head", ctypes.c_int64),
+                ("k_layer", ctypes.c_int64), ("v_page", ctypes.c_int64), ("v_token", ctypes.c_int64),
+                ("v_head", ctypes.c_int64), ("v_layer", ctypes.c_int64), ("table", ctypes.c_void_p),
+                ("table_ld", ctypes.c_int64), ("pages_per_seq", ctypes.c_int64), ("lens", ctypes.c_void_p),
+                ("batch", ctypes.c_int64)]
+
+
 class StrixwComponentC(ctypes.Structure):
     """sx_strixw_component: StrixwComponent (formats/strixw.hpp:30-33)."""
     _fields_ = [("role", ctypes.c_uint8), ("offset", ctypes.c_uint64), ("bytes", ctypes.c_uint64),
@@ -55,6 +79,7 @@ class StrixwTensorC(ctypes.Structure):
 
 _P, _I64, _INT, _D, _SZP = ctypes.c_void_p, ctypes.c_int64, ctypes.c_int, ctypes.c_double, ctypes.POINTER(ctypes.c_size_t)
 _QV = ctypes.POINTER(QView)
+_HR, _KV, _F = ctypes.POINTER(HeadRows), ctypes.POINTER(KvCacheC), ctypes.c_float
 _U64, _CP, _PCP = ctypes.c_uint64, ctypes.c_char_p, ctypes.POINTER(ctypes.c_char_p)
 _PI64 = ctypes.POINTER(ctypes.c_int64)
 
@@ -102,6 +127,13 @@ SIGNATURES = {
     "sx_mtp_head_pick": [_P, _QV, _INT, _P, _P, _P, _P, _P, _P, _P, ctypes.c_size_t, _P],
     "sx_mtp_pick_ws": [_P, _I64, _P, _P, _P, _P, _P, _P, ctypes.c_size_t, _P],
     "sx_mtp_accept": [_P, _P, _I64, _P, _I64, _P, _D, _I64, _D, _I64, _P, _P],
+    "sx_add_rms_norm_fp8": [_P, _I64, _P, _P, _I64, _I64, _F, _F, _P, _P, _P, _P, _INT, _P],
+    "sx_linear_fp8": [_P, _P, ctypes.POINTER(Fp8View), _P, _I64, _INT, _P],
+    "sx_tree_attention_workspace_bytes": [_I64, _I64, _I64, _I64, _I64, _SZP],
+    "sx_tree_attention": [_HR, _HR, _HR, _I64, _I64, _KV, _P, _I64, _P, _I64, _F, _HR, _P, _P, ctypes.c_size_t, _P, _P],
+    "sx_kv_append": [_HR, _HR, _I64, _KV, _P, _P, _I64, _P, _I64, _P, _P, _P],
+    "sx_moe_router_scored": [_P, _I64, _I64, _I64, _I64, _INT, _P, _I64, _I64, _I64, _INT, _F, _P, _I64, ctypes.c_int32,
+                             _P, _P, _INT, _P, _P],
     "sx_strix_hash64": [_P, _U64],
     "sx_strixw_open": [_CP, ctypes.POINTER(_P)],
     "sx_strixw_close": [_P],

@@ -55,6 +55,11 @@ __device__ __forceinline__ void flag_error(uint32_t *err, uint32_t a, uint32_t b
     }
 }
 
+// flag_error where the caller may have passed no slot.
+__device__ __forceinline__ void report(uint32_t *err, uint32_t a, uint32_t b) {
+    if (err != nullptr) flag_error(err, a, b);
+}
+
 // ---------------- host error channel ----------------
 
 void set_error(const std::string &msg);

@@ -8,7 +8,8 @@ import ctypes
 
 import torch
 
-from . import (ACT_BF16, ACT_F32, MOE_F32, SX_EINVAL, LogitCand, MtpPick, QView, SxError, check, lib)
+from . import (ACT_BF16, ACT_F32, KV_BF16, KV_E4M3, MOE_F32, SCORE_SIGMOID, SCORE_SOFTMAX, SX_EINVAL, Fp8View, HeadRows,
+               KvCacheC, LogitCand, MtpPick, QView, SxError, check, lib)
 
 _c = ctypes.c_void_p
 
@@ -416,3 +417,279 @@ def mtp_accept(cands, nan, drafts, u, temperature, top_k, top_p, n_valid, out=No
     check(lib().sx_mtp_accept(_p(cands), _p(nan), kc, _p(drafts), k, _p(u), float(temperature), int(top_k),
                               float(top_p), int(n_valid), _p(out), _s(stream)))
     return out
+
+
+# ---------------- a verify layer's attention half, and routing by scores ----------------
+# Strides, types, shapes and devices are checked here, where the tensors are; the library checks the rest. A call runs
+# on its tensors' device, on that device's current stream unless one is given. err (optional, a zeroed int32 [4] on the
+# device) receives what a call could not read; without it the outputs alone say so.
+
+def _refuse(*what):
+    raise SxError(SX_EINVAL, " ".join(str(w) for w in what))
+
+
+def _is(name, t, dtype, shape):
+    if t.dtype != dtype or t.shape != shape or not t.is_contiguous():
+        _refuse(name, "must be a contiguous", dtype, tuple(shape), "and is", t.dtype, tuple(t.shape), t.stride())
+
+
+def _together(dev, tensors):
+    """Refuses tensors (None: left out) that are not on GPU `dev`, a tensor's get_device()."""
+    if dev < 0:
+        _refuse("the tensors are not on a GPU")
+    for t in tensors:
+        if t is not None and t.get_device() != dev:
+            _refuse("tensors on", t.device, "and on GPU", dev, "in one call")
+
+
+def _run(dev, f, *args, stream=None):
+    """f(*args, stream) on GPU dev, whichever is current."""
+    if dev != torch.cuda.current_device():
+        with torch.cuda.device(dev):
+            return _run(dev, f, *args, stream=stream)
+    rc = f(*args, torch._C._cuda_getCurrentRawStream(dev) if stream is None else stream.cuda_stream)
+    if rc:
+        check(rc)
+
+
+def _a(t):
+    return None if t is None else t.data_ptr()
+
+
+class Fp8Weight:
+    """An e4m3 weight resident on the device: q [N, K] torch.float8_e4m3fn, scale [ceil(N / 128), K / 128] FP32, one
+    for each 128 x 128 tile (w = code * scale)."""
+
+    def __init__(self, q, scale):
+        if q.dim() != 2 or q.shape[1] % 128:
+            _refuse("an FP8 weight is [N, K], K a multiple of 128, and not", tuple(q.shape))
+        self.N, self.K = (int(n) for n in q.shape)
+        _is("q", q, torch.float8_e4m3fn, (self.N, self.K))
+        _is("scale", scale, torch.float32, (-(-self.N // 128), self.K // 128))
+        if scale.device != q.device:
+            _refuse("q is on", q.device, "and scale on", scale.device)
+        self.q, self.scale = q, scale
+        self._view = Fp8View(q.data_ptr(), scale.data_ptr(), self.N, self.K)
+
+    def view(self):
+        return ctypes.byref(self._view)
+
+    def nbytes(self):
+        return self.q.numel() + 4 * self.scale.numel()
+
+
+def add_rms_norm_fp8(x, weight, eps=1e-6, residual=None, residual_out=None, w_add=0.0, y=None, q=None, scale=None,
+                     stream=None):
+    """r = x + residual, y = r / sqrt(mean(r^2) + eps) * (weight + w_add) as e4m3 codes q [M, K] and FP32 scales
+    [M, K / 128], the activations linear_fp8 takes. x [M, K] (any row stride) in FP32 or BF16; y (optional): a buffer
+    that receives y itself in x's type. Returns (q, scale, residual_out or None); residual_out may be the residual."""
+    act, dtype, dev = act_of(x), x.dtype, x.get_device()
+    if x.dim() != 2 or x.stride(1) != 1 or x.shape[1] % 128:
+        _refuse("x must be [M, K] with dense rows, K a multiple of 128, and is", tuple(x.shape), x.stride())
+    M, K = shape = x.shape
+    _together(dev, (weight, residual, residual_out, y, q, scale))
+    _is("weight", weight, dtype, (K,))
+    if residual is not None:
+        _is("residual", residual, dtype, shape)
+        if residual_out is None:
+            residual_out = torch.empty_like(residual)
+        else:
+            _is("residual_out", residual_out, dtype, shape)
+    elif residual_out is not None:
+        _refuse("residual_out without a residual")
+    if y is not None:
+        _is("y", y, dtype, shape)
+    if q is None:
+        q = x.new_empty(shape, dtype=torch.float8_e4m3fn)
+    else:
+        _is("q", q, torch.float8_e4m3fn, shape)
+    if scale is None:
+        scale = x.new_empty((M, K // 128), dtype=torch.float32)
+    else:
+        _is("scale", scale, torch.float32, (M, K // 128))
+    _run(dev, lib().sx_add_rms_norm_fp8, x.data_ptr(), x.stride(0) if M > 1 else K, _a(residual), weight.data_ptr(), M, K,
+         eps, w_add, _a(residual_out), _a(y), q.data_ptr(), scale.data_ptr(), act, stream=stream)
+    return q, scale, residual_out
+
+
+def linear_fp8(x, x_scale, w, out_act=ACT_BF16, y=None, stream=None):
+    """y[M, N] = (x * x_scale) * w^T: x e4m3 codes [M, K] with an FP32 scale for each run of 128 (add_rms_norm_fp8's
+    outputs), w an Fp8Weight; y BF16 or (out_act ACT_F32) FP32."""
+    dev, M, dtype = x.get_device(), x.shape[0], dtype_of(out_act)
+    _together(dev, (x_scale, w.q, y))
+    _is("x", x, torch.float8_e4m3fn, (M, w.K))
+    _is("x_scale", x_scale, torch.float32, (M, w.K // 128))
+    if y is None:
+        y = x.new_empty((M, w.N), dtype=dtype)
+    else:
+        _is("y", y, dtype, (M, w.N))
+    _run(dev, lib().sx_linear_fp8, x.data_ptr(), x_scale.data_ptr(), w.view(), y.data_ptr(), M, out_act, stream=stream)
+    return y
+
+
+def _head_rows(name, t, heads, dim, layered=False):
+    """The sx_head_rows of a BF16 tensor [T, heads, dim] (layered: [layers, T, heads, dim]); dims dense, other strides
+    free."""
+    if t.dtype != torch.bfloat16 or t.dim() != 3 + layered or t.shape[-2:] != (heads, dim) or t.stride(-1) != 1:
+        _refuse(name, f"must be BF16 [tokens, {heads}, {dim}] with dense rows and is", t.dtype, tuple(t.shape), t.stride())
+    s = t.stride()
+    return HeadRows(t.data_ptr(), s[-3], s[-2], s[0] if layered else 0)
+
+
+def _kv_cache(k, v, table, lens, k_scale, v_scale, layered=False):
+    """The sx_kv_cache of [pages, page, heads, dim] tensors (layered: [layers, ...]) with free strides."""
+    dtype = k.dtype
+    if dtype != torch.bfloat16 and dtype != torch.float8_e4m3fn or v.dtype != dtype:
+        _refuse("the cache is BF16 or float8_e4m3fn, not", dtype, v.dtype)
+    ks, vs, shape = k.stride(), v.stride(), k.shape
+    if len(shape) != 4 + layered or v.shape != shape or ks[-1] != 1 or vs[-1] != 1:
+        _refuse("k and v caches must be [pages, page, heads, dim] alike with dense rows:", tuple(shape), tuple(v.shape))
+    if table.dtype != torch.int32 or table.dim() != 2 or table.stride(1) != 1:
+        _refuse("table must be int32 [batch, pages a sequence] with dense rows")
+    B, P = table.shape
+    _is("lens", lens, torch.int32, (B,))
+    pages, page, heads, dim = shape[-4:]
+    return KvCacheC(k.data_ptr(), v.data_ptr(), KV_BF16 if dtype == torch.bfloat16 else KV_E4M3, k_scale, v_scale, pages,
+                    page, heads, dim, shape[0] if layered else 1, ks[-4], ks[-3], ks[-2], ks[0] if layered else 0, vs[-4],
+                    vs[-3], vs[-2], vs[0] if layered else 0, table.data_ptr(), table.stride(0) if B > 1 else P, P,
+                    lens.data_ptr(), B)
+
+
+def tree_mask(parents):
+    """The mask of drafted trees: parents is one list a sequence, each token's parent in it (-1: a root, which sees the
+    cache alone; a parent comes before its children). Returns int64 [T, ceil(longest / 64)] on the host: bit j of a
+    token's words says that it sees drafted token j of its sequence, itself and its ancestors."""
+    words = (max((len(p) for p in parents), default=0) + 63) // 64
+    rows = []
+    for seq in parents:
+        first = len(rows)
+        for i, p in enumerate(seq):
+            if not -1 <= p < i:
+                raise ValueError(f"token {i} has parent {p}")
+            rows.append((rows[first + p] if p >= 0 else 0) | 1 << i)
+    signed = lambda w: w - (1 << 64) if w >> 63 else w
+    return torch.tensor([[signed(r >> 64 * i & (1 << 64) - 1) for i in range(words)] for r in rows], dtype=torch.int64)
+
+
+def tree_attention_workspace_bytes(B, Hq, Hkv, D, max_new):
+    n = ctypes.c_size_t()
+    check(lib().sx_tree_attention_workspace_bytes(B, Hq, Hkv, D, max_new, ctypes.byref(n)))
+    return n.value
+
+
+def tree_attention_workspace(q, k_new, starts, max_new):
+    """A workspace for tree_attention calls of these shapes (one per stream; nothing in it outlives a call)."""
+    with torch.cuda.device(q.device):
+        n = tree_attention_workspace_bytes(starts.numel() - 1, q.shape[1], k_new.shape[1], q.shape[2], max_new)
+    return torch.empty((n + 7) // 8, dtype=torch.int64, device=q.device)
+
+
+def tree_attention(q, k_new, v_new, k_cache, v_cache, table, lens, starts, mask, max_new, scale=None, k_scale=1.0,
+                   v_scale=1.0, out=None, lse=None, ws=None, err=None, stream=None):
+    """Attention of drafted tokens (q [T, Hq, D], k_new and v_new [T, Hkv, D], BF16, any token and head strides) over
+    their sequences' cached tokens and, as the mask says, each other. The cache: k_cache, v_cache [pages, page, Hkv, D]
+    (BF16, or float8_e4m3fn holding value / k_scale and value / v_scale), table int32 [B, pages a sequence], lens int32
+    [B]. starts int32 [B + 1]: sequence b's drafted tokens are rows starts[b] .. starts[b + 1] - 1, at most max_new.
+    mask int64 [T, words] as tree_mask makes it. scale: of the scores, 1 / sqrt(D) unless given. lse (optional): an
+    FP32 [T, Hq] buffer for the rows' log sums. ws: tree_attention_workspace(), made for the call unless given. Returns
+    (out [T, Hq, D] BF16, err)."""
+    dev = q.get_device()
+    if q.dim() != 3 or k_new.dim() != 3:
+        _refuse("q, k_new and v_new are [tokens, heads, dim]")
+    T, Hq, D = q.shape
+    Hkv = k_new.shape[1]
+    _together(dev, (k_new, v_new, k_cache, v_cache, table, lens, starts, mask, out, lse, ws, err))
+    cache = _kv_cache(k_cache, v_cache, table, lens, k_scale, v_scale)
+    if (cache.heads, cache.dim) != (Hkv, D) or k_new.shape[0] != T or v_new.shape[0] != T:
+        _refuse("q", tuple(q.shape), "k_new", tuple(k_new.shape), "v_new", tuple(v_new.shape), "cache", tuple(k_cache.shape))
+    _is("starts", starts, torch.int32, (cache.batch + 1,))
+    if mask.dtype != torch.int64 or mask.dim() != 2 or mask.shape[0] != T or mask.stride(1) != 1 or mask.shape[1] * 64 < max_new:
+        _refuse("mask must be int64 [T, ceil(max_new / 64)] with dense rows and is", mask.dtype, tuple(mask.shape))
+    if out is None:
+        out = torch.empty((T, Hq, D), dtype=torch.bfloat16, device=q.device)
+    elif out.dim() != 3 or out.shape[0] != T:
+        _refuse("out is", tuple(out.shape))
+    if lse is not None:
+        _is("lse", lse, torch.float32, (T, Hq))
+    if ws is None:
+        ws = tree_attention_workspace(q, k_new, starts, max_new)
+    rq, rk, rv = _head_rows("q", q, Hq, D), _head_rows("k_new", k_new, Hkv, D), _head_rows("v_new", v_new, Hkv, D)
+    ro, ref = _head_rows("out", out, Hq, D), ctypes.byref
+    _run(dev, lib().sx_tree_attention, ref(rq), ref(rk), ref(rv), T, Hq, ref(cache), starts.data_ptr(), max_new,
+         mask.data_ptr(), mask.stride(0) if T > 1 else mask.shape[1], D ** -0.5 if scale is None else scale, ref(ro),
+         _a(lse), ws.data_ptr(), ws.numel() * ws.element_size(), _a(err), stream=stream)
+    return out, err
+
+
+def kv_append(k_new, v_new, k_cache, v_cache, table, lens, starts, count, path=None, max_count=None, k_scale=1.0,
+              v_scale=1.0, lens_out=None, err=None, stream=None):
+    """The accepted drafted tokens into the paged cache, all layers in one launch: for i < count[b], row
+    starts[b] + path[b, i] (path None: starts[b] + i) of k_new and v_new [layers, T, Hkv, D] to position lens[b] + i of
+    k_cache and v_cache [layers, pages, page, Hkv, D] (one layer: without that dimension). count int32 [B]; path int32
+    [B, at most], whose width bounds the counts (without a path max_count does). Returns (lens_out = lens + count,
+    err); lens itself is only read. A sequence that cannot be appended to as asked keeps its length and its pages."""
+    dev, layered, shape = k_new.get_device(), k_new.dim() == 4, k_new.shape
+    if len(shape) not in (3, 4) or v_new.shape != shape:
+        _refuse("k_new", tuple(shape), "and v_new", tuple(v_new.shape))
+    _together(dev, (v_new, k_cache, v_cache, table, lens, starts, count, path, lens_out, err))
+    cache = _kv_cache(k_cache, v_cache, table, lens, k_scale, v_scale, layered)
+    T, B = shape[-3], cache.batch
+    if layered and shape[0] != cache.layers:
+        _refuse("k_new has", shape[0], "layers and the cache", cache.layers)
+    rk = _head_rows("k_new", k_new, cache.heads, cache.dim, layered)
+    rv = _head_rows("v_new", v_new, cache.heads, cache.dim, layered)
+    _is("starts", starts, torch.int32, (B + 1,))
+    _is("count", count, torch.int32, (B,))
+    ld = 0
+    if path is not None:
+        if path.dtype != torch.int32 or path.dim() != 2 or path.shape[0] != B or path.stride(1) != 1:
+            _refuse("path must be int32 [batch, most tokens kept] with dense rows")
+        max_count = path.shape[1] if max_count is None else max_count
+        ld = path.stride(0) if B > 1 else path.shape[1]
+        if max_count > path.shape[1]:
+            _refuse("max_count =", max_count, "is over the path's", path.shape[1])
+    elif max_count is None:
+        _refuse("max_count is needed without a path")
+    if lens_out is None:
+        lens_out = torch.empty_like(lens)
+    else:
+        _is("lens_out", lens_out, torch.int32, (B,))
+    ref = ctypes.byref
+    _run(dev, lib().sx_kv_append, ref(rk), ref(rv), T, ref(cache), starts.data_ptr(), count.data_ptr(), max_count, _a(path),
+         ld, lens_out.data_ptr(), _a(err), stream=stream)
+    return lens_out, err
+
+
+SCORES = {"sigmoid": SCORE_SIGMOID, "softmax": SCORE_SOFTMAX}
+
+
+def moe_router_scored(logits, E, k, score="sigmoid", bias=None, groups=1, top_groups=1, group_best=2, renorm=True,
+                      factor=1.0, shared=None, shared_ld=1, shared_id=0, ids=None, coef=None, err=None, stream=None):
+    """Routing by scores: s = sigmoid or softmax of logits [M, >= E] (any row stride); the k experts with the largest
+    s + bias, inside the top_groups of `groups` runs of experts by the sum of their group_best best; coef = s of those,
+    divided by their sum if renorm, times factor. bias FP32 [E] or None. The shared slot as moe_router's. Returns (ids,
+    coef, err)."""
+    dev, act = logits.get_device(), act_of(logits)
+    if logits.dim() != 2 or logits.stride(1) != 1 or logits.shape[1] < E:
+        _refuse("logits are", tuple(logits.shape), logits.stride(), "for E =", E)
+    if score not in SCORES:
+        _refuse("score is", repr(score), "and not one of", list(SCORES))
+    M = logits.shape[0]
+    shape = (M, k + (1 if shared is not None else 0))
+    _together(dev, (bias, shared, ids, coef, err))
+    if bias is not None:
+        _is("bias", bias, torch.float32, (E,))
+    if shared is not None and (shared.dtype != logits.dtype or shared.shape[0] != M):
+        _refuse("shared is", shared.dtype, tuple(shared.shape), "for logits", logits.dtype, tuple(logits.shape))
+    if ids is None:
+        ids = torch.empty(shape, dtype=torch.int32, device=logits.device)
+    else:
+        _is("ids", ids, torch.int32, shape)
+    if coef is None:
+        coef = torch.empty(shape, dtype=torch.float32, device=logits.device)
+    else:
+        _is("coef", coef, torch.float32, shape)
+    _run(dev, lib().sx_moe_router_scored, logits.data_ptr(), logits.stride(0) if M > 1 else logits.shape[1], M, E, k,
+         SCORES[score], _a(bias), groups, top_groups if groups > 1 else 1, group_best if groups > 1 else 1, int(renorm),
+         factor, _a(shared), shared_ld, shared_id, ids.data_ptr(), coef.data_ptr(), act, _a(err), stream=stream)
+    return ids, coef, err
