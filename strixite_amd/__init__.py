@@ -79,7 +79,7 @@ class StrixwTensorC(ctypes.Structure):
 
 _P, _I64, _INT, _D, _SZP = ctypes.c_void_p, ctypes.c_int64, ctypes.c_int, ctypes.c_double, ctypes.POINTER(ctypes.c_size_t)
 _QV = ctypes.POINTER(QView)
-_HR, _KV, _F = ctypes.POINTER(HeadRows), ctypes.POINTER(KvCacheC), ctypes.c_float
+_HR, _KV, _F = _P, _P, ctypes.c_float  # HeadRows and KvCacheC, by reference or as bytes
 _U64, _CP, _PCP = ctypes.c_uint64, ctypes.c_char_p, ctypes.POINTER(ctypes.c_char_p)
 _PI64 = ctypes.POINTER(ctypes.c_int64)
 

@@ -718,7 +718,7 @@ Plan plan_of(int64_t D, int64_t G, int64_t Hkv, int64_t max_new) {
 
 const char *shape_error(int64_t B, int64_t Hq, int64_t Hkv, int64_t D, int64_t max_new) {
     if (D != 64 && D != 128 && D != 256) return "head dimension: 64, 128 or 256";
-    if (Hkv < 1 || Hkv > 4096 || Hq < Hkv || Hq > 65536 || Hq % Hkv != 0) return "query heads: a multiple of the key heads";
+    if (Hkv < 1 || Hkv > 4096 || Hq < Hkv || Hq > 65535 || Hq % Hkv != 0) return "query heads: a multiple of the key heads";
     if (max_new < 1 || max_new > kMaxNew) return "max_new: 1..256";
     if (B < 1 || B > kMaxSeqs) return "sequences: 1..1024";
     return nullptr;
@@ -790,7 +790,7 @@ int sx_tree_attention(const sx_head_rows *q, const sx_head_rows *k_new, const sx
     const char *bad = shape_error(B, Hq, Hkv, D, max_new);
     SX_CHECK(bad == nullptr, bad, " (B = ", B, ", Hq = ", Hq, ", Hkv = ", Hkv, ", D = ", D, ", max_new = ", max_new, ")");
     SX_CHECK(cache->layers == 1, "layers = ", cache->layers, ": attention takes one layer's cache");
-    SX_CHECK(T >= 1 && T <= 0x7fffffff && T <= B * max_new, "T = ", T, " drafted tokens of ", B, " sequences of at most ", max_new);
+    SX_CHECK(T >= 1 && T <= 0x7fffffff, "T = ", T, " rows of drafted tokens");
     SX_CHECK(k_new->token <= (1 << 21) && v_new->token <= (1 << 21), "token strides of k_new and v_new up to 2^21 elements (", k_new->token, ", ", v_new->token, ")");
     SX_CHECK(mask_ld >= (max_new + 63) / 64, "mask_ld = ", mask_ld, " words a token for max_new = ", max_new);
     SX_CHECK(std::isfinite(scale) && scale > 0.f, "scale = ", scale, ", expected positive");

@@ -5,11 +5,12 @@ torch supplies device memory and the stream (torch.cuda.current_stream() unless 
 a libstrixite_amd.so kernel. Activations are torch.float32 (Act::F32) or torch.bfloat16 (Act::BF16, raw bits).
 """
 import ctypes
+import struct
 
 import torch
 
-from . import (ACT_BF16, ACT_F32, KV_BF16, KV_E4M3, MOE_F32, SCORE_SIGMOID, SCORE_SOFTMAX, SX_EINVAL, Fp8View, HeadRows,
-               KvCacheC, LogitCand, MtpPick, QView, SxError, check, lib)
+from . import (ACT_BF16, ACT_F32, KV_BF16, KV_E4M3, MOE_F32, SCORE_SIGMOID, SCORE_SOFTMAX, SX_EINVAL, Fp8View,
+               LogitCand, MtpPick, QView, SxError, check, lib)
 
 _c = ctypes.c_void_p
 
@@ -527,17 +528,22 @@ def linear_fp8(x, x_scale, w, out_act=ACT_BF16, y=None, stream=None):
     return y
 
 
+# sx_head_rows and sx_kv_cache as bytes: a quarter of the host time of building the ctypes structures
+_ROWS, _CACHE = struct.Struct("@P3q").pack, struct.Struct("@2Pi2f5q8qP2qPq").pack
+
+
 def _head_rows(name, t, heads, dim, layered=False):
     """The sx_head_rows of a BF16 tensor [T, heads, dim] (layered: [layers, T, heads, dim]); dims dense, other strides
     free."""
     if t.dtype != torch.bfloat16 or t.dim() != 3 + layered or t.shape[-2:] != (heads, dim) or t.stride(-1) != 1:
         _refuse(name, f"must be BF16 [tokens, {heads}, {dim}] with dense rows and is", t.dtype, tuple(t.shape), t.stride())
     s = t.stride()
-    return HeadRows(t.data_ptr(), s[-3], s[-2], s[0] if layered else 0)
+    return _ROWS(t.data_ptr(), s[-3], s[-2], s[0] if layered else 0)
 
 
 def _kv_cache(k, v, table, lens, k_scale, v_scale, layered=False):
-    """The sx_kv_cache of [pages, page, heads, dim] tensors (layered: [layers, ...]) with free strides."""
+    """The sx_kv_cache of [pages, page, heads, dim] tensors (layered: [layers, ...]) with free strides, and (sequences,
+    heads, dim, layers)."""
     dtype = k.dtype
     if dtype != torch.bfloat16 and dtype != torch.float8_e4m3fn or v.dtype != dtype:
         _refuse("the cache is BF16 or float8_e4m3fn, not", dtype, v.dtype)
@@ -549,10 +555,11 @@ def _kv_cache(k, v, table, lens, k_scale, v_scale, layered=False):
     B, P = table.shape
     _is("lens", lens, torch.int32, (B,))
     pages, page, heads, dim = shape[-4:]
-    return KvCacheC(k.data_ptr(), v.data_ptr(), KV_BF16 if dtype == torch.bfloat16 else KV_E4M3, k_scale, v_scale, pages,
-                    page, heads, dim, shape[0] if layered else 1, ks[-4], ks[-3], ks[-2], ks[0] if layered else 0, vs[-4],
-                    vs[-3], vs[-2], vs[0] if layered else 0, table.data_ptr(), table.stride(0) if B > 1 else P, P,
-                    lens.data_ptr(), B)
+    layers = shape[0] if layered else 1
+    c = _CACHE(k.data_ptr(), v.data_ptr(), KV_BF16 if dtype == torch.bfloat16 else KV_E4M3, k_scale, v_scale, pages, page,
+               heads, dim, layers, ks[-4], ks[-3], ks[-2], ks[0] if layered else 0, vs[-4], vs[-3], vs[-2],
+               vs[0] if layered else 0, table.data_ptr(), table.stride(0) if B > 1 else P, P, lens.data_ptr(), B)
+    return c, (B, heads, dim, layers)
 
 
 def tree_mask(parents):
@@ -599,10 +606,10 @@ def tree_attention(q, k_new, v_new, k_cache, v_cache, table, lens, starts, mask,
     T, Hq, D = q.shape
     Hkv = k_new.shape[1]
     _together(dev, (k_new, v_new, k_cache, v_cache, table, lens, starts, mask, out, lse, ws, err))
-    cache = _kv_cache(k_cache, v_cache, table, lens, k_scale, v_scale)
-    if (cache.heads, cache.dim) != (Hkv, D) or k_new.shape[0] != T or v_new.shape[0] != T:
+    cache, (B, heads, dim, _) = _kv_cache(k_cache, v_cache, table, lens, k_scale, v_scale)
+    if (heads, dim) != (Hkv, D) or k_new.shape[0] != T or v_new.shape[0] != T:
         _refuse("q", tuple(q.shape), "k_new", tuple(k_new.shape), "v_new", tuple(v_new.shape), "cache", tuple(k_cache.shape))
-    _is("starts", starts, torch.int32, (cache.batch + 1,))
+    _is("starts", starts, torch.int32, (B + 1,))
     if mask.dtype != torch.int64 or mask.dim() != 2 or mask.shape[0] != T or mask.stride(1) != 1 or mask.shape[1] * 64 < max_new:
         _refuse("mask must be int64 [T, ceil(max_new / 64)] with dense rows and is", mask.dtype, tuple(mask.shape))
     if out is None:
@@ -614,9 +621,8 @@ def tree_attention(q, k_new, v_new, k_cache, v_cache, table, lens, starts, mask,
     if ws is None:
         ws = tree_attention_workspace(q, k_new, starts, max_new)
     rq, rk, rv = _head_rows("q", q, Hq, D), _head_rows("k_new", k_new, Hkv, D), _head_rows("v_new", v_new, Hkv, D)
-    ro, ref = _head_rows("out", out, Hq, D), ctypes.byref
-    _run(dev, lib().sx_tree_attention, ref(rq), ref(rk), ref(rv), T, Hq, ref(cache), starts.data_ptr(), max_new,
-         mask.data_ptr(), mask.stride(0) if T > 1 else mask.shape[1], D ** -0.5 if scale is None else scale, ref(ro),
+    _run(dev, lib().sx_tree_attention, rq, rk, rv, T, Hq, cache, starts.data_ptr(), max_new, mask.data_ptr(),
+         mask.stride(0) if T > 1 else mask.shape[1], D ** -0.5 if scale is None else scale, _head_rows("out", out, Hq, D),
          _a(lse), ws.data_ptr(), ws.numel() * ws.element_size(), _a(err), stream=stream)
     return out, err
 
@@ -632,12 +638,11 @@ def kv_append(k_new, v_new, k_cache, v_cache, table, lens, starts, count, path=N
     if len(shape) not in (3, 4) or v_new.shape != shape:
         _refuse("k_new", tuple(shape), "and v_new", tuple(v_new.shape))
     _together(dev, (v_new, k_cache, v_cache, table, lens, starts, count, path, lens_out, err))
-    cache = _kv_cache(k_cache, v_cache, table, lens, k_scale, v_scale, layered)
-    T, B = shape[-3], cache.batch
-    if layered and shape[0] != cache.layers:
-        _refuse("k_new has", shape[0], "layers and the cache", cache.layers)
-    rk = _head_rows("k_new", k_new, cache.heads, cache.dim, layered)
-    rv = _head_rows("v_new", v_new, cache.heads, cache.dim, layered)
+    cache, (B, heads, dim, layers) = _kv_cache(k_cache, v_cache, table, lens, k_scale, v_scale, layered)
+    T = shape[-3]
+    if layered and shape[0] != layers:
+        _refuse("k_new has", shape[0], "layers and the cache", layers)
+    rk, rv = _head_rows("k_new", k_new, heads, dim, layered), _head_rows("v_new", v_new, heads, dim, layered)
     _is("starts", starts, torch.int32, (B + 1,))
     _is("count", count, torch.int32, (B,))
     ld = 0
@@ -654,8 +659,7 @@ def kv_append(k_new, v_new, k_cache, v_cache, table, lens, starts, count, path=N
         lens_out = torch.empty_like(lens)
     else:
         _is("lens_out", lens_out, torch.int32, (B,))
-    ref = ctypes.byref
-    _run(dev, lib().sx_kv_append, ref(rk), ref(rv), T, ref(cache), starts.data_ptr(), count.data_ptr(), max_count, _a(path),
+    _run(dev, lib().sx_kv_append, rk, rv, T, cache, starts.data_ptr(), count.data_ptr(), max_count, _a(path),
          ld, lens_out.data_ptr(), _a(err), stream=stream)
     return lens_out, err
 

@@ -13,9 +13,11 @@ class MoeVerifyLayer:
     runtime/qwen4exp.cpp:126-129). At verify width (the shapes kernels.verify_supported takes) three launches:
     router projection -> routing + gate_up + SwiGLU (the tails of its compute units' shares balanced through a sync
     buffer the layer owns) -> down + combine (the sequence qwen4exp.cpp:1139-1163 runs below kGroupedMinTokens). Otherwise (or fused=False): router projection -> moe_router + moe_group_routes -> grouped
-    gate_up with the SwiGLU epilogue -> grouped down + combine."""
+    gate_up with the SwiGLU epilogue -> grouped down + combine. routing (optional): a dict of moe_router_scored's score,
+    bias, groups, top_groups, group_best, renorm and factor; the layer then routes by those scores (grouped experts at
+    every width) and not by moe_router."""
 
-    def __init__(self, Wr, gate_up, down, E, k, max_tokens, act_dtype=torch.bfloat16, fused=True):
+    def __init__(self, Wr, gate_up, down, E, k, max_tokens, act_dtype=torch.bfloat16, fused=True, routing=None):
         self.Wr, self.gate_up, self.down, self.E, self.k = Wr, gate_up, down, E, k
         self.d = gate_up.K
         self.I = down.K
@@ -33,7 +35,8 @@ class MoeVerifyLayer:
         self.h_sums = torch.empty((M * A, (self.I + 15) // 16), dtype=torch.float32, device=dev)
         self.partial = torch.empty((M * A, self.d), dtype=torch.float32, device=dev)
         self.y = torch.empty((M, self.d), dtype=act_dtype, device=dev)
-        self.fused = fused and act_dtype == torch.bfloat16
+        self.routing = routing
+        self.fused = fused and act_dtype == torch.bfloat16 and routing is None
         # the gate_up pool's sync buffers, one per stream: launches on one buffer must run in order, which only one
         # stream guarantees
         self._syncs = {}
@@ -61,7 +64,11 @@ class MoeVerifyLayer:
             kx.verify_down(self.h[:M], self.down, self.ids[:M], self.coef[:M], self.E, y=self.y[:M],
                            expert_err=self.expert_err, h_sums=self.h_sums, plan=self.plan, stream=stream)
             return self.y[:M]
-        if M * self.k <= 2048:  # top-k + grouping in one launch
+        if self.routing is not None:
+            kx.moe_router_scored(self.logits[:M], self.E, self.k, ids=self.ids[:M], coef=self.coef[:M],
+                                 err=self.router_err, stream=stream, **self.routing)
+            kx.group_routes(self.ids[:M], self.E, ws=ws, err=self.expert_err, stream=stream)
+        elif M * self.k <= 2048:  # top-k + grouping in one launch
             kx.router_group(self.logits[:M], self.E, self.k, ws=ws, ids=self.ids[:M], coef=self.coef[:M],
                             router_err=self.router_err, expert_err=self.expert_err, stream=stream)
         else:
@@ -81,6 +88,59 @@ class MoeVerifyLayer:
         per_expert = (self.gate_up.nbytes() + self.down.nbytes()) // self.E
         act = M * self.d * self.y.element_size()
         return U, U * per_expert + self.Wr.numel() * 4 + 2 * act
+
+
+class VerifyAttention:
+    """The attention half of a verify layer: x + residual, RMS norm and FP8 codes in one launch -> FP8 query, key and value
+    projection -> attention of the drafted tokens over the layer's paged cache and each other -> output projection (a
+    q4 / q8 weight). norm_w BF16 [d]; qkv an Fp8Weight [(Hq + 2 Hkv) D, d], heads in that order; out_w a QWeight
+    [d, Hq D]. rotate (optional): called with the BF16 views q [T, Hq, D] and k [T, Hkv, D] after the projection, to turn
+    them by their positions in place. The drafted tokens' keys and values stay in k_new and v_new until the next forward:
+    what kv_append takes once the accepted path is known. Buffers for max_tokens are allocated here; a workspace is
+    kept for every stream that forward is called on."""
+
+    def __init__(self, norm_w, qkv, out_w, Hq, Hkv, D, max_tokens, max_seqs, max_new, eps=1e-6, rotate=None):
+        assert qkv.N == (Hq + 2 * Hkv) * D and out_w.K == Hq * D and out_w.N == qkv.K == norm_w.numel()
+        self.norm_w, self.qkv, self.out_w, self.Hq, self.Hkv, self.D = norm_w, qkv, out_w, Hq, Hkv, D
+        self.M, self.max_seqs, self.max_new, self.eps, self.rotate = max_tokens, max_seqs, max_new, eps, rotate
+        dev, d, M = norm_w.device, qkv.K, max_tokens
+        self._dev = dev
+        self.residual = torch.empty((M, d), dtype=torch.bfloat16, device=dev)
+        self.q8 = torch.empty((M, d), dtype=torch.float8_e4m3fn, device=dev)
+        self.scale = torch.empty((M, d // 128), dtype=torch.float32, device=dev)
+        self.heads = torch.empty((M, Hq + 2 * Hkv, D), dtype=torch.bfloat16, device=dev)
+        self.att = torch.empty((M, Hq, D), dtype=torch.bfloat16, device=dev)
+        self.y = torch.empty((M, d), dtype=torch.bfloat16, device=dev)
+        self.err = torch.zeros(4, dtype=torch.int32, device=dev)
+        self.k_new = self.v_new = None
+        self._ws = {}
+
+    def _ws_for(self, stream):
+        key = (stream or torch.cuda.current_stream(self._dev)).cuda_stream
+        if key not in self._ws:
+            with torch.cuda.device(self._dev):
+                n = kx.tree_attention_workspace_bytes(self.max_seqs, self.Hq, self.Hkv, self.D, self.max_new)
+            self._ws[key] = torch.empty((n + 7) // 8, dtype=torch.int64, device=self._dev)
+        return self._ws[key]
+
+    def forward(self, x, residual, k_cache, v_cache, table, lens, starts, mask, k_scale=1.0, v_scale=1.0, stream=None):
+        """x, residual (None in the first layer) BF16 [T, d]; the rest as tree_attention takes them. Returns (y [T, d],
+        the sum x + residual)."""
+        T = x.shape[0]
+        assert T <= self.M and lens.numel() <= self.max_seqs
+        res = None if residual is None else self.residual[:T]
+        kx.add_rms_norm_fp8(x, self.norm_w, self.eps, residual=residual, residual_out=res, q=self.q8[:T],
+                            scale=self.scale[:T], stream=stream)
+        heads = self.heads[:T]
+        kx.linear_fp8(self.q8[:T], self.scale[:T], self.qkv, y=heads.view(T, -1), stream=stream)
+        q, self.k_new, self.v_new = heads.split([self.Hq, self.Hkv, self.Hkv], dim=1)
+        if self.rotate is not None:
+            self.rotate(q, self.k_new)
+        kx.tree_attention(q, self.k_new, self.v_new, k_cache, v_cache, table, lens, starts, mask, self.max_new,
+                          k_scale=k_scale, v_scale=v_scale, out=self.att[:T], ws=self._ws_for(stream), err=self.err,
+                          stream=stream)
+        kx.linear(self.att[:T].view(T, -1), self.out_w, y=self.y[:T], stream=stream)
+        return self.y[:T], x if residual is None else res
 
 
 class VerifyTail:

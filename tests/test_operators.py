@@ -1,0 +1,190 @@
+"""The attention half of a verify layer and scored routing without a GPU: host checks of the C entries and of the Python
+functions, the mask builder, and the packed structures against the C layouts."""
+import ctypes
+import struct
+
+import pytest
+import torch
+
+import strixite_amd as sx
+from strixite_amd import kernels as kx
+
+
+@pytest.fixture(scope="module")
+def L():
+    return sx.lib()
+
+
+BUF = (ctypes.c_uint8 * (1 << 16))()
+BASE = (ctypes.addressof(BUF) + 255) // 256 * 256
+
+
+def P(off=0):
+    return ctypes.c_void_p(BASE + off)
+
+
+def refused(L, rc, text):
+    msg = L.sx_last_error().decode()
+    assert rc == sx.SX_EINVAL and text in msg, (rc, msg)
+
+
+def test_packed_structures_have_the_c_layout():
+    vals = (1, 2, 1, 0.5, 0.25, *range(5, 18), 77, 78, 79, 80, 81)
+    c = sx.KvCacheC.from_buffer_copy(kx._CACHE(*vals))
+    assert [getattr(c, f[0]) for f in c._fields_] == list(vals)
+    r = sx.HeadRows.from_buffer_copy(kx._ROWS(9, 8, 7, 6))
+    assert (r.p, r.token, r.head, r.layer) == (9, 8, 7, 6)
+    assert ctypes.sizeof(sx.KvCacheC) == struct.calcsize("@2Pi2f5q8qP2qPq")
+
+
+def test_tree_mask():
+    m = kx.tree_mask([[-1, 0, 0, 1], [-1], [-1, -1, 1]])
+    assert m.tolist() == [[0b1], [0b11], [0b101], [0b1011], [0b1], [0b1], [0b10], [0b110]]
+    chain = kx.tree_mask([list(range(-1, 69))])
+    assert chain.shape == (70, 2) and chain[63].tolist() == [-1, 0] and chain[69].tolist() == [-1, 0b111111]
+    with pytest.raises(ValueError):
+        kx.tree_mask([[0]])
+    with pytest.raises(ValueError):
+        kx.tree_mask([[-1, -2]])
+
+
+def cache(**kw):
+    d = dict(k=BASE, v=BASE + 4096, dtype=sx.KV_BF16, k_scale=1.0, v_scale=1.0, pages=4, page_size=16, heads=2, dim=64,
+             layers=1, k_page=2048, k_token=128, k_head=64, k_layer=0, v_page=2048, v_token=128, v_head=64, v_layer=0,
+             table=BASE + 8192, table_ld=2, pages_per_seq=2, lens=BASE + 8448, batch=2)
+    d.update(kw)
+    return sx.KvCacheC(**d)
+
+
+def attention(L, c=None, T=4, Hq=4, max_new=4, mask_ld=1, scale=0.1, q=(0, 256, 64), out=(16384, 256, 64), ws=1 << 40, ptr=None):
+    c = c or cache()
+    rows = lambda o, t, h: ctypes.byref(sx.HeadRows(BASE + o, t, h, 0))
+    return L.sx_tree_attention(rows(*q), rows(2048, 128, 64), rows(4096, 128, 64), T, Hq, ctypes.byref(c), P(9000 // 8 * 8),
+                               max_new, P(9216), mask_ld, scale, rows(*out), None, ptr or P(12288), ws, None, None)
+
+
+@pytest.mark.parametrize("kw,text", [
+    (dict(c=dict(page_size=24)), "power of two"), (dict(c=dict(page_size=8)), "power of two"),
+    (dict(c=dict(dim=96)), "head dimension"), (dict(Hq=5), "multiple of the key heads"), (dict(Hq=1), "multiple"),
+    (dict(max_new=257, mask_ld=5), "max_new"), (dict(max_new=0), "max_new"), (dict(max_new=65), "mask_ld"),
+    (dict(T=0), "T = 0"), (dict(scale=0.0), "scale"), (dict(scale=float("nan")), "scale"),
+    (dict(c=dict(batch=1025)), "1..1024"), (dict(c=dict(batch=0)), "batch"), (dict(c=dict(pages=0)), "pages"),
+    (dict(c=dict(k_token=130)), "multiples of 16 bytes"), (dict(c=dict(k=BASE + 8)), "16-byte aligned"),
+    (dict(c=dict(dtype=2)), "cache dtype"), (dict(c=dict(dtype=1, v_scale=0.0)), "v_scale"),
+    (dict(c=dict(table_ld=1)), "table_ld"), (dict(c=dict(k=None)), "null pointer"), (dict(c=dict(layers=2)), "one layer"),
+    (dict(c=dict(k_token=1 << 27)), "2^31"), (dict(q=(2, 256, 64)), "16-byte aligned"),
+    (dict(q=(0, 252, 64)), "multiples of 8"), (dict(q=(0, 256, 32)), "heads overlap"), (dict(out=(128, 256, 64)), "out overlaps"),
+    (dict(ws=1000), "workspace of 1000"), (dict(ptr=P(12296)), "16-byte aligned"),
+])
+def test_tree_attention_refusals(L, kw, text):
+    kw = dict(kw)
+    if isinstance(kw.get("c"), dict):
+        kw["c"] = cache(**kw["c"])
+    refused(L, attention(L, **kw), text)
+
+
+def append(L, c=None, T=4, max_count=2, path=None, path_ld=0, lens_out=9984, layer=0):
+    c = c or cache()
+    rows = lambda o: ctypes.byref(sx.HeadRows(BASE + o, 128, 64, layer))
+    return L.sx_kv_append(rows(0), rows(2048), T, ctypes.byref(c), P(9000 // 8 * 8), P(9216), max_count, path, path_ld,
+                          P(lens_out), None, None)
+
+
+@pytest.mark.parametrize("kw,text", [
+    (dict(T=0), "T = 0"), (dict(max_count=0), "max_count"), (dict(max_count=70000), "max_count"),
+    (dict(path=P(9600), path_ld=1), "path_ld"), (dict(lens_out=8448), "lens_out overlaps"), (dict(layer=12), "layer strides"),
+    (dict(c=dict(dim=60)), "dim = 60"), (dict(c=dict(page_size=17)), "power of two"),
+])
+def test_kv_append_refusals(L, kw, text):
+    kw = dict(kw)
+    if isinstance(kw.get("c"), dict):
+        kw["c"] = cache(**kw["c"])
+    refused(L, append(L, **kw), text)
+
+
+def norm(L, x=0, ldx=256, residual=None, weight=8192, M=4, K=256, eps=1e-6, w_add=0.0, residual_out=None, y=None, q=16384,
+         scale=20480, act=sx.ACT_BF16):
+    p = lambda o: None if o is None else P(o)
+    return L.sx_add_rms_norm_fp8(p(x), ldx, p(residual), p(weight), M, K, eps, w_add, p(residual_out), p(y), p(q), p(scale),
+                                 act, None)
+
+
+@pytest.mark.parametrize("kw,text", [
+    (dict(K=200), "multiple of 128"), (dict(K=32896, ldx=32896), "32768"), (dict(ldx=248), "ldx"), (dict(ldx=260), "ldx"),
+    (dict(M=0), "M = 0"), (dict(q=None, scale=None), "no output"), (dict(scale=None), "go together"),
+    (dict(residual=4096), "go together"), (dict(eps=-1.0), "eps"), (dict(w_add=float("inf")), "w_add"), (dict(act=7), "dtype 7"),
+    (dict(x=2), "aligned"), (dict(y=512), "overlaps an input"), (dict(q=256), "overlaps"), (dict(y=8192), "weight"),
+    (dict(residual=4096, residual_out=12288, y=12288), "y overlaps residual_out"),
+])
+def test_norm_refusals(L, kw, text):
+    refused(L, norm(L, **kw), text)
+
+
+def fp8(L, x=0, xs=4096, q=8192, ws=16384, y=20480, M=4, N=16, K=256, out=sx.ACT_BF16):
+    w = sx.Fp8View(BASE + q if q is not None else None, BASE + ws, N, K)
+    return L.sx_linear_fp8(P(x), P(xs), ctypes.byref(w), P(y), M, out, None)
+
+
+@pytest.mark.parametrize("kw,text", [
+    (dict(K=192), "multiple of 128"), (dict(K=1 << 17), "65536"), (dict(M=0), "M = 0"), (dict(N=0), "weight [0"),
+    (dict(out=5), "output dtype 5"), (dict(x=8), "aligned"), (dict(y=20481), "aligned"), (dict(y=0), "overlaps"),
+    (dict(y=16384), "overlaps"), (dict(q=None), "null pointer"), (dict(M=(1 << 22) + 1), "M ="),
+])
+def test_linear_fp8_refusals(L, kw, text):
+    refused(L, fp8(L, **kw), text)
+
+
+def route(L, ld=64, M=2, E=64, k=4, score=sx.SCORE_SIGMOID, groups=8, top=4, best=2, factor=1.0, shared=None, sld=1, sid=0,
+          act=sx.ACT_F32, ids=8192, coef=12288):
+    return L.sx_moe_router_scored(P(), ld, M, E, k, score, None, groups, top, best, 1, factor, shared, sld, sid, P(ids),
+                                  P(coef), act, None, None)
+
+
+@pytest.mark.parametrize("kw,text", [
+    (dict(E=1025, ld=1025), "E = 1025"), (dict(k=33), "k = 33"), (dict(k=0), "k = 0"), (dict(ld=63), "ld = 63"),
+    (dict(score=2), "unknown score"), (dict(groups=7), "divisor"), (dict(groups=128), "groups"), (dict(top=9), "top_groups"),
+    (dict(k=9, top=1), "chosen groups"), (dict(groups=64, best=2), "group_best"), (dict(best=3), "group_best"),
+    (dict(factor=float("inf")), "factor"), (dict(shared=P(), sid=-1), "shared_id"), (dict(shared=P(), sld=0), "shared_ld"),
+    (dict(act=3), "dtype 3"), (dict(M=0), "M = 0"), (dict(coef=8192), "same buffer"),
+])
+def test_scored_routing_refusals(L, kw, text):
+    refused(L, route(L, **kw), text)
+
+
+def test_workspace_bytes(L):
+    n = ctypes.c_size_t()
+    assert L.sx_tree_attention_workspace_bytes(3, 8, 2, 128, 6, ctypes.byref(n)) == 0 and n.value > 0
+    refused(L, L.sx_tree_attention_workspace_bytes(3, 8, 3, 128, 6, ctypes.byref(n)), "multiple of the key heads")
+    refused(L, L.sx_tree_attention_workspace_bytes(3, 8, 2, 100, 6, ctypes.byref(n)), "head dimension")
+
+
+def test_python_refuses_what_is_not_on_a_gpu_or_does_not_fit():
+    x = torch.zeros(2, 256, dtype=torch.bfloat16)
+    w = torch.ones(256, dtype=torch.bfloat16)
+    with pytest.raises(sx.SxError, match="not on a GPU"):
+        kx.add_rms_norm_fp8(x, w)
+    with pytest.raises(sx.SxError, match="multiple of 128"):
+        kx.add_rms_norm_fp8(x[:, :200], w[:200])
+    with pytest.raises(TypeError):
+        kx.add_rms_norm_fp8(x.half(), w)
+    with pytest.raises(sx.SxError, match="multiple of 128"):
+        kx.Fp8Weight(torch.zeros(16, 100, dtype=torch.float8_e4m3fn), torch.ones(1, 1))
+    with pytest.raises(sx.SxError, match="scale must be"):
+        kx.Fp8Weight(torch.zeros(200, 256, dtype=torch.float8_e4m3fn), torch.ones(1, 2))
+    weight = kx.Fp8Weight(torch.zeros(200, 256, dtype=torch.float8_e4m3fn), torch.ones(2, 2))
+    with pytest.raises(sx.SxError, match="not on a GPU"):
+        kx.linear_fp8(torch.zeros(2, 256, dtype=torch.float8_e4m3fn), torch.ones(2, 2), weight)
+    with pytest.raises(sx.SxError, match="not one of"):
+        kx.moe_router_scored(torch.zeros(2, 64), 64, 4, score="tanh")
+    with pytest.raises(sx.SxError, match="for E ="):
+        kx.moe_router_scored(torch.zeros(2, 64), 65, 4)
+    q = torch.zeros(3, 4, 64, dtype=torch.bfloat16)
+    kv = torch.zeros(3, 2, 64, dtype=torch.bfloat16)
+    c = torch.zeros(4, 16, 2, 64, dtype=torch.bfloat16)
+    i32 = lambda *v: torch.tensor(v, dtype=torch.int32)
+    table = i32(0, 1, 2, 3).view(2, 2)
+    mask = torch.ones(3, 1, dtype=torch.int64)
+    with pytest.raises(sx.SxError, match="not on a GPU"):
+        kx.tree_attention(q, kv, kv, c, c, table, i32(1, 2), i32(0, 1, 3), mask, 2)
+    with pytest.raises(sx.SxError, match="not on a GPU"):
+        kx.kv_append(kv, kv, c, c, table, i32(1, 2), i32(0, 1, 3), i32(1, 1), max_count=1)
