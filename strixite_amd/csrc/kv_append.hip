@@ -12,7 +12,7 @@ namespace {
 
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 
-constexpr int kThreads = 256;
+constexpr int kThreads = 256, kPieces = 4;
 
 struct Args {
     const uint16_t *kn, *vn;
@@ -61,22 +61,31 @@ __global__ void __launch_bounds__(kThreads) kv_append_kernel(const Args a) {
     const int node = a.path != nullptr ? a.path[b * a.path_ld + i] : i;
     const int pos = len + i, page = a.table[b * a.table_ld + (pos >> a.page_shift)];
     const int64_t tok = t0 + node, row = pos & ((1 << a.page_shift) - 1);
-    for (int u = blockIdx.x * kThreads + threadIdx.x; u < a.per_token; u += gridDim.x * kThreads) {
+    // kPieces pieces a thread, all read before the first is written
+    u32x4 w[kPieces];
+    uint8_t *dst[kPieces];
+    float unit[kPieces];
+#pragma unroll
+    for (int j = 0; j < kPieces; ++j) {
+        const int u = min((int)(blockIdx.x * kPieces + j) * kThreads + (int)threadIdx.x, a.per_token - 1);  // past the end: the last again
         const int d = u % a.dim8, r = u / a.dim8, h = r % a.heads, r2 = r / a.heads, layer = r2 >> 1;
         const bool is_v = r2 & 1;
-        const uint16_t *src = (is_v ? a.vn + layer * a.vn_l + tok * a.vn_t + h * a.vn_h : a.kn + layer * a.kn_l + tok * a.kn_t + h * a.kn_h) + d * 8;
-        uint8_t *dst = is_v ? a.vc + layer * a.vc_l + page * a.vc_p + row * a.vc_t + h * a.vc_h
-                            : a.kc + layer * a.kc_l + page * a.kc_p + row * a.kc_t + h * a.kc_h;
-        const u32x4 w = *reinterpret_cast<const u32x4 *>(src);
+        w[j] = *reinterpret_cast<const u32x4 *>((is_v ? a.vn + layer * a.vn_l + tok * a.vn_t + h * a.vn_h : a.kn + layer * a.kn_l + tok * a.kn_t + h * a.kn_h) + d * 8);
+        dst[j] = (is_v ? a.vc + layer * a.vc_l + page * a.vc_p + row * a.vc_t + h * a.vc_h
+                       : a.kc + layer * a.kc_l + page * a.kc_p + row * a.kc_t + h * a.kc_h) + d * (F8 ? 8 : 16);
+        unit[j] = is_v ? a.v_scale : a.k_scale;
+    }
+#pragma unroll
+    for (int j = 0; j < kPieces; ++j) {
+        if ((int)(blockIdx.x * kPieces + j) * kThreads + (int)threadIdx.x >= a.per_token) break;
         if constexpr (!F8) {
-            *reinterpret_cast<u32x4 *>(dst + d * 16) = w;
+            *reinterpret_cast<u32x4 *>(dst[j]) = w[j];
         } else {
-            const float s = is_v ? a.v_scale : a.k_scale;
             uint32_t o[2] = {0, 0};
 #pragma unroll
-            for (int j = 0; j < 4; ++j)
-                o[j >> 1] = pack2_e4m3(bf16_to_f32(w[j] & 0xFFFFu) / s, __uint_as_float(w[j] & 0xFFFF0000u) / s, o[j >> 1], j & 1);
-            *reinterpret_cast<uint2 *>(dst + d * 8) = uint2{o[0], o[1]};
+            for (int k = 0; k < 4; ++k)
+                o[k >> 1] = pack2_e4m3(bf16_to_f32(w[j][k] & 0xFFFFu) / unit[j], __uint_as_float(w[j][k] & 0xFFFF0000u) / unit[j], o[k >> 1], k & 1);
+            *reinterpret_cast<uint2 *>(dst[j]) = uint2{o[0], o[1]};
         }
     }
 }
@@ -117,7 +126,7 @@ extern "C" int sx_kv_append(const sx_head_rows *k_new, const sx_head_rows *v_new
     a.page_shift = __builtin_ctzll((uint64_t)cache->page_size), a.heads = (int32_t)cache->heads;
     a.dim8 = (int32_t)(cache->dim / 8), a.per_token = (int32_t)(2 * cache->layers * cache->heads * a.dim8);
     a.max_count = (int32_t)max_count, a.k_scale = cache->k_scale, a.v_scale = cache->v_scale;
-    const dim3 grid((unsigned)((a.per_token + kThreads - 1) / kThreads), (unsigned)max_count, (unsigned)cache->batch);
+    const dim3 grid((unsigned)((a.per_token + kThreads * kPieces - 1) / (kThreads * kPieces)), (unsigned)max_count, (unsigned)cache->batch);
     if (cache->dtype == SX_KV_E4M3) kv_append_kernel<true><<<grid, kThreads, 0, stream_of(stream)>>>(a);
     else kv_append_kernel<false><<<grid, kThreads, 0, stream_of(stream)>>>(a);
     SX_LAUNCHED("kv_append B=", cache->batch, " layers=", cache->layers);

@@ -159,24 +159,19 @@ void go(const Args &a, hipStream_t s) {
     norm_fp8_kernel<T, TPR, NV><<<(unsigned)((a.M + rows - 1) / rows), TPR < 256 ? 256 : TPR, 0, s>>>(a);
 }
 
-// A row of up to 4096 features goes to one wave where there are rows for every wave of the chip (no barrier, four rows
-// a block), else to a block of 256, whose loads of one row are in flight together.
+// One run of 8 a thread, so that a row's loads are all in flight at once, up to 8192 features; rows of few features share
+// a block. (2048 rows of 2560 in us: a wave a row and five runs a lane 16.9, 256 threads 15.0, 512 14.7; 6 of 4096: 512
+// threads 4.1, 256 and two runs 5.2.)
 template <typename T>
 void launch(const Args &a, hipStream_t s) {
     const int n8 = a.K / 8;
-    if (a.M >= 4 * device_cus() && n8 <= 64 * 8) {
-        if (n8 <= 64 * 2) go<T, 64, 2>(a, s);
-        else if (n8 <= 64 * 5) go<T, 64, 5>(a, s);
-        else go<T, 64, 8>(a, s);
-    } else if (n8 <= 256) {
-        go<T, 256, 1>(a, s);
-    } else if (n8 <= 256 * 2) {
-        go<T, 256, 2>(a, s);
-    } else if (n8 <= 1024 * 2) {
-        go<T, 1024, 2>(a, s);
-    } else {
-        go<T, 1024, 4>(a, s);
-    }
+    if (n8 <= 64) go<T, 64, 1>(a, s);
+    else if (n8 <= 128) go<T, 128, 1>(a, s);
+    else if (n8 <= 256) go<T, 256, 1>(a, s);
+    else if (n8 <= 512) go<T, 512, 1>(a, s);
+    else if (n8 <= 1024) go<T, 1024, 1>(a, s);
+    else if (n8 <= 2048) go<T, 1024, 2>(a, s);
+    else go<T, 1024, 4>(a, s);
 }
 
 }  // namespace

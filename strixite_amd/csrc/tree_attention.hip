@@ -37,7 +37,6 @@ typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 
 constexpr int kStep = 32, kMaxSeqs = 1024, kMaxNew = 256, kJoinThreads = 256;
-constexpr int kHalfStage = 32768;  // bytes of keys (of values) a stage
 constexpr float kNegInf = -INFINITY;
 
 struct Args {
@@ -55,15 +54,15 @@ struct Args {
     int64_t kc_h, vc_h;                        // head,
     int32_t kc_t, vc_t;                        // token (a page's span fits 31 bits)
     int64_t out_t, out_h, lse_t, table_ld, mask_ld;
-    int32_t B, T, G, P, pages, page_shift, max_new, nb;
+    int32_t B, T, G, P, pages, page_shift, max_new, nb, heads;
     float scale, k_scale, v_scale;  // scale: softmax scale * log2(e)
 };
 
 // How a cache row of D values lies in a stage and in the operands.
-template <int D, bool F8>
+template <int D, bool F8, int HS>  // HS: bytes of keys (of values) a stage
 struct Lay {
     static constexpr int E = F8 ? 1 : 2, RB = D * E;                       // bytes of a value, of a row
-    static constexpr int KEYS = kHalfStage / RB < 256 ? kHalfStage / RB : 256;  // keys a stage
+    static constexpr int KEYS = HS / RB < 256 ? HS / RB : 256;  // keys a stage
     static constexpr int CH = RB / 16;                                     // 16-byte chunks a row
     static constexpr int VEC = D / 16, PE = F8 ? VEC : (VEC < 8 ? VEC : 8);  // dims a lane of a value row; in one piece
     static constexpr int VB = PE * E;                                      // bytes of a piece: 4, 8 or 16
@@ -358,16 +357,16 @@ __device__ __forceinline__ int seq_at(const uint32_t *pre, int B, uint32_t u) { 
     return lo;
 }
 
-template <int D, int NT, int WR, int WK, bool F8>
-__global__ void __launch_bounds__(64 * WR * WK) tree_attn_kernel(const Args a) {
-    using C_ = Lay<D, F8>;     // cached stages
-    using N_ = Lay<D, false>;  // drafted stages
+template <int D, int NT, int WR, int WK, int HS, bool F8>
+__global__ void __launch_bounds__(64 * WR * WK, HS < 32768 || WR * WK > 4 ? 2 : 1) tree_attn_kernel(const Args a) {
+    using C_ = Lay<D, F8, HS>;     // cached stages
+    using N_ = Lay<D, false, HS>;  // drafted stages
     // BF16 values meet P in two terms where there are few rows and products to spare (at 16 rows and 65,536 keys the time
     // is the same), else in one: the output's error is its own rounding, or 1.4 times that
     constexpr int kWaves = WR * WK, ROWS = 16 * NT * WR, KEYS = C_::KEYS, FRESH = N_::KEYS, VEC = D / 16, BF16_TERMS = ROWS <= 64 ? 2 : 1;
-    static_assert(WK == 1 || 16 * NT * D * 4 <= kHalfStage, "a wave's O fits a stage's keys");
+    static_assert(WK / 2 * WR <= 4, "an array for each pair of waves that meet");
     // one array a stage and operand, so that the wait-count pass tells a stage's loads apart from the other's
-    __shared__ __attribute__((aligned(1024))) uint8_t k0[kHalfStage], k1[kHalfStage], v0[kHalfStage], v1[kHalfStage];
+    __shared__ __attribute__((aligned(1024))) uint8_t k0[HS], k1[HS], v0[HS], v1[HS];
     __shared__ List ls;
     __shared__ float merge_ml[kWaves][16 * NT][2];
     scan_units<ROWS, KEYS, FRESH, 64 * kWaves>(a, ls);
@@ -568,28 +567,39 @@ __global__ void __launch_bounds__(64 * WR * WK) tree_attn_kernel(const Args a) {
         // The stages' arrays hold them (every wave is past its last stage once all pass the barrier). ----
 #pragma unroll
         for (int half = WK / 2; half >= 1; half >>= 1) {
-            __syncthreads();
-            if (wk >= half && wk < 2 * half) {
-                float *dst = reinterpret_cast<float *>((wk - half) * WR + wr == 0 ? k0 : (wk - half) * WR + wr == 1 ? k1 : (wk - half) * WR + wr == 2 ? v0 : v1);
+            const bool gives = wk >= half && wk < 2 * half, takes = wk < half;
+            const int place = (gives ? wk - half : wk) * WR + wr;  // whose array: one for each pair of waves
+            float *at = reinterpret_cast<float *>(place == 0 ? k0 : place == 1 ? k1 : place == 2 ? v0 : v1);
+            float f1[NT], f2[NT];
+            if (gives && g == 0) {
 #pragma unroll
-                for (int t = 0; t < NT; ++t) {
-#pragma unroll
-                    for (int e = 0; e < VEC; ++e) *reinterpret_cast<f32x4 *>(dst + ((t * VEC + e) * 64 + lane) * 4) = acc.o[t][e];
-                    if (g == 0) merge_ml[wave][t * 16 + n16][0] = acc.m[t], merge_ml[wave][t * 16 + n16][1] = acc.l[t];
-                }
+                for (int t = 0; t < NT; ++t) merge_ml[wave][t * 16 + n16][0] = acc.m[t], merge_ml[wave][t * 16 + n16][1] = acc.l[t];
             }
-            __syncthreads();
-            if (wk < half) {
-                const float *src = reinterpret_cast<const float *>(wk * WR + wr == 0 ? k0 : wk * WR + wr == 1 ? k1 : wk * WR + wr == 2 ? v0 : v1);
+            constexpr int kParts = (16 * NT * D * 4 + HS - 1) / HS, kEach = VEC / kParts;  // O in as many parts as arrays hold
+#pragma unroll
+            for (int part = 0; part < kParts; ++part) {
+                __syncthreads();
+                if (gives) {
+#pragma unroll
+                    for (int t = 0; t < NT; ++t)
+#pragma unroll
+                        for (int e = 0; e < kEach; ++e)
+                            *reinterpret_cast<f32x4 *>(at + ((t * kEach + e) * 64 + lane) * 4) = acc.o[t][part * kEach + e];
+                }
+                __syncthreads();
+                if (!takes) continue;
 #pragma unroll
                 for (int t = 0; t < NT; ++t) {
-                    const float m2 = merge_ml[wave + half * WR][t * 16 + n16][0], l2 = merge_ml[wave + half * WR][t * 16 + n16][1];
-                    const float m = fmaxf(acc.m[t], m2), base = m == kNegInf ? 0.f : m;
-                    const float f1 = __builtin_amdgcn_exp2f(acc.m[t] - base), f2 = __builtin_amdgcn_exp2f(m2 - base);
-                    acc.m[t] = m, acc.l[t] = acc.l[t] * f1 + l2 * f2;
+                    if (part == 0) {
+                        const float m2 = merge_ml[wave + half * WR][t * 16 + n16][0], l2 = merge_ml[wave + half * WR][t * 16 + n16][1];
+                        const float m = fmaxf(acc.m[t], m2), base = m == kNegInf ? 0.f : m;
+                        f1[t] = __builtin_amdgcn_exp2f(acc.m[t] - base), f2[t] = __builtin_amdgcn_exp2f(m2 - base);
+                        acc.m[t] = m, acc.l[t] = acc.l[t] * f1[t] + l2 * f2[t];
+                    }
 #pragma unroll
-                    for (int e = 0; e < VEC; ++e)
-                        acc.o[t][e] = acc.o[t][e] * f1 + *reinterpret_cast<const f32x4 *>(src + ((t * VEC + e) * 64 + lane) * 4) * f2;
+                    for (int e = 0; e < kEach; ++e)
+                        acc.o[t][part * kEach + e] = acc.o[t][part * kEach + e] * f1[t] +
+                                                     *reinterpret_cast<const f32x4 *>(at + ((t * kEach + e) * 64 + lane) * 4) * f2[t];
                 }
             }
         }
@@ -640,14 +650,16 @@ __global__ void __launch_bounds__(64 * WR * WK) tree_attn_kernel(const Args a) {
     }
 }
 
-// The partials of a row, and the rows of sequences that could not be read (NaN). A block takes one row: D / 4 lanes hold
-// four dims each, the block's kJoinThreads / (D / 4) slices of lanes the partials in turn; the slices meet in LDS in order.
-template <int D, int ROWS, int KEYS, int FRESH>
+// The partials of a row, and the rows of sequences that could not be read (NaN). D / 4 lanes hold four dims each of one
+// row. With few partials a row (many short sequences) every such group of lanes takes a row of its own, heads side by
+// side; with many, all groups of a block take one row's partials in turn and meet in LDS in order (SHARE).
+template <int D, int ROWS, int KEYS, int FRESH, bool SHARE>
 __global__ void __launch_bounds__(kJoinThreads) tree_attn_join_kernel(const Args a) {
-    constexpr int kLanes = D / 4, kSlices = kJoinThreads / kLanes;
-    __shared__ f32x4 sums[kSlices][kLanes];
-    __shared__ float ml[kSlices][2];
-    const int tok = blockIdx.x, head = blockIdx.y, kvh = head / a.G, h = head % a.G, tid = threadIdx.x, ln = tid % kLanes, sl = tid / kLanes;
+    constexpr int kLanes = D / 4, kGroups = kJoinThreads / kLanes, kStride = SHARE ? kGroups : 1;
+    __shared__ f32x4 sums[SHARE ? kGroups : 1][kLanes];
+    __shared__ float ml[SHARE ? kGroups : 1][2];
+    const int ln = threadIdx.x % kLanes, grp = threadIdx.x / kLanes;
+    const int tok = blockIdx.x, head = SHARE ? blockIdx.y : blockIdx.y * kGroups + grp, kvh = head / a.G, h = head % a.G;
     int lo = 0, hi = a.B - 1;
     while (lo < hi) {  // the sequence of this token
         const int mid = (lo + hi) >> 1;
@@ -655,7 +667,7 @@ __global__ void __launch_bounds__(kJoinThreads) tree_attn_join_kernel(const Args
         else hi = mid;
     }
     const int b = lo;
-    if (tok < a.starts[b] || tok >= a.starts[b + 1]) return;  // a row behind the last sequence
+    if (head >= a.heads || tok < a.starts[b] || tok >= a.starts[b + 1]) return;  // a row behind the last sequence
     const Seq sq = seq_of<ROWS, KEYS, FRESH>(a, b);
     f32x4 o = {0.f, 0.f, 0.f, 0.f};
     float m = kNegInf, l = 0.f;
@@ -666,7 +678,7 @@ __global__ void __launch_bounds__(kJoinThreads) tree_attn_join_kernel(const Args
         const int i0 = (int)((((uint64_t)u0 + 1) * nb - 1) / U), i1 = (int)(((uint64_t)u1 * nb - 1) / U);
         if (i0 == i1) return;  // written whole
 #pragma unroll 4
-        for (int i = i0 + sl; i <= i1; i += kSlices) {
+        for (int i = i0 + (SHARE ? grp : 0); i <= i1; i += kStride) {
             // only the first block of the pair can hold it as its run's last one
             const bool second = i == i0 && (uint32_t)((uint64_t)U * i / nb) < u0;
             const int64_t row = (((int64_t)kvh * a.nb + i) * 2 + (second ? 1 : 0)) * ROWS + (r - rg * ROWS);
@@ -679,14 +691,16 @@ __global__ void __launch_bounds__(kJoinThreads) tree_attn_join_kernel(const Args
     } else {
         l = qnan();
     }
-    sums[sl][ln] = o;
-    if (ln == 0) ml[sl][0] = m, ml[sl][1] = l;
-    __syncthreads();
-    if (sl != 0) return;
-    for (int i = 1; i < kSlices; ++i) {
-        const float m2 = ml[i][0], l2 = ml[i][1], mx = fmaxf(m, m2), base = mx == kNegInf ? 0.f : mx;
-        const float f1 = __builtin_amdgcn_exp2f(m - base), f2 = __builtin_amdgcn_exp2f(m2 - base);
-        o = o * f1 + sums[i][ln] * f2, l = l * f1 + l2 * f2, m = mx;
+    if constexpr (SHARE) {
+        sums[grp][ln] = o;
+        if (ln == 0) ml[grp][0] = m, ml[grp][1] = l;
+        __syncthreads();
+        if (grp != 0) return;
+        for (int i = 1; i < kGroups; ++i) {
+            const float m2 = ml[i][0], l2 = ml[i][1], mx = fmaxf(m, m2), base = mx == kNegInf ? 0.f : mx;
+            const float f1 = __builtin_amdgcn_exp2f(m - base), f2 = __builtin_amdgcn_exp2f(m2 - base);
+            o = o * f1 + sums[i][ln] * f2, l = l * f1 + l2 * f2, m = mx;
+        }
     }
     const float inv = l == 0.f ? 0.f : 1.0f / l;
     *reinterpret_cast<uint2 *>(a.out + tok * a.out_t + head * a.out_h + ln * 4) =
@@ -694,10 +708,14 @@ __global__ void __launch_bounds__(kJoinThreads) tree_attn_join_kernel(const Args
     if (a.lse != nullptr && ln == 0) a.lse[tok * a.lse_t + head] = log_sum(m, l);
 }
 
-// The rows a block holds - NT tiles of 16 a wave, WR waves side by side on the same keys - and the blocks a key head,
-// one a compute unit. The smallest tile that takes all rows of a sequence is taken, so that the cache is read once; a
-// call with more rows than the largest tile takes further row groups, which read the cache again. Above 32 rows eight
-// waves, two a SIMD: one's exponentials overlap the other's products.
+// The rows a block holds - NT tiles of 16 a wave, WR waves side by side on the same keys - and the blocks a key head. The
+// smallest tile that takes all rows of a sequence is taken, so that the cache is read once; a call with more rows than
+// the largest tile takes further row groups, which read the cache again.
+// Up to 32 rows a block of four waves a compute unit keeps 64 KB of loads in flight and has little else to do. Above, a
+// step's chain of products and exponentials is as long as its loads, and two blocks of four waves with half the stage a
+// compute unit, out of step with each other, beat one of eight (65,536 keys, 8 key heads of 128, us: 48 rows 67.4 / 74.2,
+// 64 68.4 / 75.9, 96 78.5 / 82.8, 128 83.2 / 89.2, 192 alike; FP8 at 131,072: 48 rows 81 / 96, 128 121 / 134). 256 rows, and
+// more than 64 at D = 256, take a block of eight waves (D = 256, 128 rows: 103 / 114).
 struct Plan {
     int nt, wr, nb;
     int64_t rows() const { return 16 * nt * wr; }
@@ -712,7 +730,8 @@ Plan plan_of(int64_t D, int64_t G, int64_t Hkv, int64_t max_new) {
     } else {
         p.nt = rows <= 64 ? 2 : rows <= 96 ? 3 : rows <= 128 ? 2 : rows <= 192 ? 3 : 2, p.wr = rows <= 96 ? 2 : rows <= 192 ? 4 : 8;
     }
-    p.nb = (int)std::max<int64_t>(1, (int64_t)device_cus() / Hkv);
+    const int per_cu = D == 256 ? (p.wr == 4 && p.nt == 1 ? 2 : 1) : p.wr == 2 || p.wr == 4 ? 2 : 1;
+    p.nb = (int)std::max<int64_t>(1, (int64_t)device_cus() * per_cu / Hkv);
     return p;
 }
 
@@ -734,29 +753,30 @@ Space space_of(const Plan &p, int64_t B, int64_t Hkv, int64_t D) {
     return s;
 }
 
-template <int D, int NT, int WR, int WK>
+template <int D, int NT, int WR, int WK, int HS, bool F8>
+void launch_type(const Args &a, int64_t Hkv, hipStream_t stream) {
+    constexpr int ROWS = 16 * NT * WR, KEYS = Lay<D, F8, HS>::KEYS, FRESH = Lay<D, false, HS>::KEYS, kGroups = kJoinThreads / (D / 4);
+    tree_attn_kernel<D, NT, WR, WK, HS, F8><<<dim3((unsigned)a.nb, (unsigned)Hkv), 64 * WR * WK, 0, stream>>>(a);
+    // about nb / B + 1 partials a row (32 sequences, 64 blocks a head, 361 x 32 rows: 23.4 us shared, 8.0 not)
+    if (a.nb > 8 * a.B) tree_attn_join_kernel<D, ROWS, KEYS, FRESH, true><<<dim3((unsigned)a.T, (unsigned)a.heads), kJoinThreads, 0, stream>>>(a);
+    else tree_attn_join_kernel<D, ROWS, KEYS, FRESH, false><<<dim3((unsigned)a.T, (unsigned)((a.heads + kGroups - 1) / kGroups)), kJoinThreads, 0, stream>>>(a);
+}
+
+template <int D, int NT, int WR, int WK, int HS = 32768>
 void launch(const Args &a, int64_t Hkv, bool f8, hipStream_t stream) {
-    constexpr int ROWS = 16 * NT * WR, kThreads = 64 * WR * WK;
-    const dim3 grid((unsigned)a.nb, (unsigned)Hkv), join((unsigned)a.T, (unsigned)(Hkv * a.G));
-    if (f8) {
-        tree_attn_kernel<D, NT, WR, WK, true><<<grid, kThreads, 0, stream>>>(a);
-        tree_attn_join_kernel<D, ROWS, Lay<D, true>::KEYS, Lay<D, false>::KEYS><<<join, kJoinThreads, 0, stream>>>(a);
-    } else {
-        tree_attn_kernel<D, NT, WR, WK, false><<<grid, kThreads, 0, stream>>>(a);
-        tree_attn_join_kernel<D, ROWS, Lay<D, false>::KEYS, Lay<D, false>::KEYS><<<join, kJoinThreads, 0, stream>>>(a);
-    }
+    f8 ? launch_type<D, NT, WR, WK, HS, true>(a, Hkv, stream) : launch_type<D, NT, WR, WK, HS, false>(a, Hkv, stream);
 }
 
 template <int D>
 void launch_rows(const Plan &p, const Args &a, int64_t Hkv, bool f8, hipStream_t s) {
     if constexpr (D == 256) {
         if (p.wr == 2) launch<D, 1, 2, 2>(a, Hkv, f8, s);
-        else if (p.wr == 4) p.nt == 1 ? launch<D, 1, 4, 2>(a, Hkv, f8, s) : launch<D, 2, 4, 2>(a, Hkv, f8, s);
+        else if (p.wr == 4) p.nt == 1 ? launch<D, 1, 4, 1, 16384>(a, Hkv, f8, s) : launch<D, 2, 4, 2>(a, Hkv, f8, s);
         else launch<D, 2, 8, 1>(a, Hkv, f8, s);
     } else {
         if (p.wr == 1) p.nt == 1 ? launch<D, 1, 1, 4>(a, Hkv, f8, s) : launch<D, 2, 1, 4>(a, Hkv, f8, s);
-        else if (p.wr == 2) p.nt == 2 ? launch<D, 2, 2, 4>(a, Hkv, f8, s) : launch<D, 3, 2, 4>(a, Hkv, f8, s);
-        else if (p.wr == 4) p.nt == 2 ? launch<D, 2, 4, 2>(a, Hkv, f8, s) : launch<D, 3, 4, 2>(a, Hkv, f8, s);
+        else if (p.wr == 2) p.nt == 2 ? launch<D, 2, 2, 2, 16384>(a, Hkv, f8, s) : launch<D, 3, 2, 2, 16384>(a, Hkv, f8, s);
+        else if (p.wr == 4) p.nt == 2 ? launch<D, 2, 4, 1, 16384>(a, Hkv, f8, s) : launch<D, 3, 4, 1, 16384>(a, Hkv, f8, s);
         else launch<D, 2, 8, 1>(a, Hkv, f8, s);
     }
 }
@@ -828,7 +848,7 @@ int sx_tree_attention(const sx_head_rows *q, const sx_head_rows *k_new, const sx
     a.prefix = reinterpret_cast<uint32_t *>(w + sp.prefix);
     a.B = (int32_t)B, a.T = (int32_t)T, a.G = (int32_t)(Hq / Hkv), a.P = (int32_t)cache->pages_per_seq;
     a.pages = (int32_t)cache->pages, a.page_shift = __builtin_ctzll((uint64_t)cache->page_size);
-    a.max_new = (int32_t)max_new, a.nb = p.nb;
+    a.max_new = (int32_t)max_new, a.nb = p.nb, a.heads = (int32_t)Hq;
     a.scale = scale * 1.4426950408889634f, a.k_scale = cache->k_scale, a.v_scale = cache->v_scale;
     const bool f8 = cache->dtype == SX_KV_E4M3;
     hipStream_t s = stream_of(stream);
