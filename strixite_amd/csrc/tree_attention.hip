@@ -21,6 +21,10 @@
 // (they are on the device: a captured graph replays with other ones). A block whose run covers a pair of sequence and
 // row group whole writes its rows; else it leaves a partial (at most two a block: its run's first and last pair) that
 // tree_attn_join_kernel adds up in the order of the list, so the result does not depend on the schedule.
+//
+// Measured (both kernels): 131,072 keys, 8 key heads of 128, 4 rows each: 112 us, 4.8 TB/s (5.5 beyond the first 65,536; the
+// rest is launch, first stage, merge and join: 15 us). Bound by the loads up to 64 rows, by a step's chain of products and
+// exponentials above (256 rows: 123 us for 65,536 keys, 0.56 PFLOP/s).
 #include "common.hpp"
 #include "kv_cache.hpp"
 #include "route_impl.hpp"
