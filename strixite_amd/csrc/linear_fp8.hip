@@ -58,7 +58,7 @@ __device__ __forceinline__ f32x4 block_products(i32x8 a, i32x8 b) {
 
 // ---------------- few tokens: the weight's bytes are the cost ----------------
 // A block takes 16 NT weight rows and 16 MT tokens; its 8 waves split K block by block, straight from memory into the
-// operands, and their sums meet in LDS in wave order. 12288 x 4096, M = 6: 13.9 us, 3.6 TB/s with the launch.
+// operands, and their sums meet in LDS in wave order. 12288 x 4096, M = 6: 14.0 us, 3.6 TB/s with the launch.
 __device__ __forceinline__ void store4(float *p, f32x4 v) { *reinterpret_cast<f32x4 *>(p) = v; }
 __device__ __forceinline__ void store4(uint16_t *p, f32x4 v) {
     *reinterpret_cast<uint2 *>(p) = uint2{f32_to_bf16(v[0]) | (f32_to_bf16(v[1]) << 16), f32_to_bf16(v[2]) | (f32_to_bf16(v[3]) << 16)};

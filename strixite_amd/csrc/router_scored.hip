@@ -8,7 +8,7 @@
 // belongs to P = 64 / ceil_pow2(groups) neighbouring lanes (one group: all 64), lane `sub` of them holding experts gi *
 // per + sub + P i, so a group's best two are a butterfly over P lanes. The top k as in the plain router: a threshold
 // that k lanes' maxima reach, by a search over the keys' high words, then the few keys above it ranked against each
-// other. 8.4 us from 6 tokens to 2048: one wave's chain of FP64 exponentials, shuffles and LDS reads, not its work.
+// other. 8.4 us for 6 tokens and for 2048: one wave's chain, not the amount of work.
 #include "common.hpp"
 #include "route_impl.hpp"
 

@@ -6,7 +6,7 @@
 //
 // The cost is the cache: 2 L Hkv D values read once, against 4 R L D flops for the R = tokens * (query heads a key
 // head) rows that share them. A block therefore takes all rows of a sequence and key head (up to its tile of rows) and
-// streams 64 KB stages of keys and values (32 KB each) through LDS, two stages deep: the loads of the next stage are
+// streams stages of keys and values (32 KB each; 16 KB where two blocks share a compute unit) through LDS, two deep: the loads of the next stage are
 // asynchronous and in flight, without registers, for as long as this stage is worked on.
 //   S^T = K Q^T: 16 keys are the A operand, Q^T stays in registers as the B operand; a lane gets 4 keys of a 16-key
 //   tile for one row.
@@ -22,9 +22,9 @@
 // row group whole writes its rows; else it leaves a partial (at most two a block: its run's first and last pair) that
 // tree_attn_join_kernel adds up in the order of the list, so the result does not depend on the schedule.
 //
-// Measured (both kernels): 131,072 keys, 8 key heads of 128, 4 rows each: 112 us, 4.8 TB/s (5.5 beyond the first 65,536; the
-// rest is launch, first stage, merge and join: 15 us). Bound by the loads up to 64 rows, by a step's chain of products and
-// exponentials above (256 rows: 123 us for 65,536 keys, 0.56 PFLOP/s).
+// Measured (both kernels): 131,072 keys, 8 key heads of 128, 4 rows each: 112 to 115 us, 4.7 TB/s; 65,536 keys: 65 us, so
+// 5.4 to 5.8 TB/s beyond them and 15 to 19 us that do not grow with the keys. Up to 64 rows the time hardly moves (71 us for
+// 65,536 keys), above it grows with the rows (96: 79 us; 256: 123 us, 0.56 PFLOP/s).
 #include "common.hpp"
 #include "kv_cache.hpp"
 #include "route_impl.hpp"
