@@ -95,7 +95,7 @@ class VerifyAttention:
     projection -> attention of the drafted tokens over the layer's paged cache and each other -> output projection (a
     q4 / q8 weight). norm_w BF16 [d]; qkv an Fp8Weight [(Hq + 2 Hkv) D, d], heads in that order; out_w a QWeight
     [d, Hq D]. rotate (optional): called with the BF16 views q [T, Hq, D] and k [T, Hkv, D] after the projection, to turn
-    them by their positions in place. The drafted tokens' keys and values stay in k_new and v_new until the next forward:
+    them by their positions in place, forward's stream being the current one. The drafted tokens' keys and values stay in k_new and v_new until the next forward:
     what kv_append takes once the accepted path is known. Buffers for max_tokens are allocated here; a workspace is
     kept for every stream that forward is called on."""
 
@@ -135,7 +135,8 @@ class VerifyAttention:
         kx.linear_fp8(self.q8[:T], self.scale[:T], self.qkv, y=heads.view(T, -1), stream=stream)
         q, self.k_new, self.v_new = heads.split([self.Hq, self.Hkv, self.Hkv], dim=1)
         if self.rotate is not None:
-            self.rotate(q, self.k_new)
+            with torch.cuda.stream(stream):  # the projection and the attention run there (None: the current one)
+                self.rotate(q, self.k_new)
         kx.tree_attention(q, self.k_new, self.v_new, k_cache, v_cache, table, lens, starts, mask, self.max_new,
                           k_scale=k_scale, v_scale=v_scale, out=self.att[:T], ws=self._ws_for(stream), err=self.err,
                           stream=stream)

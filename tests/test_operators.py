@@ -188,3 +188,34 @@ def test_python_refuses_what_is_not_on_a_gpu_or_does_not_fit():
         kx.tree_attention(q, kv, kv, c, c, table, i32(1, 2), i32(0, 1, 3), mask, 2)
     with pytest.raises(sx.SxError, match="not on a GPU"):
         kx.kv_append(kv, kv, c, c, table, i32(1, 2), i32(0, 1, 3), i32(1, 1), max_count=1)
+
+
+def test_verify_attention_rotates_on_the_stream_of_its_kernels(monkeypatch):
+    from contextlib import contextmanager
+
+    from strixite_amd import verify
+    current, seen = ["its caller's"], []
+
+    @contextmanager
+    def on(stream):
+        before, current[0] = current[0], stream or current[0]
+        yield
+        current[0] = before
+
+    for f in ("add_rms_norm_fp8", "linear_fp8", "tree_attention", "linear"):
+        monkeypatch.setattr(verify.kx, f, lambda *a, stream=None, **kw: seen.append(stream or current[0]))
+    monkeypatch.setattr(torch.cuda, "stream", on)
+    monkeypatch.setattr(verify.VerifyAttention, "_ws_for", lambda self, stream: None)
+
+    class W:
+        N, K = 128, 128
+
+    class Qkv:
+        N, K = 384, 128
+    att = verify.VerifyAttention(torch.ones(128), Qkv, W, 2, 2, 64, 4, 1, 4, rotate=lambda q, k: seen.append(current[0]))
+    x, lens = torch.zeros(4, 128), torch.zeros(1, dtype=torch.int32)
+    att.forward(x, None, None, None, None, lens, None, None, stream="its own")
+    assert seen == ["its own"] * 5
+    seen.clear()
+    att.forward(x, None, None, None, None, lens, None, None)
+    assert seen == ["its caller's"] * 5
