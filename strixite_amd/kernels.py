@@ -443,6 +443,11 @@ def _together(dev, tensors):
             _refuse("tensors on", t.device, "and on GPU", dev, "in one call")
 
 
+def _is_err(err):
+    if err is not None and (err.dtype != torch.int32 or err.numel() < 4 or not err.is_contiguous()):
+        _refuse("err must be a contiguous int32 [4] and is", err.dtype, tuple(err.shape), err.stride())
+
+
 def _run(dev, f, *args, stream=None):
     """f(*args, stream) on GPU dev, whichever is current."""
     if dev != torch.cuda.current_device():
@@ -619,7 +624,11 @@ def tree_attention(q, k_new, v_new, k_cache, v_cache, table, lens, starts, mask,
     if lse is not None:
         _is("lse", lse, torch.float32, (T, Hq))
     if ws is None:
-        ws = tree_attention_workspace(q, k_new, starts, max_new)
+        with torch.cuda.stream(stream):  # from its pool (None: the current one's): the buffer ends with this call, the kernels later
+            ws = tree_attention_workspace(q, k_new, starts, max_new)
+    elif not ws.is_contiguous():
+        _refuse("ws must be contiguous and has strides", ws.stride())
+    _is_err(err)
     rq, rk, rv = _head_rows("q", q, Hq, D), _head_rows("k_new", k_new, Hkv, D), _head_rows("v_new", v_new, Hkv, D)
     _run(dev, lib().sx_tree_attention, rq, rk, rv, T, Hq, cache, starts.data_ptr(), max_new, mask.data_ptr(),
          mask.stride(0) if T > 1 else mask.shape[1], D ** -0.5 if scale is None else scale, _head_rows("out", out, Hq, D),
@@ -659,6 +668,7 @@ def kv_append(k_new, v_new, k_cache, v_cache, table, lens, starts, count, path=N
         lens_out = torch.empty_like(lens)
     else:
         _is("lens_out", lens_out, torch.int32, (B,))
+    _is_err(err)
     _run(dev, lib().sx_kv_append, rk, rv, T, cache, starts.data_ptr(), count.data_ptr(), max_count, _a(path),
          ld, lens_out.data_ptr(), _a(err), stream=stream)
     return lens_out, err
@@ -693,6 +703,7 @@ def moe_router_scored(logits, E, k, score="sigmoid", bias=None, groups=1, top_gr
         coef = torch.empty(shape, dtype=torch.float32, device=logits.device)
     else:
         _is("coef", coef, torch.float32, shape)
+    _is_err(err)
     _run(dev, lib().sx_moe_router_scored, logits.data_ptr(), logits.stride(0) if M > 1 else logits.shape[1], M, E, k,
          SCORES[score], _a(bias), groups, top_groups if groups > 1 else 1, group_best if groups > 1 else 1, int(renorm),
          factor, _a(shared), shared_ld, shared_id, ids.data_ptr(), coef.data_ptr(), act, _a(err), stream=stream)

@@ -219,3 +219,48 @@ def test_verify_attention_rotates_on_the_stream_of_its_kernels(monkeypatch):
     seen.clear()
     att.forward(x, None, None, None, None, lens, None, None)
     assert seen == ["its caller's"] * 5
+
+
+def test_workspace_and_err_have_to_hold_what_is_written(monkeypatch):
+    """Before anything reaches the library: what the strides or the size of a buffer would let a kernel write beside it."""
+    def unreached(*a, **kw):
+        raise AssertionError("the call went on")
+    monkeypatch.setattr(kx, "_together", lambda dev, tensors: None)
+    monkeypatch.setattr(kx, "_run", unreached)
+    q, kv = torch.zeros(3, 4, 64, dtype=torch.bfloat16), torch.zeros(3, 2, 64, dtype=torch.bfloat16)
+    c = torch.zeros(4, 16, 2, 64, dtype=torch.bfloat16)
+    i32 = lambda *v: torch.tensor(v, dtype=torch.int32)
+    table, mask, ws = i32(0, 1, 2, 3).view(2, 2), torch.ones(3, 1, dtype=torch.int64), torch.zeros(64, dtype=torch.int64)
+    att = lambda **kw: kx.tree_attention(q, kv, kv, c, c, table, i32(1, 2), i32(0, 1, 3), mask, 2, **{"ws": ws, **kw})
+    with pytest.raises(sx.SxError, match="ws must be contiguous"):
+        att(ws=ws[::2])
+    for err in (i32(0), torch.zeros(4), torch.zeros(8, dtype=torch.int32)[::2]):
+        with pytest.raises(sx.SxError, match="err must be"):
+            att(err=err)
+        with pytest.raises(sx.SxError, match="err must be"):
+            kx.kv_append(kv, kv, c, c, table, i32(1, 2), i32(0, 1, 3), i32(1, 1), max_count=1, err=err)
+        with pytest.raises(sx.SxError, match="err must be"):
+            kx.moe_router_scored(torch.zeros(2, 64), 64, 4, err=err)
+
+
+def test_a_workspace_made_for_a_call_belongs_to_the_stream_of_the_call(monkeypatch):
+    from contextlib import contextmanager
+    current, made = ["its caller's"], []
+
+    @contextmanager
+    def on(stream):
+        before, current[0] = current[0], stream or current[0]
+        yield
+        current[0] = before
+
+    monkeypatch.setattr(torch.cuda, "stream", on)
+    monkeypatch.setattr(kx, "_together", lambda dev, tensors: None)
+    monkeypatch.setattr(kx, "_run", lambda *a, **kw: None)
+    monkeypatch.setattr(kx, "tree_attention_workspace", lambda *a: made.append(current[0]) or torch.zeros(8, dtype=torch.int64))
+    q, kv = torch.zeros(3, 4, 64, dtype=torch.bfloat16), torch.zeros(3, 2, 64, dtype=torch.bfloat16)
+    c = torch.zeros(4, 16, 2, 64, dtype=torch.bfloat16)
+    i32 = lambda *v: torch.tensor(v, dtype=torch.int32)
+    for stream in ("its own", None):
+        kx.tree_attention(q, kv, kv, c, c, i32(0, 1, 2, 3).view(2, 2), i32(1, 2), i32(0, 1, 3),
+                          torch.ones(3, 1, dtype=torch.int64), 2, stream=stream)
+    assert made == ["its own", "its caller's"]
