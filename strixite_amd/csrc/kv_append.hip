@@ -111,7 +111,13 @@ extern "C" int sx_kv_append(const sx_head_rows *k_new, const sx_head_rows *v_new
     SX_CHECK(T >= 1 && T <= 0x7fffffff, "T = ", T);
     SX_CHECK(max_count >= 1 && max_count <= 65535, "max_count = ", max_count, ", expected 1..65535");
     SX_CHECK(path == nullptr || path_ld >= max_count, "path_ld = ", path_ld, " < max_count = ", max_count);
-    SX_CHECK(lens_out == nullptr || apart(lens_out, cache->batch * 4, cache->lens, cache->batch * 4), "lens_out overlaps lens");
+    // one block writes a sequence's lens_out while its others still read these
+    const int64_t n4 = cache->batch * 4;
+    SX_CHECK(lens_out == nullptr ||
+                 (apart(lens_out, n4, cache->lens, n4) && apart(lens_out, n4, starts, n4 + 4) && apart(lens_out, n4, count, n4) &&
+                  apart(lens_out, n4, cache->table, 4 * ((cache->batch - 1) * cache->table_ld + cache->pages_per_seq)) &&
+                  (path == nullptr || apart(lens_out, n4, path, 4 * ((cache->batch - 1) * path_ld + max_count)))),
+             "lens_out overlaps lens, starts, count, path or the table");
     SX_CHECK(cache->layers * cache->heads * cache->dim <= 0x3fffffff, "layers * heads * dim too large");
     const int e = kv_bytes(*cache);
     Args a;

@@ -264,3 +264,8 @@ def test_a_workspace_made_for_a_call_belongs_to_the_stream_of_the_call(monkeypat
         kx.tree_attention(q, kv, kv, c, c, i32(0, 1, 2, 3).view(2, 2), i32(1, 2), i32(0, 1, 3),
                           torch.ones(3, 1, dtype=torch.int64), 2, stream=stream)
     assert made == ["its own", "its caller's"]
+
+
+@pytest.mark.parametrize("lens_out", [8192, 8196, 9000 // 8 * 8, 9004, 9216, 9220, 9600, 9612])
+def test_append_refuses_lens_out_in_what_its_blocks_read(L, lens_out):
+    refused(L, append(L, path=P(9600), path_ld=2, lens_out=lens_out), "lens_out overlaps")
