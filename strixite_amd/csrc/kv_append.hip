@@ -109,6 +109,10 @@ extern "C" int sx_kv_append(const sx_head_rows *k_new, const sx_head_rows *v_new
     SX_CHECK(k_new->layer >= 0 && v_new->layer >= 0 && k_new->layer % 8 == 0 && v_new->layer % 8 == 0,
              "layer strides must be multiples of 8 elements (", k_new->layer, ", ", v_new->layer, ")");
     SX_CHECK(T >= 1 && T <= 0x7fffffff, "T = ", T);
+    const sx_kv_cache &c = *cache;
+    SX_CHECK(rows_apart(c.dim, {{c.layers, c.k_layer}, {c.pages, c.k_page}, {c.page_size, c.k_token}, {c.heads, c.k_head}}) &&
+                 rows_apart(c.dim, {{c.layers, c.v_layer}, {c.pages, c.v_page}, {c.page_size, c.v_token}, {c.heads, c.v_head}}),
+             "rows of the cache share memory");
     SX_CHECK(max_count >= 1 && max_count <= 65535, "max_count = ", max_count, ", expected 1..65535");
     SX_CHECK(path == nullptr || path_ld >= max_count, "path_ld = ", path_ld, " < max_count = ", max_count);
     // one block writes a sequence's lens_out while its others still read these

@@ -3,9 +3,25 @@
 #pragma once
 #include "common.hpp"
 
+#include <algorithm>
 #include <cmath>
+#include <utility>
 
 namespace sx {
+
+// Whether rows of dim values at these (count, element stride) steps share no memory: each stride passes what the
+// smaller ones cover. Asked of what a kernel writes; what it reads may be expanded.
+inline bool rows_apart(int64_t dim, std::initializer_list<std::pair<int64_t, int64_t>> steps) {
+    std::pair<int64_t, int64_t> s[4];
+    const int n = (int)(std::copy_if(steps.begin(), steps.end(), s, [](const auto &x) { return x.first > 1; }) - s);
+    std::sort(s, s + n, [](const auto &x, const auto &y) { return x.second < y.second; });
+    __int128 covered = dim;
+    for (int i = 0; i < n; ++i) {
+        if (s[i].second < covered) return false;
+        covered += (__int128)(s[i].first - 1) * s[i].second;
+    }
+    return true;
+}
 
 inline int kv_bytes(const sx_kv_cache &c) { return c.dtype == SX_KV_E4M3 ? 1 : 2; }
 

@@ -823,6 +823,7 @@ int sx_tree_attention(const sx_head_rows *q, const sx_head_rows *k_new, const sx
     if (why.empty()) why = head_rows_error(*v_new, "v_new", Hkv, D);
     if (why.empty()) why = head_rows_error(*out, "out", Hq, D);
     SX_CHECK(why.empty(), why);
+    SX_CHECK(rows_apart(D, {{T, out->token}, {Hq, out->head}}), "rows of out share memory (strides: token ", out->token, ", head ", out->head, ")");
     SX_CHECK(aligned(mask, 8) && aligned(ws, 16), "mask must be 8-byte and the workspace 16-byte aligned");
     const int64_t out_bytes = head_rows_bytes(*out, T, Hq, D);
     SX_CHECK(apart(out->p, out_bytes, q->p, head_rows_bytes(*q, T, Hq, D)) &&
@@ -832,6 +833,8 @@ int sx_tree_attention(const sx_head_rows *q, const sx_head_rows *k_new, const sx
     const Plan p = plan_of(D, Hq / Hkv, Hkv, max_new);
     const Space sp = space_of(p, B, Hkv, D);
     SX_CHECK(ws_bytes >= (size_t)sp.bytes, "workspace of ", ws_bytes, " bytes, needs ", sp.bytes);
+    SX_CHECK(apart(ws, sp.bytes, out->p, out_bytes) && (lse == nullptr || (apart(lse, 4 * T * Hq, ws, sp.bytes) && apart(lse, 4 * T * Hq, out->p, out_bytes))),
+             "out, lse and the workspace overlap");
     const int64_t most = cache->pages_per_seq * cache->page_size / 64 + 6;  // stages hold 64 keys or more
     const int64_t groups = (max_new * (Hq / Hkv) + p.rows() - 1) / p.rows();
     SX_CHECK(B * groups * most < ((int64_t)1 << 31), "more than 2^31 units of work (B = ", B, ", pages a sequence ", cache->pages_per_seq, ")");

@@ -269,3 +269,31 @@ def test_a_workspace_made_for_a_call_belongs_to_the_stream_of_the_call(monkeypat
 @pytest.mark.parametrize("lens_out", [8192, 8196, 9000 // 8 * 8, 9004, 9216, 9220, 9600, 9612])
 def test_append_refuses_lens_out_in_what_its_blocks_read(L, lens_out):
     refused(L, append(L, path=P(9600), path_ld=2, lens_out=lens_out), "lens_out overlaps")
+
+
+@pytest.mark.parametrize("strides", [(0, 64), (192, 64), (64, 128), (64, 192)])
+def test_attention_refuses_an_output_whose_rows_share_memory(L, strides):
+    refused(L, attention(L, ws=100, out=(16384, *strides)), "rows of out share memory")
+
+
+@pytest.mark.parametrize("strides", [(256, 64), (64, 256), (512, 128), (128, 512), (128, 64 + 448)])
+def test_attention_takes_an_output_whose_rows_are_apart(L, strides):
+    refused(L, attention(L, ws=100, out=(16384, *strides)), "workspace of 100")  # the next check
+
+
+def test_attention_refuses_a_workspace_in_its_output(L):
+    n = ctypes.c_size_t()
+    assert L.sx_tree_attention_workspace_bytes(2, 4, 2, 64, 4, ctypes.byref(n)) == sx.SX_OK
+    refused(L, attention(L, ws=n.value, ptr=P(16384 + 256)), "workspace overlap")
+
+
+@pytest.mark.parametrize("kw", [dict(k_page=0), dict(v_page=2040), dict(k_token=64), dict(v_token=0), dict(layers=2),
+                                dict(layers=2, k_layer=8192, v_layer=2048)])
+def test_append_refuses_a_cache_whose_rows_share_memory(L, kw):
+    refused(L, append(L, c=cache(**kw)), "rows of the cache share memory")
+
+
+@pytest.mark.parametrize("kw", [dict(layers=2, k_layer=8192, v_layer=8192), dict(k_page=2048, k_token=64, k_head=1024),
+                                dict(layers=2, k_layer=2048, k_page=4096, v_layer=2048, v_page=4096), dict(pages=1, k_page=0)])
+def test_append_takes_layers_heads_and_pages_in_any_order(L, kw):
+    refused(L, append(L, c=cache(**kw), max_count=0), "max_count = 0")  # the next check
