@@ -215,8 +215,10 @@ extern "C" int sx_moe_router_scored(const void *logits, int64_t ld, int64_t M, i
         SX_CHECK(shared_ld >= 1, "shared_ld = ", shared_ld, ", expected >= 1");
         SX_CHECK(shared_id >= 0, "shared_id = ", shared_id, ", expected >= 0 (its expert row block)");
     }
-    SX_CHECK((const void *)ids != (const void *)coef, "ids and coef are the same buffer");
     SX_CHECK(act == SX_ACT_F32 || act == SX_ACT_BF16, "unsupported activation dtype ", act);
+    const int64_t slots = 4 * M * (k + (shared_logit != nullptr ? 1 : 0)), read = ((M - 1) * ld + E) * act_bytes(act);
+    SX_CHECK(apart(ids, slots, coef, slots), "ids and coef are the same buffer or overlap");
+    SX_CHECK(apart(ids, slots, logits, read) && apart(coef, slots, logits, read), "ids or coef overlap the logits");
     int P = 64;
     while (P * groups > 64) P >>= 1;
     const int per = (int)(E / groups), need = (per + P - 1) / P;

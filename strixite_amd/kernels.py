@@ -695,6 +695,8 @@ def moe_router_scored(logits, E, k, score="sigmoid", bias=None, groups=1, top_gr
         _is("bias", bias, torch.float32, (E,))
     if shared is not None and (shared.dtype != logits.dtype or shared.shape[0] != M):
         _refuse("shared is", shared.dtype, tuple(shared.shape), "for logits", logits.dtype, tuple(logits.shape))
+    if shared is not None and (shared.storage_offset() + (M - 1) * shared_ld + 1) * shared.element_size() > shared.untyped_storage().nbytes():
+        _refuse("shared_ld =", shared_ld, "leads past the shared logits", tuple(shared.shape), shared.stride())
     if ids is None:
         ids = torch.empty(shape, dtype=torch.int32, device=logits.device)
     else:

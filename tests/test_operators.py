@@ -297,3 +297,23 @@ def test_append_refuses_a_cache_whose_rows_share_memory(L, kw):
                                 dict(layers=2, k_layer=2048, k_page=4096, v_layer=2048, v_page=4096), dict(pages=1, k_page=0)])
 def test_append_takes_layers_heads_and_pages_in_any_order(L, kw):
     refused(L, append(L, c=cache(**kw), max_count=0), "max_count = 0")  # the next check
+
+
+@pytest.mark.parametrize("kw,text", [(dict(coef=8192 + 28), "same buffer or overlap"), (dict(ids=508), "overlap the logits"),
+                                     (dict(coef=0), "overlap the logits")])
+def test_routing_refuses_outputs_in_its_logits_or_each_other(L, kw, text):
+    refused(L, route(L, **kw), text)
+
+
+def test_routing_refuses_a_shared_stride_past_the_tensor(monkeypatch):
+    calls = []
+    monkeypatch.setattr(kx, "_together", lambda dev, tensors: None)
+    monkeypatch.setattr(kx, "_run", lambda *a, **kw: calls.append(a))
+    logits = torch.zeros(3, 65)
+    go = lambda shared, ld: kx.moe_router_scored(logits, 64, 4, shared=shared, shared_ld=ld, shared_id=64)
+    with pytest.raises(sx.SxError, match="leads past"):
+        go(torch.zeros(3), 65)
+    with pytest.raises(sx.SxError, match="leads past"):
+        go(logits[:, 64], 66)
+    go(torch.zeros(3), 1), go(logits[:, 64], 65)
+    assert len(calls) == 2
