@@ -687,3 +687,51 @@ def test_a_verify_layer_with_its_attention():
         torch.cuda.synchronize()
         assert all(torch.equal(a, w) for a, w in zip(got, want))
         assert torch.equal(b.kc, after_k) and torch.equal(b.vc, after_v)
+
+
+def test_two_graphs_with_one_workspace_replayed_in_turn():
+    """Nothing in a workspace outlives a call: graphs of different shapes that share one, on one stream, with eager work
+    between the replays, give what each gives alone."""
+    a, b = Batch(128, 8, 2, 32, [700, 3], [5, 1], seed=61), Batch(128, 8, 2, 16, [90], [24], seed=62)
+    want = [x.run()[0].clone() for x in (a, b)]
+    n = max(kx.tree_attention_workspace_bytes(x.lens.numel(), 8, 2, 128, x.max_new) for x in (a, b))
+    ws = torch.empty((n + 7) // 8, dtype=torch.int64, device="cuda")
+    outs, graphs = [], []
+    for x in (a, b):
+        outs.append(torch.empty_like(x.q))
+        graphs.append(torch.cuda.CUDAGraph())
+        torch.cuda.synchronize()
+        with torch.cuda.graph(graphs[-1]):
+            x.run(ws=ws, out=outs[-1])
+    for turn in range(4):
+        for i in ((0, 1) if turn % 2 else (1, 0)):
+            outs[i].zero_()
+            ws.fill_(-1)
+            graphs[i].replay()
+            assert torch.equal(outs[i], want[i]), (turn, i)
+
+
+def test_verify_attention_with_a_rotation_on_another_stream():
+    from strixite_amd import synthetic as syn
+    from strixite_amd.verify import VerifyAttention
+    d, Hq, Hkv, D = 512, 4, 2, 128
+    b = Batch(D, Hq, Hkv, 16, [37], [6], seed=63)
+    mask = kx.tree_mask([list(range(-1, 5))]).cuda()
+    qkv = fp8_case(1, (Hq + 2 * Hkv) * D, d, seed=64)[2]
+    qkv.scale.mul_(0.01)
+    streams = []
+
+    def rotate(q, k):
+        streams.append(torch.cuda.current_stream().cuda_stream)
+        q.neg_(), k.mul_(0.5)  # exact
+    att = VerifyAttention(torch.ones(d, dtype=BF, device="cuda"), qkv, syn.qweight(8, d, Hq * D, 64, seed=65), Hq, Hkv, D, 8, 2, 8,
+                          rotate=rotate)
+    x = syn.activations(6, d, seed=66)
+    want = att.forward(x, None, b.kc, b.vc, b.table, b.lens, b.starts, mask)[0].clone()
+    heads = att.heads[:6].clone()
+    torch.cuda.synchronize()
+    s = torch.cuda.Stream()
+    got = att.forward(x, None, b.kc, b.vc, b.table, b.lens, b.starts, mask, stream=s)[0]
+    s.synchronize()
+    assert streams[1] == s.cuda_stream != streams[0]
+    assert torch.equal(att.heads[:6], heads) and torch.equal(got, want)
