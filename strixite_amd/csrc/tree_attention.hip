@@ -151,22 +151,24 @@ struct Acc {
 };
 
 // s: raw scores (-inf where a row does not see the key) of keys {4g + i, 16 + 4g + i}; leaves p = 2^(s ks - m) in s. m is
-// a row's maximum at the last time that a score went more than 2^8 over it: sums and O grow by that factor at most, far
-// inside FP32, and O is rescaled a few times a run and not at every new maximum.
-template <int D, int NT>
+// a row's maximum, less kLift, at the last time that a p went over 2^kTop: sums and O grow by that factor at most, far
+// inside FP32, and O is rescaled a few times a run and not at every new maximum. Where P becomes FP16 (F16) the lift puts
+// the largest p at FP16's upper end: FP16 takes 2^-25 at most from a key, against a sum of 2^7 and more, so many keys far
+// under a row's maximum count down to 2^-32 of it (65,536 keys a wave: 2^-16 of the largest value is lost at most).
+template <int D, int NT, bool F16>
 __device__ __forceinline__ void softmax_step(Acc<D, NT> &acc, float (&s)[NT][8], float ks) {
-    constexpr float kSlack = 8.f;
+    constexpr float kLift = F16 ? 7.f : 0.f, kTop = F16 ? 15.f : 8.f;
     float mx[NT];
     bool up = false;
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
         mx[t] = fmaxf(fmaxf(fmaxf(s[t][0], s[t][1]), fmaxf(s[t][2], s[t][3])), fmaxf(fmaxf(s[t][4], s[t][5]), fmaxf(s[t][6], s[t][7])));
-        up |= mx[t] * ks > acc.m[t] + kSlack;
+        up |= mx[t] * ks > acc.m[t] + kTop;
     }
     if (__any(up)) {
 #pragma unroll
         for (int t = 0; t < NT; ++t) {
-            const float m = fmaxf(acc.m[t], over_g(mx[t], true) * ks);
+            const float m = fmaxf(acc.m[t], over_g(mx[t], true) * ks - kLift);
             const float c = __builtin_amdgcn_exp2f(acc.m[t] - (m == kNegInf ? 0.f : m));
             acc.l[t] *= c, acc.m[t] = m;
 #pragma unroll
@@ -225,7 +227,7 @@ __device__ __forceinline__ void scores(F frag, const bf16x8 (&q)[NT][D / 32], fl
 }
 
 // P as the B operand. BF16 values: TERMS BF16 numbers that add up to p (one: 2^-9 of it is lost, two: 2^-17). E4M3 values
-// are exact in FP16 too, so there one FP16 number does (2^-12; what falls under 2^-25 is lost, against sums of 1 and more).
+// are exact in FP16 too, so there one FP16 number does (2^-12; small ones: see softmax_step).
 template <int NT, int TERMS, bool F16>
 __device__ __forceinline__ void as_operand(const float (&p)[NT][8], float factor, bool scaled, u32x4 (&b)[TERMS][NT]) {
 #pragma unroll
@@ -508,7 +510,7 @@ __global__ void __launch_bounds__(64 * WR * WK, HS < 32768 || WR * WK > 4 ? 2 : 
                             for (int t = 0; t < NT; ++t) s[t][i] = kNegInf;
                         }
                 }
-                softmax_step<D, NT>(acc, s, ks);
+                softmax_step<D, NT, F8>(acc, s, ks);
                 constexpr int TERMS = E4 ? 1 : BF16_TERMS;
                 u32x4 p[TERMS][NT];
                 as_operand<NT, TERMS, E4>(s, inv_v, F8 && NEW, p);

@@ -735,3 +735,45 @@ def test_verify_attention_with_a_rotation_on_another_stream():
     s.synchronize()
     assert streams[1] == s.cuda_stream != streams[0]
     assert torch.equal(att.heads[:6], heads) and torch.equal(got, want)
+
+
+# ---------------- attention: FP16 P, many sequences ----------------
+
+@pytest.mark.parametrize("D,G,news", [(64, 2, 1), (128, 4, 6), (128, 8, 8), (128, 8, 12), (128, 8, 24), (64, 8, 32), (256, 8, 3),
+                                      (256, 8, 8), (256, 8, 16), (256, 8, 32)])
+def test_attention_fp8_keeps_a_long_tail_under_a_peak(D, G, news):
+    """The first key 2^26 over the 2047 others of its sequence, which hold all of the values: in units of the peak each is
+    under FP16's smallest number, together they are the output. FP16 P loses 2^-25 a key on a sum of 2^7: keys 2^-32 max |v|;
+    the rest as above. Enough sequences and heads that a block takes whole ones."""
+    print(f"attention fp8 tail D={D} G={G} news={news}", flush=True)
+    page, L, B, Hkv = 128, 2048, 64, 8
+    pages = L // page
+    kc, vc = (torch.zeros(pages, page, Hkv, D, device="cuda") for _ in range(2))
+    vc[:] = 0.5 + torch.rand(Hkv, D, device="cuda", generator=gen(D))
+    kc[0, 0, :, 0], vc[0, 0] = 18.0, 0.0
+    T = B * news
+    q = torch.zeros(T, Hkv * G, D, dtype=BF, device="cuda")
+    q[:, :, 0] = 1.0
+    new = torch.ones(T, Hkv, D, dtype=BF, device="cuda")
+    lse = torch.empty(T, Hkv * G, device="cuda")
+    table = torch.arange(pages, dtype=torch.int32, device="cuda").repeat(B, 1)
+    out, _ = kx.tree_attention(q, new, new, kc.to(F8), vc.to(F8), table, i32([L] * B), i32(list(range(0, T + 1, news))),
+                               torch.zeros(T, 1, dtype=torch.int64, device="cuda"), news, scale=1.0, lse=lse)
+    v = vc[0, 1].to(F8).double().repeat_interleave(G, 0)
+    tail = (L - 1) * math.exp(-18.0)
+    want = v * tail / (1 + tail)
+    e = (D + 4) * U32 * 18.0
+    tol = U16 * want + (2.0 ** -11 + 2 * e + (L + 64) * U32) * want + L * 2.0 ** -32 * v.max()
+    assert ((out.double() - want).abs() <= tol).all(), float(((out.double() - want).abs() / tol).max())
+    assert ((lse.double() - (18.0 + math.log1p(tail))).abs() <= e + (L + 64) * U32 + 4 * U32 * 18.0).all()
+
+
+@pytest.mark.parametrize("D,Hq,news", [(128, 4, [6]), (128, 8, [12]), (64, 8, [24]), (256, 8, [6]), (256, 8, [20])])
+def test_attention_fp8_rising_maxima(D, Hq, news):
+    """Scores that rise by tens through a long FP8 cache: FP16 P never leaves its range."""
+    print(f"attention fp8 rising D={D} Hq={Hq} news={news}", flush=True)
+    b = Batch(D, Hq, 1, 64, [9001], news, "fp8", seed=6, amp=3.0)
+    k = b.kc.view(-1, 1, D)
+    b.kc = (k.float() * torch.linspace(0.1, 2.0, k.shape[0], device="cuda").view(-1, 1, 1)).to(F8).view_as(b.kc)
+    b.table = torch.arange(b.table.numel(), dtype=torch.int32, device="cuda").view_as(b.table)
+    check(b, b.run()[0])
