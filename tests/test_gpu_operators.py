@@ -777,3 +777,91 @@ def test_attention_fp8_rising_maxima(D, Hq, news):
     b.kc = (k.float() * torch.linspace(0.1, 2.0, k.shape[0], device="cuda").view(-1, 1, 1)).to(F8).view_as(b.kc)
     b.table = torch.arange(b.table.numel(), dtype=torch.int32, device="cuda").view_as(b.table)
     check(b, b.run()[0])
+
+
+def many(D, Hq, Hkv, B, most, cache, seed):
+    """B sequences of up to 90 cached and `most` drafted tokens, some of them with none of either."""
+    g = torch.Generator().manual_seed(seed)
+    lens = torch.randint(0, 91, (B,), generator=g)
+    news = torch.randint(0, 4, (B,), generator=g)
+    lens[torch.rand(B, generator=g) < 0.1] = 0
+    lens[B // 2], news[B // 2], news[B // 3], news[-1] = 90, most, most, 1
+    return Batch(D, Hq, Hkv, 16, lens.tolist(), news.tolist(), cache, seed=seed, mask="any")
+
+
+@pytest.mark.parametrize("cache", ["bf16", "fp8"])
+@pytest.mark.parametrize("D,Hq,Hkv,B,most", [
+    (64, 24, 8, 40, 3), (64, 40, 8, 40, 20), (128, 12, 4, 40, 5), (128, 40, 8, 33, 20), (256, 10, 2, 70, 6), (256, 24, 8, 40, 40),
+    (64, 3, 1, 64, 2),                                                                    # a row a lane group, heads left over
+    (128, 4, 2, 600, 3), (64, 6, 3, 1024, 9), (128, 8, 2, 1000, 64), (256, 2, 1, 257, 4),  # several sequences a thread
+])
+def test_attention_many_short_sequences(D, Hq, Hkv, B, most, cache):
+    """More sequences than an eighth of the blocks: the join gives every row a lane group of its own."""
+    print(f"attention many D={D} {cache} Hq={Hq} Hkv={Hkv} B={B} most={most}", flush=True)
+    b = many(D, Hq, Hkv, B, most, cache, seed=B + D)
+    lse = torch.empty(b.T, Hq, device="cuda")
+    out, err = b.run(lse=lse, err=torch.zeros(4, dtype=torch.int32, device="cuda"))
+    torch.cuda.synchronize()
+    assert err.tolist()[0] == 0
+    check(b, out, lse)
+
+
+@pytest.mark.parametrize("D,Hq,Hkv,B", [(64, 24, 8, 40), (128, 12, 4, 40), (256, 10, 2, 70), (128, 4, 2, 600)])
+def test_attention_one_unreadable_sequence_among_many(D, Hq, Hkv, B):
+    print(f"attention unreadable D={D} B={B}", flush=True)
+    b = many(D, Hq, Hkv, B, 7, "bf16", seed=B)
+    o, tol, l, ltol = b.reference()
+    i = B // 2
+    rows = torch.zeros(b.T, dtype=torch.bool, device="cuda")
+    rows[int(b.starts[i]):int(b.starts[i + 1])] = True
+    room = b.table.shape[1] * 16
+    for word, at in ((room + 1, "lens"), (-5, "lens"), (b.kc.shape[0], "page")):
+        where = b.lens[i:i + 1] if at == "lens" else b.table[i, 1:2]
+        keep = where.clone()
+        where.fill_(word)
+        lse, err = torch.zeros(b.T, Hq, device="cuda"), torch.zeros(4, dtype=torch.int32, device="cuda")
+        out = b.run(lse=lse, err=err)[0].double()
+        torch.cuda.synchronize()
+        assert err.tolist()[:3] == [1, word, i]
+        assert torch.isnan(out[rows]).all() and torch.isnan(lse[rows]).all()
+        assert ((out - o).abs() <= tol)[~rows].all()
+        none = l.isinf()
+        assert torch.equal(lse.isinf()[~rows], none[~rows])
+        ok = ~rows[:, None] & ~none
+        assert ((lse.double() - l).abs() <= ltol)[ok].all()
+        where.copy_(keep)
+    check(b, b.run()[0])
+
+
+@pytest.mark.parametrize("cache", ["bf16", "fp8"])
+@pytest.mark.parametrize("layers,Hkv,D,page,lens,news", [
+    (2, 2, 64, 16, [5, 0, 130], [700, 1, 257]),
+    (1, 1, 128, 64, [63], [2049]),
+    (3, 8, 128, 256, [0, 255], [513, 300]),
+])
+def test_kv_append_of_prompt_chunks(cache, layers, Hkv, D, page, lens, news):
+    """Whole chunks without a path, hundreds of tokens over many pages; what lies beside them stays."""
+    print(f"append chunk {cache} layers={layers} D={D} lens={lens} news={news}", flush=True)
+    host = torch.Generator().manual_seed(D)
+    B, T = len(lens), sum(news)
+    P = max(-(-(a + n) // page) for a, n in zip(lens, news))
+    table = torch.randperm(B * P + 2, generator=host)[:B * P].to(torch.int32).view(B, P).cuda()
+    kv = (2 * torch.randn(2, layers, T, Hkv, D, device="cuda", generator=gen(D))).to(BF)
+    old = torch.randn(2, layers, B * P + 2, page, Hkv, D, device="cuda", generator=gen(D + 1)).to(BF if cache == "bf16" else F8)
+    ks, vs = (1.0, 1.0) if cache == "bf16" else (0.0625, 0.125)  # powers of two: the quotients are exact
+    got, starts, err = old.clone(), i32([0] + np.cumsum(news).tolist()), torch.zeros(4, dtype=torch.int32, device="cuda")
+    out, _ = kx.kv_append(kv[0], kv[1], got[0], got[1], table, i32(lens), starts, i32(news), max_count=max(news), k_scale=ks,
+                          v_scale=vs, err=err)
+    torch.cuda.synchronize()
+    assert err.tolist()[0] == 0 and out.tolist() == [a + n for a, n in zip(lens, news)]
+    want = old.double().view(2, layers, -1, Hkv, D)
+    t0 = 0
+    for b, (a, n) in enumerate(zip(lens, news)):
+        pos = torch.arange(a, a + n, device="cuda")
+        slot = table[b].long()[pos // page] * page + pos % page
+        x = kv[:, :, t0:t0 + n].double()
+        if cache == "fp8":
+            x = e4m3(torch.stack([x[0] / ks, x[1] / vs]))
+        want[:, :, slot] = x
+        t0 += n
+    assert torch.equal(got.double().view_as(want), want)
