@@ -118,9 +118,9 @@ class VerifyAttention:
     def _ws_for(self, stream):
         key = (stream or torch.cuda.current_stream(self._dev)).cuda_stream
         if key not in self._ws:
-            with torch.cuda.device(self._dev):
+            with torch.cuda.device(self._dev), torch.cuda.stream(stream):  # from the stream's pool (None: the current one's)
                 n = kx.tree_attention_workspace_bytes(self.max_seqs, self.Hq, self.Hkv, self.D, self.max_new)
-            self._ws[key] = torch.empty((n + 7) // 8, dtype=torch.int64, device=self._dev)
+                self._ws[key] = torch.empty((n + 7) // 8, dtype=torch.int64, device=self._dev)
         return self._ws[key]
 
     def forward(self, x, residual, k_cache, v_cache, table, lens, starts, mask, k_scale=1.0, v_scale=1.0, stream=None):

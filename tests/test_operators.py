@@ -317,3 +317,52 @@ def test_routing_refuses_a_shared_stride_past_the_tensor(monkeypatch):
         go(logits[:, 64], 66)
     go(torch.zeros(3), 1), go(logits[:, 64], 65)
     assert len(calls) == 2
+
+
+class Streams:
+    """Stands in for torch's streams and devices on the CPU: `now` is the stream that torch would call current, `made` the
+    one that was current at each torch.empty."""
+
+    class Stream:
+        def __init__(self, n):
+            self.cuda_stream = n
+
+    def __init__(self, monkeypatch):
+        from contextlib import contextmanager, nullcontext
+        self.default, self.now, self.made = self.Stream(0), self.Stream(0), []
+        empty = torch.empty
+
+        @contextmanager
+        def on(stream):
+            before, self.now = self.now, stream or self.now
+            yield
+            self.now = before
+        monkeypatch.setattr(torch.cuda, "stream", on)
+        monkeypatch.setattr(torch.cuda, "device", lambda d: nullcontext())
+        monkeypatch.setattr(torch.cuda, "current_stream", lambda d=None: self.now)
+        monkeypatch.setattr(torch, "empty", lambda *a, **kw: self.made.append(self.now.cuda_stream) or empty(*a, **kw))
+
+
+class Weight:
+    """The shape of an attention layer's weights, without them: 2 + 2 + 2 heads of 64 over 128 features."""
+
+    def __init__(self, N):
+        self.N, self.K = N, 128
+
+
+def attention_layer():
+    from strixite_amd import verify
+    return verify.VerifyAttention(torch.ones(128), Weight(384), Weight(128), 2, 2, 64, 4, 1, 4)
+
+
+def test_a_workspace_that_a_layer_keeps_belongs_to_its_stream(monkeypatch):
+    streams, layer = Streams(monkeypatch), attention_layer()
+    streams.made.clear()
+    layer._ws_for(Streams.Stream(7))
+    assert streams.made and set(streams.made) == {7}
+    streams.made.clear()
+    layer._ws_for(Streams.Stream(7))
+    assert streams.made == []
+    with torch.cuda.stream(Streams.Stream(9)):
+        layer._ws_for(None)
+    assert streams.made and set(streams.made) == {9}
