@@ -95,32 +95,44 @@ class VerifyAttention:
     projection -> attention of the drafted tokens over the layer's paged cache and each other -> output projection (a
     q4 / q8 weight). norm_w BF16 [d]; qkv an Fp8Weight [(Hq + 2 Hkv) D, d], heads in that order; out_w a QWeight
     [d, Hq D]. rotate (optional): called with the BF16 views q [T, Hq, D] and k [T, Hkv, D] after the projection, to turn
-    them by their positions in place, forward's stream being the current one. The drafted tokens' keys and values stay in k_new and v_new until the next forward:
-    what kv_append takes once the accepted path is known. Buffers for max_tokens are allocated here; a workspace is
-    kept for every stream that forward is called on."""
+    them by their positions in place, forward's stream being the current one. The drafted tokens' keys and values stay in
+    k_new and v_new, the last forward's, until the next forward on its stream: what kv_append takes once the accepted path is
+    known. Buffers for max_tokens and a workspace are kept for every stream that forward is called on (a captured graph has
+    those of the stream that it was captured on), so forwards on different streams do not meet; residual, q8, scale, heads,
+    att and y are the last forward's."""
 
     def __init__(self, norm_w, qkv, out_w, Hq, Hkv, D, max_tokens, max_seqs, max_new, eps=1e-6, rotate=None):
         assert qkv.N == (Hq + 2 * Hkv) * D and out_w.K == Hq * D and out_w.N == qkv.K == norm_w.numel()
         self.norm_w, self.qkv, self.out_w, self.Hq, self.Hkv, self.D = norm_w, qkv, out_w, Hq, Hkv, D
         self.M, self.max_seqs, self.max_new, self.eps, self.rotate = max_tokens, max_seqs, max_new, eps, rotate
-        dev, d, M = norm_w.device, qkv.K, max_tokens
-        self._dev = dev
-        self.residual = torch.empty((M, d), dtype=torch.bfloat16, device=dev)
-        self.q8 = torch.empty((M, d), dtype=torch.float8_e4m3fn, device=dev)
-        self.scale = torch.empty((M, d // 128), dtype=torch.float32, device=dev)
-        self.heads = torch.empty((M, Hq + 2 * Hkv, D), dtype=torch.bfloat16, device=dev)
-        self.att = torch.empty((M, Hq, D), dtype=torch.bfloat16, device=dev)
-        self.y = torch.empty((M, d), dtype=torch.bfloat16, device=dev)
-        self.err = torch.zeros(4, dtype=torch.int32, device=dev)
+        self._dev = norm_w.device
+        self.err = torch.zeros(4, dtype=torch.int32, device=self._dev)
         self.k_new = self.v_new = None
-        self._ws = {}
+        first = self._make_buffers()
+        self._buffers, self._ws = {}, {}
+        if norm_w.is_cuda:  # they come from the current stream's pool
+            self._buffers[torch.cuda.current_stream(self._dev).cuda_stream] = first
+        vars(self).update(first)
+
+    def _make_buffers(self):
+        dev, d, M = self._dev, self.qkv.K, self.M
+        return dict(residual=torch.empty((M, d), dtype=torch.bfloat16, device=dev),
+                    q8=torch.empty((M, d), dtype=torch.float8_e4m3fn, device=dev),
+                    scale=torch.empty((M, d // 128), dtype=torch.float32, device=dev),
+                    heads=torch.empty((M, self.Hq + 2 * self.Hkv, self.D), dtype=torch.bfloat16, device=dev),
+                    att=torch.empty((M, self.Hq, self.D), dtype=torch.bfloat16, device=dev),
+                    y=torch.empty((M, d), dtype=torch.bfloat16, device=dev))
 
     def _ws_for(self, stream):
+        """The stream's workspace. The stream's buffers become the layer's."""
         key = (stream or torch.cuda.current_stream(self._dev)).cuda_stream
         if key not in self._ws:
             with torch.cuda.device(self._dev), torch.cuda.stream(stream):  # from the stream's pool (None: the current one's)
                 n = kx.tree_attention_workspace_bytes(self.max_seqs, self.Hq, self.Hkv, self.D, self.max_new)
                 self._ws[key] = torch.empty((n + 7) // 8, dtype=torch.int64, device=self._dev)
+                if key not in self._buffers:
+                    self._buffers[key] = self._make_buffers()
+        vars(self).update(self._buffers[key])
         return self._ws[key]
 
     def forward(self, x, residual, k_cache, v_cache, table, lens, starts, mask, k_scale=1.0, v_scale=1.0, stream=None):
@@ -128,6 +140,7 @@ class VerifyAttention:
         the sum x + residual)."""
         T = x.shape[0]
         assert T <= self.M and lens.numel() <= self.max_seqs
+        ws = self._ws_for(stream)
         res = None if residual is None else self.residual[:T]
         kx.add_rms_norm_fp8(x, self.norm_w, self.eps, residual=residual, residual_out=res, q=self.q8[:T],
                             scale=self.scale[:T], stream=stream)
@@ -138,7 +151,7 @@ class VerifyAttention:
             with torch.cuda.stream(stream):  # the projection and the attention run there (None: the current one)
                 self.rotate(q, self.k_new)
         kx.tree_attention(q, self.k_new, self.v_new, k_cache, v_cache, table, lens, starts, mask, self.max_new,
-                          k_scale=k_scale, v_scale=v_scale, out=self.att[:T], ws=self._ws_for(stream), err=self.err,
+                          k_scale=k_scale, v_scale=v_scale, out=self.att[:T], ws=ws, err=self.err,
                           stream=stream)
         kx.linear(self.att[:T].view(T, -1), self.out_w, y=self.y[:T], stream=stream)
         return self.y[:T], x if residual is None else res

@@ -865,3 +865,24 @@ def test_kv_append_of_prompt_chunks(cache, layers, Hkv, D, page, lens, news):
         want[:, :, slot] = x
         t0 += n
     assert torch.equal(got.double().view_as(want), want)
+
+
+def test_verify_attention_on_two_streams_at_once():
+    from strixite_amd import synthetic as syn
+    from strixite_amd.verify import VerifyAttention
+    d, Hq, Hkv, D = 512, 4, 2, 128
+    b = Batch(D, Hq, Hkv, 16, [900], [6], seed=71)
+    mask = kx.tree_mask([list(range(-1, 5))]).cuda()
+    qkv = fp8_case(1, (Hq + 2 * Hkv) * D, d, seed=72)[2]
+    qkv.scale.mul_(0.01)
+    att = VerifyAttention(torch.ones(d, dtype=BF, device="cuda"), qkv, syn.qweight(8, d, Hq * D, 64, seed=73), Hq, Hkv, D, 8, 2, 8)
+    xs = [syn.activations(6, d, seed=74 + i) for i in range(2)]
+    go = lambda x, s=None: att.forward(x, x, b.kc, b.vc, b.table, b.lens, b.starts, mask, stream=s)
+    want = [[t.clone() for t in (*go(x), att.k_new)] for x in xs]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    for _ in range(5):
+        got = [(*go(x, s), att.k_new) for x, s in zip(xs, streams)]
+        torch.cuda.synchronize()
+        for w, g in zip(want, got):
+            assert all(torch.equal(p, q) for p, q in zip(w, g))

@@ -366,3 +366,27 @@ def test_a_workspace_that_a_layer_keeps_belongs_to_its_stream(monkeypatch):
     with torch.cuda.stream(Streams.Stream(9)):
         layer._ws_for(None)
     assert streams.made and set(streams.made) == {9}
+
+
+def test_forwards_of_a_layer_on_two_streams_share_no_buffer(monkeypatch):
+    from strixite_amd import verify
+    streams, written = Streams(monkeypatch), []
+    span = lambda t: (t.data_ptr(), t.data_ptr() + t.numel() * t.element_size())
+    outs = dict(add_rms_norm_fp8=("residual_out", "q", "scale"), linear_fp8=("y",), tree_attention=("out", "ws"), linear=("y",))
+    for f, names in outs.items():
+        monkeypatch.setattr(verify.kx, f, lambda *a, names=names, **kw: written.extend(span(kw[n]) for n in names))
+    layer, x, lens = attention_layer(), torch.zeros(4, 128, dtype=torch.bfloat16), torch.zeros(1, dtype=torch.int32)
+    layer_parts = ("residual", "q8", "scale", "heads", "att", "y")
+
+    def forward(stream):
+        written.clear()
+        y, r = layer.forward(x, x, None, None, None, lens, None, None, stream=stream)
+        assert y.data_ptr() == layer.y.data_ptr() and r.data_ptr() == layer.residual.data_ptr()
+        assert layer.k_new.data_ptr() == layer.heads[:, 2].data_ptr()
+        return list(written), [span(getattr(layer, n)) for n in layer_parts]
+    one, two = Streams.Stream(1), Streams.Stream(2)
+    (a, parts_a), (b, parts_b), (again, _) = forward(one), forward(two), forward(one)
+    assert len(a) == 7 and a == again
+    assert all(lo2 >= hi1 or lo1 >= hi2 for lo1, hi1 in a + parts_a for lo2, hi2 in b + parts_b)
+    with torch.cuda.stream(two):
+        assert forward(None)[0] == b
