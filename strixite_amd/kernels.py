@@ -422,8 +422,9 @@ def mtp_accept(cands, nan, drafts, u, temperature, top_k, top_p, n_valid, out=No
 
 # ---------------- a verify layer's attention half, and routing by scores ----------------
 # Strides, types, shapes and devices are checked here, where the tensors are; the library checks the rest. A call runs
-# on its tensors' device, on that device's current stream unless one is given. err (optional, a zeroed int32 [4] on the
-# device) receives what a call could not read; without it the outputs alone say so.
+# on its tensors' device, on that device's current stream unless one is given; buffers that it makes come from that
+# stream's pool. err (optional, a zeroed int32 [4] on the device) receives what a call could not read; without it the
+# outputs alone say so.
 
 def _refuse(*what):
     raise SxError(SX_EINVAL, " ".join(str(w) for w in what))
@@ -462,6 +463,16 @@ def _a(t):
     return None if t is None else t.data_ptr()
 
 
+def _empty(like, shape, dtype, stream):
+    """A buffer that a call makes, on like's device, from the pool of the stream that the call runs on: from another one
+    it could be memory that work queued there still uses, and if it is dropped, be given to such work while the call's
+    kernels still write it."""
+    if stream is None:
+        return like.new_empty(shape, dtype=dtype)
+    with torch.cuda.stream(stream):
+        return like.new_empty(shape, dtype=dtype)
+
+
 class Fp8Weight:
     """An e4m3 weight resident on the device: q [N, K] torch.float8_e4m3fn, scale [ceil(N / 128), K / 128] FP32, one
     for each 128 x 128 tile (w = code * scale)."""
@@ -498,7 +509,7 @@ def add_rms_norm_fp8(x, weight, eps=1e-6, residual=None, residual_out=None, w_ad
     if residual is not None:
         _is("residual", residual, dtype, shape)
         if residual_out is None:
-            residual_out = torch.empty_like(residual)
+            residual_out = _empty(x, shape, dtype, stream)
         else:
             _is("residual_out", residual_out, dtype, shape)
     elif residual_out is not None:
@@ -506,11 +517,11 @@ def add_rms_norm_fp8(x, weight, eps=1e-6, residual=None, residual_out=None, w_ad
     if y is not None:
         _is("y", y, dtype, shape)
     if q is None:
-        q = x.new_empty(shape, dtype=torch.float8_e4m3fn)
+        q = _empty(x, shape, torch.float8_e4m3fn, stream)
     else:
         _is("q", q, torch.float8_e4m3fn, shape)
     if scale is None:
-        scale = x.new_empty((M, K // 128), dtype=torch.float32)
+        scale = _empty(x, (M, K // 128), torch.float32, stream)
     else:
         _is("scale", scale, torch.float32, (M, K // 128))
     _run(dev, lib().sx_add_rms_norm_fp8, x.data_ptr(), x.stride(0) if M > 1 else K, _a(residual), weight.data_ptr(), M, K,
@@ -526,7 +537,7 @@ def linear_fp8(x, x_scale, w, out_act=ACT_BF16, y=None, stream=None):
     _is("x", x, torch.float8_e4m3fn, (M, w.K))
     _is("x_scale", x_scale, torch.float32, (M, w.K // 128))
     if y is None:
-        y = x.new_empty((M, w.N), dtype=dtype)
+        y = _empty(x, (M, w.N), dtype, stream)
     else:
         _is("y", y, dtype, (M, w.N))
     _run(dev, lib().sx_linear_fp8, x.data_ptr(), x_scale.data_ptr(), w.view(), y.data_ptr(), M, out_act, stream=stream)
@@ -618,13 +629,13 @@ def tree_attention(q, k_new, v_new, k_cache, v_cache, table, lens, starts, mask,
     if mask.dtype != torch.int64 or mask.dim() != 2 or mask.shape[0] != T or mask.stride(1) != 1 or mask.shape[1] * 64 < max_new:
         _refuse("mask must be int64 [T, ceil(max_new / 64)] with dense rows and is", mask.dtype, tuple(mask.shape))
     if out is None:
-        out = torch.empty((T, Hq, D), dtype=torch.bfloat16, device=q.device)
+        out = _empty(q, (T, Hq, D), torch.bfloat16, stream)
     elif out.dim() != 3 or out.shape[0] != T:
         _refuse("out is", tuple(out.shape))
     if lse is not None:
         _is("lse", lse, torch.float32, (T, Hq))
     if ws is None:
-        with torch.cuda.stream(stream):  # from its pool (None: the current one's): the buffer ends with this call, the kernels later
+        with torch.cuda.stream(stream):  # as _empty's (None: the current one's)
             ws = tree_attention_workspace(q, k_new, starts, max_new)
     elif not ws.is_contiguous():
         _refuse("ws must be contiguous and has strides", ws.stride())
@@ -665,7 +676,7 @@ def kv_append(k_new, v_new, k_cache, v_cache, table, lens, starts, count, path=N
     elif max_count is None:
         _refuse("max_count is needed without a path")
     if lens_out is None:
-        lens_out = torch.empty_like(lens)
+        lens_out = _empty(lens, (B,), torch.int32, stream)
     else:
         _is("lens_out", lens_out, torch.int32, (B,))
     _is_err(err)
@@ -698,11 +709,11 @@ def moe_router_scored(logits, E, k, score="sigmoid", bias=None, groups=1, top_gr
     if shared is not None and (shared.storage_offset() + (M - 1) * shared_ld + 1) * shared.element_size() > shared.untyped_storage().nbytes():
         _refuse("shared_ld =", shared_ld, "leads past the shared logits", tuple(shared.shape), shared.stride())
     if ids is None:
-        ids = torch.empty(shape, dtype=torch.int32, device=logits.device)
+        ids = _empty(logits, shape, torch.int32, stream)
     else:
         _is("ids", ids, torch.int32, shape)
     if coef is None:
-        coef = torch.empty(shape, dtype=torch.float32, device=logits.device)
+        coef = _empty(logits, shape, torch.float32, stream)
     else:
         _is("coef", coef, torch.float32, shape)
     _is_err(err)

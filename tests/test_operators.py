@@ -341,6 +341,9 @@ class Streams:
         monkeypatch.setattr(torch.cuda, "device", lambda d: nullcontext())
         monkeypatch.setattr(torch.cuda, "current_stream", lambda d=None: self.now)
         monkeypatch.setattr(torch, "empty", lambda *a, **kw: self.made.append(self.now.cuda_stream) or empty(*a, **kw))
+        like, new = torch.empty_like, torch.Tensor.new_empty
+        monkeypatch.setattr(torch, "empty_like", lambda *a, **kw: self.made.append(self.now.cuda_stream) or like(*a, **kw))
+        monkeypatch.setattr(torch.Tensor, "new_empty", lambda *a, **kw: self.made.append(self.now.cuda_stream) or new(*a, **kw))
 
 
 class Weight:
@@ -390,3 +393,36 @@ def test_forwards_of_a_layer_on_two_streams_share_no_buffer(monkeypatch):
     assert all(lo2 >= hi1 or lo1 >= hi2 for lo1, hi1 in a + parts_a for lo2, hi2 in b + parts_b)
     with torch.cuda.stream(two):
         assert forward(None)[0] == b
+
+
+def operator_calls():
+    """Each of the five operators on small tensors, without the buffers that it can make, and how many it makes then."""
+    bf, f8 = torch.bfloat16, torch.float8_e4m3fn
+    i32 = lambda *v: torch.tensor(v, dtype=torch.int32)
+    x, q = torch.zeros(3, 128, dtype=bf), torch.zeros(3, 4, 64, dtype=bf)
+    kv, c = torch.zeros(3, 2, 64, dtype=bf), torch.zeros(4, 16, 2, 64, dtype=bf)
+    w = kx.Fp8Weight(torch.zeros(16, 128, dtype=torch.uint8).view(f8), torch.ones(1, 1))
+    codes, scale = torch.zeros(3, 128, dtype=torch.uint8).view(f8), torch.ones(3, 1)
+    seqs = (i32(0, 1, 2, 3).view(2, 2), i32(1, 2), i32(0, 1, 3))
+    mask, logits = torch.ones(3, 1, dtype=torch.int64), torch.zeros(3, 64)
+    return {
+        "norm": (3, lambda s: kx.add_rms_norm_fp8(x, x[0], residual=x, stream=s)),
+        "linear": (1, lambda s: kx.linear_fp8(codes, scale, w, stream=s)),
+        "attention": (2, lambda s: kx.tree_attention(q, kv, kv, c, c, *seqs, mask, 2, stream=s)),
+        "append": (1, lambda s: kx.kv_append(kv, kv, c, c, *seqs, i32(1, 1), max_count=1, stream=s)),
+        "routing": (2, lambda s: kx.moe_router_scored(logits, 64, 4, stream=s)),
+    }
+
+
+@pytest.mark.parametrize("name", ["norm", "linear", "attention", "append", "routing"])
+def test_buffers_that_a_call_makes_belong_to_its_stream(monkeypatch, name):
+    n, call = operator_calls()[name]
+    streams = Streams(monkeypatch)
+    monkeypatch.setattr(kx, "_together", lambda dev, tensors: None)
+    monkeypatch.setattr(kx, "_run", lambda *a, **kw: None)
+    monkeypatch.setattr(kx, "tree_attention_workspace_bytes", lambda *a: 64)
+    call(Streams.Stream(3))
+    assert streams.made == [3] * n
+    streams.made.clear()
+    call(None)
+    assert streams.made == [0] * n
