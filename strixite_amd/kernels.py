@@ -35,6 +35,17 @@ def dtype_of(act):
     return torch.float32 if act == ACT_F32 else torch.bfloat16
 
 
+def _empty(like, shape, dtype, stream, fill=None):
+    """A buffer that a call makes, on like's device, from the pool of the stream that the call runs on (and filled there):
+    from another one it could be memory that work queued there still uses, and if it is dropped, be given to such work
+    while the call's kernels still write it."""
+    if stream is not None:
+        with torch.cuda.stream(stream):
+            return _empty(like, shape, dtype, None, fill)
+    t = like.new_empty(shape, dtype=dtype)
+    return t if fill is None else t.fill_(fill)
+
+
 class QWeight:
     """A q4 / q8 weight resident on the device (Q4Device / Q8Device, runtime/q4_device.hpp:23-36): codes uint8,
     scale / min as BF16 bits (int16 tensors), in the formats/q4.hpp / q8.hpp layout."""
@@ -63,7 +74,7 @@ def linear(x, w, out_act=None, y=None, stream=None):
     out_act = act if out_act is None else out_act
     M = x.shape[0]
     if y is None:
-        y = torch.empty((M, w.N), dtype=dtype_of(out_act), device=x.device)
+        y = _empty(x, (M, w.N), dtype_of(out_act), stream)
     f = lib().sx_linear_q4 if w.bits == 4 else lib().sx_linear_q8
     check(f(_p(x), w.view(), _p(y), M, act, out_act, _s(stream)))
     return y
@@ -86,8 +97,9 @@ def experts_grouped_kernel(w, E, M, A, act=ACT_BF16):
     return name.decode()
 
 
-def _err(device):
-    return torch.zeros(4, dtype=torch.int32, device=device)
+def _err(like, stream):
+    """Zeroed error words for a call, on the call's stream (_empty)."""
+    return _empty(like, (4,), torch.int32, stream, 0)
 
 
 def experts_gather(x, w, E, ids, swiglu=False, y=None, err=None, stream=None):
@@ -96,8 +108,8 @@ def experts_gather(x, w, E, ids, swiglu=False, y=None, err=None, stream=None):
     M, A = ids.shape
     N = w.N // E
     out_n = N // 2 if swiglu else N
-    y = torch.empty((M, A, out_n), dtype=x.dtype, device=x.device) if y is None else y
-    err = _err(x.device) if err is None else err
+    y = _empty(x, (M, A, out_n), x.dtype, stream) if y is None else y
+    err = _err(x, stream) if err is None else err
     f = lib().sx_linear_q4_experts_gather_swiglu if swiglu else lib().sx_linear_q4_experts_gather
     check(f(_p(x), w.view(), E, _p(ids), M, A, _p(y), act, _p(err), _s(stream)))
     return y, err
@@ -107,8 +119,8 @@ def experts_combine(h, w, E, ids, coef, y=None, err=None, stream=None):
     act = act_of(h)
     M, A = ids.shape
     N = w.N // E
-    y = torch.empty((M, N), dtype=h.dtype, device=h.device) if y is None else y
-    err = _err(h.device) if err is None else err
+    y = _empty(h, (M, N), h.dtype, stream) if y is None else y
+    err = _err(h, stream) if err is None else err
     check(lib().sx_linear_q4_experts_combine(_p(h), w.view(), E, _p(ids), _p(coef), M, A, _p(y), act, _p(err),
                                              _s(stream)))
     return y, err
@@ -117,9 +129,9 @@ def experts_combine(h, w, E, ids, coef, y=None, err=None, stream=None):
 def moe_router(logits, E, k, shared=None, shared_ld=1, shared_id=0, ids=None, coef=None, err=None, stream=None):
     M, ld = logits.shape
     A = k + (1 if shared is not None else 0)
-    ids = torch.empty((M, A), dtype=torch.int32, device=logits.device) if ids is None else ids
-    coef = torch.empty((M, A), dtype=torch.float32, device=logits.device) if coef is None else coef
-    err = _err(logits.device) if err is None else err
+    ids = _empty(logits, (M, A), torch.int32, stream) if ids is None else ids
+    coef = _empty(logits, (M, A), torch.float32, stream) if coef is None else coef
+    err = _err(logits, stream) if err is None else err
     check(lib().sx_moe_router(_p(logits), ld, M, E, k, _p(shared), shared_ld, shared_id, _p(ids), _p(coef),
                               act_of(logits), _p(err), _s(stream)))
     return ids, coef, err
@@ -134,12 +146,11 @@ def route_workspace_bytes(M, A, E):
 def router_group(logits, E, k, ws=None, ids=None, coef=None, router_err=None, expert_err=None, stream=None):
     """moe_router + moe_group_routes in one launch (M * k <= 2048)."""
     M, ld = logits.shape
-    dev = logits.device
-    ws = torch.empty(route_workspace_bytes(M, k, E) // 4, dtype=torch.int32, device=dev) if ws is None else ws
-    ids = torch.empty((M, k), dtype=torch.int32, device=dev) if ids is None else ids
-    coef = torch.empty((M, k), dtype=torch.float32, device=dev) if coef is None else coef
-    router_err = _err(dev) if router_err is None else router_err
-    expert_err = _err(dev) if expert_err is None else expert_err
+    ws = _empty(logits, (route_workspace_bytes(M, k, E) // 4,), torch.int32, stream) if ws is None else ws
+    ids = _empty(logits, (M, k), torch.int32, stream) if ids is None else ids
+    coef = _empty(logits, (M, k), torch.float32, stream) if coef is None else coef
+    router_err = _err(logits, stream) if router_err is None else router_err
+    expert_err = _err(logits, stream) if expert_err is None else expert_err
     check(lib().sx_moe_router_group(_p(logits), ld, M, E, k, act_of(logits), _p(ids), _p(coef), _p(router_err),
                                     _p(ws), ws.numel() * 4, _p(expert_err), _s(stream)))
     return ids, coef, ws, router_err, expert_err
@@ -161,12 +172,11 @@ def verify_gate_up(x, logits, w, E, k, Ew=None, shared_logit=None, shared_id=0, 
     Ew = E if Ew is None else Ew
     A = k + (shared_logit is not None)
     I = w.N // Ew // 2
-    dev = x.device
-    ids = torch.empty((M, A), dtype=torch.int32, device=dev) if ids is None else ids
-    coef = torch.empty((M, A), dtype=torch.float32, device=dev) if coef is None else coef
-    h = torch.empty((M, A, I), dtype=x.dtype, device=dev) if h is None else h
-    router_err = _err(dev) if router_err is None else router_err
-    expert_err = _err(dev) if expert_err is None else expert_err
+    ids = _empty(x, (M, A), torch.int32, stream) if ids is None else ids
+    coef = _empty(x, (M, A), torch.float32, stream) if coef is None else coef
+    h = _empty(x, (M, A, I), x.dtype, stream) if h is None else h
+    router_err = _err(x, stream) if router_err is None else router_err
+    expert_err = _err(x, stream) if expert_err is None else expert_err
     sld = 0 if shared_logit is None else shared_logit.stride(0)
     check(lib().sx_moe_verify_gate_up(_p(x), M, _p(logits), ld, E, k, _p(shared_logit), sld, shared_id, w.view(), Ew,
                                       _p(ids), _p(coef), _p(h), _p(h_sums), act_of(x), _p(router_err),
@@ -179,8 +189,8 @@ def verify_down(h, w, ids, coef, Ew, y=None, expert_err=None, h_sums=None, plan=
     sums of this h, optional; plan: the routing plan verify_gate_up stored with these ids, optional)."""
     M, A = ids.shape
     N = w.N // Ew
-    y = torch.empty((M, N), dtype=h.dtype, device=h.device) if y is None else y
-    expert_err = _err(h.device) if expert_err is None else expert_err
+    y = _empty(h, (M, N), h.dtype, stream) if y is None else y
+    expert_err = _err(h, stream) if expert_err is None else expert_err
     check(lib().sx_moe_verify_down(_p(h), _p(h_sums), M, A, _p(ids), _p(coef), w.view(), Ew, _p(y), act_of(h),
                                    _p(expert_err), _p(plan), _s(stream)))
     return y, expert_err
@@ -210,16 +220,15 @@ def verify_layer(x, Wr, gate_up, down, E, k, sync, shared=False, shared_id=0, Ew
     Ew = E if Ew is None else Ew
     A = k + (1 if shared else 0)
     I = gate_up.N // Ew // 2
-    dev = x.device
     wr_act = ACT_F32 if Wr.dtype == torch.float32 else ACT_BF16
-    logits = torch.empty((M, rows), dtype=torch.float32, device=dev) if logits is None else logits
-    ids = torch.empty((M, A), dtype=torch.int32, device=dev) if ids is None else ids
-    coef = torch.empty((M, A), dtype=torch.float32, device=dev) if coef is None else coef
-    h = torch.empty((M, A, I), dtype=x.dtype, device=dev) if h is None else h
-    h_sums = torch.empty((M * A, (I + 15) // 16), dtype=torch.float32, device=dev) if h_sums is None else h_sums
-    y = torch.empty((M, down.N // Ew), dtype=x.dtype, device=dev) if y is None else y
-    router_err = _err(dev) if router_err is None else router_err
-    expert_err = _err(dev) if expert_err is None else expert_err
+    logits = _empty(x, (M, rows), torch.float32, stream) if logits is None else logits
+    ids = _empty(x, (M, A), torch.int32, stream) if ids is None else ids
+    coef = _empty(x, (M, A), torch.float32, stream) if coef is None else coef
+    h = _empty(x, (M, A, I), x.dtype, stream) if h is None else h
+    h_sums = _empty(x, (M * A, (I + 15) // 16), torch.float32, stream) if h_sums is None else h_sums
+    y = _empty(x, (M, down.N // Ew), x.dtype, stream) if y is None else y
+    router_err = _err(x, stream) if router_err is None else router_err
+    expert_err = _err(x, stream) if expert_err is None else expert_err
     check(lib().sx_moe_verify_layer(_p(x), M, _p(Wr), wr_act, rows, E, k, int(shared), shared_id, gate_up.view(),
                                     down.view(), Ew, _p(logits), _p(ids), _p(coef), _p(h), _p(h_sums), _p(y),
                                     act_of(x), _p(router_err), _p(expert_err), _p(sync), _s(stream)))
@@ -229,8 +238,8 @@ def verify_layer(x, Wr, gate_up, down, E, k, sync, shared=False, shared_id=0, Ew
 def group_routes(ids, E, ws=None, err=None, stream=None):
     M, A = ids.shape
     nb = route_workspace_bytes(M, A, E)
-    ws = torch.empty(nb // 4, dtype=torch.int32, device=ids.device) if ws is None else ws
-    err = _err(ids.device) if err is None else err
+    ws = _empty(ids, (nb // 4,), torch.int32, stream) if ws is None else ws
+    err = _err(ids, stream) if err is None else err
     check(lib().sx_moe_group_routes(_p(ids), M, A, E, _p(ws), ws.numel() * 4, _p(err), _s(stream)))
     return ws, err
 
@@ -239,7 +248,7 @@ def gather_grouped(x, w, E, ws, M, A, swiglu=False, y=None, math=MOE_F32, stream
     act = act_of(x)
     N = w.N // E
     out_n = N // 2 if swiglu else N
-    y = torch.empty((M, A, out_n), dtype=x.dtype, device=x.device) if y is None else y
+    y = _empty(x, (M, A, out_n), x.dtype, stream) if y is None else y
     if swiglu:
         check(lib().sx_linear_q4_experts_gather_swiglu_grouped(_p(x), w.view(), E, _p(ws), ws.numel() * 4, M, A, _p(y),
                                                                act, _s(stream)))
@@ -253,8 +262,8 @@ def combine_grouped(h, w, E, ids, coef, ws, partial=None, y=None, math=MOE_F32, 
     act = act_of(h)
     M, A = ids.shape
     N = w.N // E
-    y = torch.empty((M, N), dtype=h.dtype, device=h.device) if y is None else y
-    partial = torch.empty((M * A, N), dtype=torch.float32, device=h.device) if partial is None else partial
+    y = _empty(h, (M, N), h.dtype, stream) if y is None else y
+    partial = _empty(h, (M * A, N), torch.float32, stream) if partial is None else partial
     check(lib().sx_linear_q4_experts_combine_grouped(_p(h), w.view(), E, _p(ids), _p(coef), _p(ws), ws.numel() * 4,
                                                      _p(partial), M, A, _p(y), act, math, _s(stream)))
     return y
@@ -262,7 +271,7 @@ def combine_grouped(h, w, E, ids, coef, ws, partial=None, y=None, math=MOE_F32, 
 
 def swiglu(gu, h=None, stream=None):
     rows, I2 = gu.shape
-    h = torch.empty((rows, I2 // 2), dtype=gu.dtype, device=gu.device) if h is None else h
+    h = _empty(gu, (rows, I2 // 2), gu.dtype, stream) if h is None else h
     check(lib().sx_swiglu(_p(gu), _p(h), rows, I2 // 2, act_of(gu), _s(stream)))
     return h
 
@@ -270,7 +279,7 @@ def swiglu(gu, h=None, stream=None):
 def linear_f32w(x, W, y=None, stream=None):
     M, K = x.shape
     N = W.shape[0]
-    y = torch.empty((M, N), dtype=torch.float32, device=x.device) if y is None else y
+    y = _empty(x, (M, N), torch.float32, stream) if y is None else y
     check(lib().sx_linear_f32w(_p(x), _p(W), N, K, _p(y), M, act_of(x), _s(stream)))
     return y
 
@@ -281,7 +290,7 @@ def linear_bf16w(x, W, out_act=None, y=None, wmma=False, stream=None):
     out_act = act if out_act is None else out_act
     M, K = x.shape
     N = W.shape[0]
-    y = torch.empty((M, N), dtype=dtype_of(out_act), device=x.device) if y is None else y
+    y = _empty(x, (M, N), dtype_of(out_act), stream) if y is None else y
     f = lib().sx_linear_bf16w_wmma if wmma else lib().sx_linear_bf16w
     check(f(_p(x), _p(W), _p(y), M, N, K, act, out_act, _s(stream)))
     return y
@@ -311,10 +320,10 @@ def logits_topk(logits, n_valid, k=20, mask=None, ws=None, out=None, nan=None, s
     """Per row the best k (value desc, lower id on a tie) of logits [rows, >= n_valid] (any row stride). Returns
     (values f32 [rows, k], ids i32 [rows, k], nan, the raw [rows, k, 2] candidates)."""
     rows, ld = logits.shape[0], logits.stride(0)
-    out = torch.empty((rows, k, 2), dtype=torch.int32, device=logits.device) if out is None else out
-    nan = torch.empty(rows, dtype=torch.int32, device=logits.device) if nan is None else nan
+    out = _empty(logits, (rows, k, 2), torch.int32, stream) if out is None else out
+    nan = _empty(logits, (rows,), torch.int32, stream) if nan is None else nan
     if ws is None:
-        ws = torch.empty(topk_workspace_bytes(rows, n_valid, k) // 8 + 1, dtype=torch.int64, device=logits.device)
+        ws = _empty(logits, (topk_workspace_bytes(rows, n_valid, k) // 8 + 1,), torch.int64, stream)
     mw = 0 if mask is None else mask.shape[1]
     check(lib().sx_logits_topk(_p(logits), rows, ld, n_valid, k, _p(out), _p(nan), _p(ws), ws.numel() * 8, _p(mask), mw,
                                _s(stream)))
@@ -325,8 +334,8 @@ def logits_topk_noalloc(logits, n_valid, k=20, mask=None, out=None, nan=None, st
     """logits_topk on the library's fixed scratch (sx_logits_topk_noalloc: no workspace, nothing allocated by the
     call). Same returns as logits_topk."""
     rows, ld = logits.shape[0], logits.stride(0)
-    out = torch.empty((rows, k, 2), dtype=torch.int32, device=logits.device) if out is None else out
-    nan = torch.empty(rows, dtype=torch.int32, device=logits.device) if nan is None else nan
+    out = _empty(logits, (rows, k, 2), torch.int32, stream) if out is None else out
+    nan = _empty(logits, (rows,), torch.int32, stream) if nan is None else nan
     mw = 0 if mask is None else mask.shape[1]
     check(lib().sx_logits_topk_noalloc(_p(logits), rows, ld, n_valid, k, _p(out), _p(nan), _p(mask), mw, _s(stream)))
     return out[..., 0].view(torch.float32), out[..., 1], nan, out
@@ -335,11 +344,10 @@ def logits_topk_noalloc(logits, n_valid, k=20, mask=None, out=None, nan=None, st
 def quantize_q4_from_q8(w8, G=64, rows=None, err=None, stream=None):
     """The Q4 copy of the first `rows` rows of a Q8 weight (formats/q4_from_q8.hpp), made on the device: a QWeight."""
     rows = w8.N if rows is None else rows
-    dev = w8.q.device
-    q = torch.empty(rows * w8.K // 2, dtype=torch.uint8, device=dev)
-    s = torch.empty(rows * (w8.K // G), dtype=torch.int16, device=dev)
-    m = torch.empty(rows * (w8.K // G), dtype=torch.int16, device=dev)
-    err = _err(dev) if err is None else err
+    q = _empty(w8.q, (rows * w8.K // 2,), torch.uint8, stream)
+    s = _empty(w8.q, (rows * (w8.K // G),), torch.int16, stream)
+    m = _empty(w8.q, (rows * (w8.K // G),), torch.int16, stream)
+    err = _err(w8.q, stream) if err is None else err
     src = QView(w8.q.data_ptr(), w8.scale.data_ptr(), w8.minv.data_ptr(), rows, w8.K, w8.G)
     check(lib().sx_quantize_q4_from_q8(ctypes.byref(src), G, _p(q), _p(s), _p(m), _p(err), _s(stream)))
     return QWeight(4, q, s, m, rows, w8.K, G), err
@@ -354,7 +362,7 @@ def mtp_pick_ws_bytes(n):
 def mtp_pick(logits, router_err, expert_err, attn_err, emb_err, out=None, ws=None, stream=None):
     """The 64-byte pick of `logits`. With `ws` (a zeroed device uint8 buffer of mtp_pick_ws_bytes, reused across
     calls on one stream) the one-launch many-block pick runs; its output is bit-identical to the single-block one's."""
-    out = torch.empty(64, dtype=torch.uint8, device=logits.device) if out is None else out
+    out = _empty(logits, (64,), torch.uint8, stream) if out is None else out
     if ws is None:
         check(lib().sx_mtp_pick(_p(logits), logits.numel(), _p(router_err), _p(expert_err), _p(attn_err),
                                 _p(emb_err), _p(out), _s(stream)))
@@ -367,7 +375,7 @@ def mtp_pick(logits, router_err, expert_err, attn_err, emb_err, out=None, ws=Non
 def mtp_head_pick(x, w, logits, router_err, expert_err, attn_err, emb_err, ws, out=None, stream=None):
     """The draft head's logits (x BF16 [1, K] against the q4 / q8 head, FP32 [N] into `logits`) and their pick, one
     launch; `ws` a zeroed device uint8 buffer of mtp_pick_ws_bytes. Returns the 64-byte pick."""
-    out = torch.empty(64, dtype=torch.uint8, device=x.device) if out is None else out
+    out = _empty(x, (64,), torch.uint8, stream) if out is None else out
     assert x.dtype == torch.bfloat16 and x.numel() == w.K and logits.numel() >= w.N
     check(lib().sx_mtp_head_pick(_p(x), w.view(), w.bits, _p(logits), _p(router_err), _p(expert_err), _p(attn_err),
                                  _p(emb_err), _p(out), _p(ws), ws.numel() * ws.element_size(), _s(stream)))
@@ -395,12 +403,11 @@ def verify_tail(logits, n_valid, kc, ws, drafts=None, u=None, temperature=0.0, t
     """logits_topk (kc candidates a row) and, with drafts, mtp_accept in one launch. Returns (cands [rows, kc, 2],
     nan, out or None)."""
     rows, ld = logits.shape[0], logits.stride(0)
-    dev = logits.device
-    cands = torch.empty((rows, kc, 2), dtype=torch.int32, device=dev) if cands is None else cands
-    nan = torch.empty(rows, dtype=torch.int32, device=dev) if nan is None else nan
+    cands = _empty(logits, (rows, kc, 2), torch.int32, stream) if cands is None else cands
+    nan = _empty(logits, (rows,), torch.int32, stream) if nan is None else nan
     k = 0 if drafts is None else drafts.numel()
     if drafts is not None and out is None:
-        out = torch.full((2 + k + 1,), -1, dtype=torch.int32, device=dev)
+        out = _empty(logits, (2 + k + 1,), torch.int32, stream, -1)
     mw = 0 if mask is None else mask.shape[1]
     check(lib().sx_verify_tail(_p(logits), rows, ld, n_valid, kc, _p(cands), _p(nan), _p(mask), mw, _p(drafts), k,
                                _p(u), float(temperature), int(top_k), float(top_p),
@@ -414,7 +421,7 @@ def mtp_accept(cands, nan, drafts, u, temperature, top_k, top_p, n_valid, out=No
     rows, kc = cands.shape[0], cands.shape[1]
     k = drafts.numel()
     assert rows >= k + 1, "one candidate row per draft plus the last"
-    out = torch.full((2 + k + 1,), -1, dtype=torch.int32, device=cands.device) if out is None else out
+    out = _empty(cands, (2 + k + 1,), torch.int32, stream, -1) if out is None else out
     check(lib().sx_mtp_accept(_p(cands), _p(nan), kc, _p(drafts), k, _p(u), float(temperature), int(top_k),
                               float(top_p), int(n_valid), _p(out), _s(stream)))
     return out
@@ -461,16 +468,6 @@ def _run(dev, f, *args, stream=None):
 
 def _a(t):
     return None if t is None else t.data_ptr()
-
-
-def _empty(like, shape, dtype, stream):
-    """A buffer that a call makes, on like's device, from the pool of the stream that the call runs on: from another one
-    it could be memory that work queued there still uses, and if it is dropped, be given to such work while the call's
-    kernels still write it."""
-    if stream is None:
-        return like.new_empty(shape, dtype=dtype)
-    with torch.cuda.stream(stream):
-        return like.new_empty(shape, dtype=dtype)
 
 
 class Fp8Weight:

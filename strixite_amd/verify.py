@@ -46,7 +46,8 @@ class MoeVerifyLayer:
     def _sync_for(self, stream):
         key = (stream or torch.cuda.current_stream(self._dev)).cuda_stream
         if key not in self._syncs:
-            self._syncs[key] = kx.verify_layer_sync(self._dev)
+            with torch.cuda.stream(stream):  # zeroed in the stream's own order (None: the current one)
+                self._syncs[key] = kx.verify_layer_sync(self._dev)
         return self._syncs[key]
 
     def _fused(self, M):

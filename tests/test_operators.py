@@ -344,6 +344,10 @@ class Streams:
         like, new = torch.empty_like, torch.Tensor.new_empty
         monkeypatch.setattr(torch, "empty_like", lambda *a, **kw: self.made.append(self.now.cuda_stream) or like(*a, **kw))
         monkeypatch.setattr(torch.Tensor, "new_empty", lambda *a, **kw: self.made.append(self.now.cuda_stream) or new(*a, **kw))
+        for f in ("zeros", "full"):  # made and filled
+            monkeypatch.setattr(torch, f, lambda *a, real=getattr(torch, f), **kw: self.made.append(self.now.cuda_stream) or real(*a, **kw))
+        fill = torch.Tensor.fill_
+        monkeypatch.setattr(torch.Tensor, "fill_", lambda *a: self.made.append(self.now.cuda_stream) or fill(*a))
 
 
 class Weight:
@@ -426,3 +430,58 @@ def test_buffers_that_a_call_makes_belong_to_its_stream(monkeypatch, name):
     streams.made.clear()
     call(None)
     assert streams.made == [0] * n
+
+
+def earlier_calls():
+    """The other operators that make buffers: the arguments are placeholders, nothing is launched."""
+    x, ids = torch.zeros(2, 64), torch.zeros(2, 3, dtype=torch.int32)
+    w, e = Weight(64), Weight(8 * 64)
+    w.bits, w.G, w.q, w.scale, w.minv, w.view = 8, 64, torch.zeros(64 * 128, dtype=torch.uint8), ids, ids, lambda: None
+    e.view = w.view
+    big = torch.zeros(2, 3, 2, dtype=torch.int32)
+    return {
+        "linear": lambda s: kx.linear(x, w, stream=s),
+        "experts_gather": lambda s: kx.experts_gather(x, e, 8, ids, stream=s),
+        "experts_combine": lambda s: kx.experts_combine(x, e, 8, ids, x, stream=s),
+        "moe_router": lambda s: kx.moe_router(x, 8, 3, stream=s),
+        "router_group": lambda s: kx.router_group(x, 8, 3, stream=s),
+        "verify_gate_up": lambda s: kx.verify_gate_up(x, x, e, 8, 3, stream=s),
+        "verify_down": lambda s: kx.verify_down(x, e, ids, x, 8, stream=s),
+        "verify_layer": lambda s: kx.verify_layer(x, x, e, e, 8, 3, ids, stream=s),
+        "group_routes": lambda s: kx.group_routes(ids, 8, stream=s),
+        "gather_grouped": lambda s: kx.gather_grouped(x, e, 8, ids, 2, 3, stream=s),
+        "combine_grouped": lambda s: kx.combine_grouped(x, e, 8, ids, x, ids, stream=s),
+        "swiglu": lambda s: kx.swiglu(x, stream=s),
+        "linear_f32w": lambda s: kx.linear_f32w(x, x, stream=s),
+        "linear_bf16w": lambda s: kx.linear_bf16w(x, x, stream=s),
+        "logits_topk": lambda s: kx.logits_topk(x, 64, stream=s),
+        "logits_topk_noalloc": lambda s: kx.logits_topk_noalloc(x, 64, stream=s),
+        "quantize_q4_from_q8": lambda s: kx.quantize_q4_from_q8(w, stream=s),
+        "mtp_pick": lambda s: kx.mtp_pick(x, ids, ids, ids, ids, stream=s),
+        "verify_tail": lambda s: kx.verify_tail(x, 64, 3, ids, drafts=ids[0], stream=s),
+        "mtp_accept": lambda s: kx.mtp_accept(big, ids, ids[0, :1], None, 0.0, 3, 1.0, 64, stream=s),
+    }
+
+
+@pytest.mark.parametrize("name", list(earlier_calls()))
+def test_buffers_of_the_other_operators_belong_to_the_call_s_stream(monkeypatch, name):
+    class Library:
+        def __getattr__(self, name):
+            return lambda *a: 0
+    call = earlier_calls()[name]
+    streams = Streams(monkeypatch)
+    monkeypatch.setattr(kx, "lib", Library)
+    call(Streams.Stream(3))
+    assert streams.made and set(streams.made) == {3}
+    made = len(streams.made)
+    call(None)
+    assert streams.made[made:] == [0] * made
+
+
+def test_a_sync_buffer_that_a_layer_keeps_is_zeroed_on_its_stream(monkeypatch):
+    from strixite_amd import verify
+    streams = Streams(monkeypatch)
+    layer = verify.MoeVerifyLayer.__new__(verify.MoeVerifyLayer)
+    layer._syncs, layer._dev = {}, torch.device("cpu")
+    layer._sync_for(Streams.Stream(4))
+    assert streams.made == [4]
