@@ -123,6 +123,9 @@ extern "C" int sx_kv_append(const sx_head_rows *k_new, const sx_head_rows *v_new
                   (path == nullptr || apart(lens_out, n4, path, 4 * ((cache->batch - 1) * path_ld + max_count)))),
              "lens_out overlaps lens, starts, count, path or the table");
     SX_CHECK(cache->layers * cache->heads * cache->dim <= 0x3fffffff, "layers * heads * dim too large");
+    SX_CHECK(strided_apart(kv_block(c, false), kv_block(c, true)), "the caches of keys and values share memory");
+    SX_CHECK(aligned(starts, 4) && aligned(count, 4) && aligned(path, 4) && aligned(lens_out, 4) && aligned(err, 4),
+             "starts, count, path, lens_out and err must be 4-byte aligned");
     const int e = kv_bytes(*cache);
     Args a;
     a.kn = static_cast<const uint16_t *>(k_new->p), a.kn_l = k_new->layer, a.kn_t = k_new->token, a.kn_h = k_new->head;

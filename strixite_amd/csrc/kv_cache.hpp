@@ -23,6 +23,39 @@ inline bool rows_apart(int64_t dim, std::initializer_list<std::pair<int64_t, int
     return true;
 }
 
+// `bytes` bytes at p, again at each of up to four (count, byte stride) steps.
+struct Strided {
+    const void *p;
+    int64_t bytes;
+    std::pair<int64_t, int64_t> steps[4];
+};
+
+// Whether two such blocks surely share no memory: some of the steps that they have in common (number i of both, of equal
+// count and stride) repeat a piece that holds one block's span and, behind it, the other's. None of them: the whole spans
+// are apart. Interleaved keys and values and slabs of pages and rows are told apart that way.
+inline bool strided_apart(Strided a, Strided b) {
+    auto pa = reinterpret_cast<uintptr_t>(a.p), pb = reinterpret_cast<uintptr_t>(b.p);
+    if (pa > pb) std::swap(a, b), std::swap(pa, pb);
+    for (int common = 0; common < 16; ++common) {
+        __int128 la = a.bytes, lb = b.bytes;
+        std::pair<int64_t, int64_t> outer[4];
+        bool both = true;
+        for (int i = 0; i < 4; ++i) {
+            outer[i] = {1, 0};
+            if (common >> i & 1) {
+                both &= a.steps[i] == b.steps[i] && a.steps[i].first > 1;
+                outer[i] = a.steps[i];
+            } else {
+                la += (__int128)std::max<int64_t>(a.steps[i].first - 1, 0) * a.steps[i].second;
+                lb += (__int128)std::max<int64_t>(b.steps[i].first - 1, 0) * b.steps[i].second;
+            }
+        }
+        const __int128 d = (__int128)pb - pa, piece = d + lb;
+        if (both && la <= d && (common == 0 || (piece < ((__int128)1 << 62) && rows_apart((int64_t)piece, {outer[0], outer[1], outer[2], outer[3]})))) return true;
+    }
+    return false;
+}
+
 inline int kv_bytes(const sx_kv_cache &c) { return c.dtype == SX_KV_E4M3 ? 1 : 2; }
 
 // Why a cache is not one that the kernels take; empty where it is. Pages hold whole 16-token tiles, rows are loaded
@@ -62,6 +95,13 @@ inline std::string head_rows_error(const sx_head_rows &r, const char *name, int6
 
 inline int64_t head_rows_bytes(const sx_head_rows &r, int64_t T, int64_t heads, int64_t dim) {
     return 2 * ((T - 1) * r.token + (heads - 1) * r.head + dim);
+}
+
+// What a cache of all its layers holds for keys (values).
+inline Strided kv_block(const sx_kv_cache &c, bool values) {
+    const int64_t e = kv_bytes(c);
+    if (values) return {c.v, c.dim * e, {{c.layers, c.v_layer * e}, {c.pages, c.v_page * e}, {c.page_size, c.v_token * e}, {c.heads, c.v_head * e}}};
+    return {c.k, c.dim * e, {{c.layers, c.k_layer * e}, {c.pages, c.k_page * e}, {c.page_size, c.k_token * e}, {c.heads, c.k_head * e}}};
 }
 
 }  // namespace sx

@@ -485,3 +485,40 @@ def test_a_sync_buffer_that_a_layer_keeps_is_zeroed_on_its_stream(monkeypatch):
     layer._syncs, layer._dev = {}, torch.device("cpu")
     layer._sync_for(Streams.Stream(4))
     assert streams.made == [4]
+
+
+FAR = 1 << 24  # behind all that the caches of these tests span; nothing is read there
+
+
+def append_far(L, **kw):
+    """kv_append with everything but the caches out of their way."""
+    a = dict(k=FAR, v=FAR + 4096, strides=(128, 64, 0), starts=FAR + 8192, count=FAR + 8448, lens_out=FAR + 8704, err=None)
+    a.update({n[4:]: v for n, v in kw.items() if n.startswith("new_")})
+    c = cache(table=BASE + FAR + 9216, lens=BASE + FAR + 9472, **{n: v for n, v in kw.items() if not n.startswith("new_")})
+    rows = lambda o: ctypes.byref(sx.HeadRows(BASE + o, *a["strides"]))
+    p = lambda o: None if o is None else P(o)
+    return L.sx_kv_append(rows(a["k"]), rows(a["v"]), 4, ctypes.byref(c), p(a["starts"]), p(a["count"]), 2, None, 0,
+                          p(a["lens_out"]), p(a["err"]), None)
+@pytest.mark.parametrize("kw", [
+    dict(v=BASE), dict(v=BASE + 128),                                                # the keys' own, a row on
+    dict(v=BASE + 4096 - 256),                                                       # into the second page
+    dict(k=BASE + 128, v=BASE, k_token=192, v_token=192, k_page=4096, v_page=4096),  # interleaved rows that reach into each other
+    dict(v=BASE + 256, k_token=256, k_page=4096, v_page=4096),                       # beside each other, steps that differ
+    dict(layers=2, k_layer=16384, v_layer=8192),                                     # the second layer's values over the pages
+])
+def test_append_refuses_caches_of_keys_and_values_that_share_memory(L, kw):
+    refused(L, append_far(L, **{**dict(v=BASE + 4 * 4096), **kw}), "keys and values share memory")
+
+
+@pytest.mark.parametrize("kw", [
+    dict(v=BASE + 4 * 4096), dict(k=BASE + 4 * 4096, v=BASE),                        # one behind the other
+    dict(v=BASE + 4096, k_page=4096, v_page=4096),                                   # [pages, 2, page, heads, dim]
+    dict(k=BASE + 4096, v=BASE, k_page=4096, v_page=4096, v_token=64, v_head=1024),  # the same, heads outermost in the values
+    dict(v=BASE + 256, k_page=4096, v_page=4096, k_token=256, v_token=256),          # [pages, page, 2, heads, dim]
+    dict(v=BASE + 128, k_page=4096, v_page=4096, k_token=256, v_token=256, k_head=128, v_head=128),  # [.., heads, 2, dim]
+    dict(layers=3, v=BASE + 16384, k_layer=16384, v_layer=16384),                    # [layers, 2, pages, ..]
+    dict(layers=3, v=BASE + 4096, k_page=12288, v_page=12288, k_layer=4096, v_layer=4096),  # [pages, layers, 2, ..]
+    dict(v=BASE + 16, dtype=sx.KV_E4M3, dim=16, k_head=32, v_head=32, k_token=64, v_token=64),
+])
+def test_append_takes_keys_and_values_in_one_buffer(L, kw):
+    refused(L, append_far(L, new_err=FAR + 9, **kw), "4-byte aligned")  # the last check
