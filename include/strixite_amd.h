@@ -332,7 +332,8 @@ int sx_tree_attention(const sx_head_rows *q, const sx_head_rows *k_new, const sx
 /* The accepted tokens into every layer of the cache: for i < count[b] (device int32 [batch], up to max_count), drafted
  * row starts[b] + path[b * path_ld + i] (path null: starts[b] + i) goes to position lens[b] + i. BF16 rows are copied,
  * E4M3 takes the nearest code of x / scale, saturating at 448. lens is only read; lens_out (nullable, apart from all
- * that is read) gets lens + count. Keys and values of the cache lie apart (in one buffer, interleaved too). The pages for
+ * that is read) gets lens + count. Keys, values (in one
+ * buffer, interleaved too) and k_new, v_new lie apart. The pages for
  * the new positions are the caller's to provide, each to one sequence. A sequence
  * with an impossible word (a run of tokens as above, a count over max_count or the table, a path entry outside the
  * sequence's drafted tokens, a page outside the cache) keeps its length and gets nothing; err (nullable) is then {1,

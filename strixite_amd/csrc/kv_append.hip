@@ -124,6 +124,10 @@ extern "C" int sx_kv_append(const sx_head_rows *k_new, const sx_head_rows *v_new
              "lens_out overlaps lens, starts, count, path or the table");
     SX_CHECK(cache->layers * cache->heads * cache->dim <= 0x3fffffff, "layers * heads * dim too large");
     SX_CHECK(strided_apart(kv_block(c, false), kv_block(c, true)), "the caches of keys and values share memory");
+    for (const bool values : {false, true})  // rows are read while others are written
+        SX_CHECK(strided_apart(rows_block(*k_new, T, c.heads, c.dim, c.layers), kv_block(c, values)) &&
+                     strided_apart(rows_block(*v_new, T, c.heads, c.dim, c.layers), kv_block(c, values)),
+                 "k_new or v_new lies in the cache that is written");
     SX_CHECK(aligned(starts, 4) && aligned(count, 4) && aligned(path, 4) && aligned(lens_out, 4) && aligned(err, 4),
              "starts, count, path, lens_out and err must be 4-byte aligned");
     const int e = kv_bytes(*cache);

@@ -93,6 +93,10 @@ inline std::string head_rows_error(const sx_head_rows &r, const char *name, int6
     return "";
 }
 
+inline Strided rows_block(const sx_head_rows &r, int64_t T, int64_t heads, int64_t dim, int64_t layers = 1) {
+    return {r.p, dim * 2, {{layers, r.layer * 2}, {1, 0}, {T, r.token * 2}, {heads, r.head * 2}}};
+}
+
 inline int64_t head_rows_bytes(const sx_head_rows &r, int64_t T, int64_t heads, int64_t dim) {
     return 2 * ((T - 1) * r.token + (heads - 1) * r.head + dim);
 }

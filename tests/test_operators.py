@@ -522,3 +522,20 @@ def test_append_refuses_caches_of_keys_and_values_that_share_memory(L, kw):
 ])
 def test_append_takes_keys_and_values_in_one_buffer(L, kw):
     refused(L, append_far(L, new_err=FAR + 9, **kw), "4-byte aligned")  # the last check
+
+
+@pytest.mark.parametrize("kw", [
+    dict(new_k=0), dict(new_v=128), dict(new_k=16384 + 4096), dict(new_v=16384 + 8192), dict(new_k=2 * 16384 - 128),
+    dict(new_k=16384 - 1024, new_strides=(128, 64, 0)),                                    # its last row is a row of the values
+    dict(layers=2, k_layer=32768, v_layer=32768, new_k=8192, new_strides=(128, 64, 16384)),  # in the pages of every layer
+])
+def test_append_refuses_new_rows_in_the_cache(L, kw):
+    refused(L, append_far(L, v=BASE + 16384, **kw), "lies in the cache")
+
+
+@pytest.mark.parametrize("kw", [
+    dict(new_k=2 * 16384, new_v=2 * 16384 + 1024),
+    dict(layers=2, k_layer=32768, v_layer=32768, new_k=32768, new_v=33792, new_strides=(128, 64, 32768)),  # a slab a layer: pages, rows
+])
+def test_append_takes_new_rows_beside_the_cache(L, kw):
+    refused(L, append_far(L, v=BASE + 16384, new_err=FAR + 9, **kw), "4-byte aligned")  # the last check
