@@ -320,7 +320,8 @@ typedef struct sx_kv_cache {
  * that a row does not see does not touch it, NaN and infinities included. lse (nullable) [T, Hq] FP32: the natural
  * logarithm of each row's sum of exp(score). Rows behind starts[batch] are left as they are. dim 64, 128 or 256; Hq a
  * multiple of heads; batch up to 1024. ws: sx_tree_attention_workspace_bytes bytes, 16-byte aligned, its contents
- * never read before they are written; one per stream. A sequence with impossible words (a length its table does not
+ * never read before they are written; one per stream. out, lse and ws lie apart from each other and from all that is read
+ * (out may be a slice of the buffer that holds q). A sequence with impossible words (a length its table does not
  * hold, a run of tokens that is negative, over max_new or outside T) or a page outside the cache is not read: its
  * rows come out NaN (none, where the run itself is impossible) and err (nullable) is {1, the length or page, the
  * sequence}. */

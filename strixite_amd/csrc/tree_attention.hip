@@ -828,10 +828,8 @@ int sx_tree_attention(const sx_head_rows *q, const sx_head_rows *k_new, const sx
     SX_CHECK(rows_apart(D, {{T, out->token}, {Hq, out->head}}), "rows of out share memory (strides: token ", out->token, ", head ", out->head, ")");
     SX_CHECK(aligned(mask, 8) && aligned(ws, 16), "mask must be 8-byte and the workspace 16-byte aligned");
     const int64_t out_bytes = head_rows_bytes(*out, T, Hq, D);
-    SX_CHECK(apart(out->p, out_bytes, q->p, head_rows_bytes(*q, T, Hq, D)) &&
-                 apart(out->p, out_bytes, k_new->p, head_rows_bytes(*k_new, T, Hkv, D)) &&
-                 apart(out->p, out_bytes, v_new->p, head_rows_bytes(*v_new, T, Hkv, D)),
-             "out overlaps q, k_new or v_new");
+    const Strided rows[3] = {rows_block(*q, T, Hq, D), rows_block(*k_new, T, Hkv, D), rows_block(*v_new, T, Hkv, D)}, o = rows_block(*out, T, Hq, D);
+    SX_CHECK(strided_apart(o, rows[0]) && strided_apart(o, rows[1]) && strided_apart(o, rows[2]), "out overlaps q, k_new or v_new");
     const Plan p = plan_of(D, Hq / Hkv, Hkv, max_new);
     const Space sp = space_of(p, B, Hkv, D);
     SX_CHECK(ws_bytes >= (size_t)sp.bytes, "workspace of ", ws_bytes, " bytes, needs ", sp.bytes);
@@ -840,6 +838,16 @@ int sx_tree_attention(const sx_head_rows *q, const sx_head_rows *k_new, const sx
     const int64_t most = cache->pages_per_seq * cache->page_size / 64 + 6;  // stages hold 64 keys or more
     const int64_t groups = (max_new * (Hq / Hkv) + p.rows() - 1) / p.rows();
     SX_CHECK(B * groups * most < ((int64_t)1 << 31), "more than 2^31 units of work (B = ", B, ", pages a sequence ", cache->pages_per_seq, ")");
+    // blocks read all of these until the call's last one ends
+    const Strided reads[9] = {rows[0], rows[1], rows[2], kv_block(*cache, false), kv_block(*cache, true),
+                              {mask, (max_new + 63) / 64 * 8, {{1, 0}, {1, 0}, {T, mask_ld * 8}, {1, 0}}},
+                              {starts, 4 * (B + 1), {}}, {cache->lens, 4 * B, {}},
+                              {cache->table, 4 * cache->pages_per_seq, {{1, 0}, {1, 0}, {B, cache->table_ld * 4}, {1, 0}}}};
+    for (const Strided &r : reads)
+        SX_CHECK(strided_apart(o, r) && strided_apart({ws, sp.bytes, {}}, r) && (lse == nullptr || strided_apart({lse, 4 * T * Hq, {}}, r)),
+                 "out, lse or the workspace overlaps the inputs, the cache or its words");
+    SX_CHECK(aligned(starts, 4) && aligned(cache->lens, 4) && aligned(cache->table, 4) && aligned(lse, 4) && aligned(err, 4),
+             "starts, lens, table, lse and err must be 4-byte aligned");
 
     Args a;
     const int e = kv_bytes(*cache);

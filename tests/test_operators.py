@@ -539,3 +539,36 @@ def test_append_refuses_new_rows_in_the_cache(L, kw):
 ])
 def test_append_takes_new_rows_beside_the_cache(L, kw):
     refused(L, append_far(L, v=BASE + 16384, new_err=FAR + 9, **kw), "4-byte aligned")  # the last check
+
+
+def attention_far(L, T=4, err=FAR + 9, **at):
+    """tree_attention with everything apart: offsets of its arguments, those of out with strides."""
+    a = dict(q=(0, 256, 64), k_new=(4096, 128, 64), v_new=(8192, 128, 64), k=16384, v=32768, table=49152, lens=49664, starts=50176,
+             mask=50688, out=(53248, 256, 64), lse=57344, ws=FAR)
+    a.update(at)
+    c = cache(k=BASE + a["k"], v=BASE + a["v"], table=BASE + a["table"], lens=BASE + a["lens"])
+    rows = lambda n: ctypes.byref(sx.HeadRows(BASE + a[n][0], *a[n][1:], 0))
+    return L.sx_tree_attention(rows("q"), rows("k_new"), rows("v_new"), T, 4, ctypes.byref(c), P(a["starts"]), 4, P(a["mask"]), 1,
+                               0.1, rows("out"), P(a["lse"]), P(a["ws"]), 1 << 40, P(err), None)
+
+
+def test_attention_takes_arguments_that_lie_apart(L):
+    refused(L, attention_far(L), "4-byte aligned")  # the last check
+    # one buffer of [tokens, query | key | value | output heads, 64]
+    refused(L, attention_far(L, q=(0, 768, 64), k_new=(512, 768, 64), v_new=(768, 768, 64), out=(1024, 768, 64)), "4-byte aligned")
+
+
+@pytest.mark.parametrize("kw", [
+    *[dict(out=(o, 256, 64)) for o in (16384, 32768 + 8192, 49152, 49664, 50176 - 1920, 50688, 50704)],
+    *[dict(lse=o) for o in (0, 2044, 4096, 8192 + 1020, 16384, 49148, 49152, 49668, 50180, 50684, 50712)],
+    *[dict(ws=o) for o in (0, 4096, 8192, 49152, 49664, 50176, 50688, -4096)],
+    dict(T=3, q=(0, 512, 64), out=(768, 512, 64)),               # in one buffer, its last head the next token's q
+])
+def test_attention_refuses_outputs_in_what_it_reads(L, kw):
+    rc, msg = attention_far(L, **kw), L.sx_last_error().decode()
+    assert rc == sx.SX_EINVAL and "overlap" in msg, msg
+
+
+@pytest.mark.parametrize("kw", [dict(starts=50178), dict(lens=49666), dict(table=49153), dict(lse=57346), dict(err=FAR + 2)])
+def test_attention_refuses_misaligned_words(L, kw):
+    refused(L, attention_far(L, **{"err": FAR + 8, **kw}), "4-byte aligned")
