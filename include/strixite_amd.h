@@ -348,8 +348,8 @@ int sx_kv_append(const sx_head_rows *k_new, const sx_head_rows *v_new, int64_t T
  * runs of E / groups experts) only the top_groups groups with the largest sum of their group_best (1 or 2) best c stay
  * in the choice. ids: the k largest c, larger first; every tie, of groups too, goes to the lower index. coef = s of
  * the chosen ones (without the bias), divided by their sum if renorm (a sum of zero leaves them zero), times factor.
- * Scores and choices are FP64, coef rounded once. Shared slot, errors (a non-finite logit or bias; err nullable) and layouts
- * as sx_moe_router's; factor does not touch the shared slot. groups <= 64, k in 1..min(E, 32), E in 1..1024. */
+ * Scores and choices are FP64, coef rounded once. ids and coef lie apart from each other and from all that is read.
+ * Shared slot, errors (a non-finite logit or bias; err nullable) and layouts as sx_moe_router's; factor does not touch the shared slot. groups <= 64, k in 1..min(E, 32), E in 1..1024. */
 enum sx_score { SX_SCORE_SIGMOID = 0, SX_SCORE_SOFTMAX = 1 };
 int sx_moe_router_scored(const void *logits, int64_t ld, int64_t M, int64_t E, int64_t k, int score, const float *bias,
                          int64_t groups, int64_t top_groups, int64_t group_best, int renorm, float factor,

@@ -219,6 +219,13 @@ extern "C" int sx_moe_router_scored(const void *logits, int64_t ld, int64_t M, i
     const int64_t slots = 4 * M * (k + (shared_logit != nullptr ? 1 : 0)), read = ((M - 1) * ld + E) * act_bytes(act);
     SX_CHECK(apart(ids, slots, coef, slots), "ids and coef are the same buffer or overlap");
     SX_CHECK(apart(ids, slots, logits, read) && apart(coef, slots, logits, read), "ids or coef overlap the logits");
+    SX_CHECK(bias == nullptr || (apart(ids, slots, bias, 4 * E) && apart(coef, slots, bias, 4 * E)), "ids or coef overlap the bias");
+    const int64_t shared_read = ((M - 1) * shared_ld + 1) * act_bytes(act);
+    SX_CHECK(shared_logit == nullptr || (apart(ids, slots, shared_logit, shared_read) && apart(coef, slots, shared_logit, shared_read)),
+             "ids or coef overlap the shared logits");
+    SX_CHECK(aligned(ids, 4) && aligned(coef, 4) && aligned(bias, 4) && aligned(err, 4) && aligned(logits, act_bytes(act)) &&
+                 aligned(shared_logit, act_bytes(act)),
+             "ids, coef, bias and err must be 4-byte aligned, the logits to their elements");
     int P = 64;
     while (P * groups > 64) P >>= 1;
     const int per = (int)(E / groups), need = (per + P - 1) / P;

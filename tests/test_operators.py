@@ -572,3 +572,20 @@ def test_attention_refuses_outputs_in_what_it_reads(L, kw):
 @pytest.mark.parametrize("kw", [dict(starts=50178), dict(lens=49666), dict(table=49153), dict(lse=57346), dict(err=FAR + 2)])
 def test_attention_refuses_misaligned_words(L, kw):
     refused(L, attention_far(L, **{"err": FAR + 8, **kw}), "4-byte aligned")
+
+
+def route_far(L, logits=32768, ids=8192, coef=12288, bias=16384, shared=20480, sld=1, M=64, k=4, err=FAR + 1, act=sx.ACT_F32):
+    return L.sx_moe_router_scored(P(logits), 64, M, 64, k, sx.SCORE_SIGMOID, P(bias), 1, 1, 1, 1, 1.0, P(shared), sld, 64, P(ids),
+                                  P(coef), act, P(err), None)
+
+
+@pytest.mark.parametrize("kw,text", [
+    (dict(bias=12288 + 64 * 5 * 4 - 4), "overlap the bias"), (dict(bias=8192 - 252), "overlap the bias"), (dict(ids=16384), "overlap the bias"),
+    (dict(shared=8192), "overlap the shared"), (dict(shared=12288 - 63 * 4 * 8, sld=8, ids=FAR), "overlap the shared"),
+    (dict(coef=20480 + 252), "overlap the shared"),
+    (dict(), "4-byte aligned"),  # apart: the last check
+    *[({n: o, "err": FAR}, "4-byte aligned") for n, o in
+      (("ids", 8194), ("coef", 12289), ("bias", 16386), ("shared", 20482), ("logits", 32770))],
+])
+def test_routing_refuses_outputs_in_its_bias_or_shared_logits(L, kw, text):
+    refused(L, route_far(L, **kw), text)
