@@ -138,7 +138,10 @@ class VerifyAttention:
 
     def forward(self, x, residual, k_cache, v_cache, table, lens, starts, mask, k_scale=1.0, v_scale=1.0, stream=None):
         """x, residual (None in the first layer) BF16 [T, d]; the rest as tree_attention takes them. Returns (y [T, d],
-        the sum x + residual)."""
+        the sum x + residual). Runs on the layer's device, whichever is current."""
+        if self.norm_w.is_cuda and self._dev.index != torch.cuda.current_device():
+            with torch.cuda.device(self._dev):
+                return self.forward(x, residual, k_cache, v_cache, table, lens, starts, mask, k_scale, v_scale, stream)
         T = x.shape[0]
         assert T <= self.M and lens.numel() <= self.max_seqs
         ws = self._ws_for(stream)

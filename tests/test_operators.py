@@ -589,3 +589,30 @@ def route_far(L, logits=32768, ids=8192, coef=12288, bias=16384, shared=20480, s
 ])
 def test_routing_refuses_outputs_in_its_bias_or_shared_logits(L, kw, text):
     refused(L, route_far(L, **kw), text)
+
+
+def test_verify_attention_runs_on_its_device_whichever_is_current(monkeypatch):
+    from contextlib import contextmanager
+
+    from strixite_amd import verify
+    current, seen = [0], []
+
+    @contextmanager
+    def on(device):
+        before, current[0] = current[0], torch.device(device).index
+        yield
+        current[0] = before
+
+    class OnGpu1:  # in the place of the norm's weight
+        is_cuda = True
+    streams, layer = Streams(monkeypatch), attention_layer()
+    monkeypatch.setattr(torch.cuda, "device", on)
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: current[0])
+    monkeypatch.setattr(verify.VerifyAttention, "_ws_for", lambda self, stream: None)
+    for f in ("add_rms_norm_fp8", "linear_fp8", "tree_attention", "linear"):
+        monkeypatch.setattr(verify.kx, f, lambda *a, **kw: seen.append(current[0]))
+    layer.norm_w, layer._dev, layer.rotate = OnGpu1, torch.device("cuda", 1), lambda q, k: seen.append(current[0])
+    args = (torch.zeros(4, 128), None, None, None, None, torch.zeros(1, dtype=torch.int32), None, None)
+    layer.forward(*args)
+    layer.forward(*args, stream=streams.default)
+    assert seen == [1] * 10 and current == [0]
