@@ -54,6 +54,9 @@ class MoeVerifyLayer:
         return self.fused and kx.verify_supported(M, self.k, self.E, self.k, self.E, self.gate_up, self.down)
 
     def forward(self, x, stream=None):
+        if self.Wr.is_cuda and self._dev.index != torch.cuda.current_device():
+            with torch.cuda.device(self._dev):
+                return self.forward(x, stream)
         M = x.shape[0]
         assert M <= self.M
         ws = self.ws if M == self.M else self.ws[:kx.route_workspace_bytes(M, self.k, self.E) // 4]

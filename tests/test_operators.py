@@ -616,3 +616,30 @@ def test_verify_attention_runs_on_its_device_whichever_is_current(monkeypatch):
     layer.forward(*args)
     layer.forward(*args, stream=streams.default)
     assert seen == [1] * 10 and current == [0]
+
+
+@pytest.mark.parametrize("M,routing", [(3, dict(score="softmax")), (3, None), (2000, None)])
+def test_moe_verify_layer_runs_on_its_device_whichever_is_current(monkeypatch, M, routing):
+    from contextlib import contextmanager
+
+    from strixite_amd import verify
+    current, seen = [0], []
+
+    @contextmanager
+    def on(device):
+        before, current[0] = current[0], torch.device(device).index
+        yield
+        current[0] = before
+
+    class OnGpu1:  # in the place of the router's weight
+        is_cuda = True
+    gate_up, down = Weight(4 * 256), Weight(4 * 128)
+    layer = verify.MoeVerifyLayer(torch.zeros(4, 128), gate_up, down, 4, 2, M, routing=routing)
+    monkeypatch.setattr(torch.cuda, "device", on)
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: current[0])
+    for f in ("linear_f32w", "moe_router_scored", "group_routes", "router_group", "moe_router", "gather_grouped", "combine_grouped"):
+        monkeypatch.setattr(verify.kx, f, lambda *a, **kw: seen.append(current[0]))
+    monkeypatch.setattr(verify.MoeVerifyLayer, "_fused", lambda self, M: False)
+    layer.Wr, layer._dev = OnGpu1, torch.device("cuda", 1)
+    layer.forward(torch.zeros(M, 128))
+    assert len(seen) >= 4 and set(seen) == {1} and current == [0]
