@@ -299,7 +299,8 @@ enum sx_kv_dtype { SX_KV_BF16 = 0, SX_KV_E4M3 = 1 };
 /* A paged cache of keys and values: position p of sequence b is row p % page_size of page table[b, p / page_size],
  * at k[layer * k_layer + page * k_page + row * k_token + head * k_head + d] (strides in elements, multiples of 16
  * bytes, any order; v alike). page_size a power of two, 16 to 65536. table [batch, pages_per_seq] with row stride
- * table_ld and lens [batch] (cached tokens) are device int32. E4M3: value = code * k_scale (v_scale). */
+ * table_ld and lens [batch] (cached tokens) are device int32. E4M3: value = code * k_scale (v_scale), both 2^-100 to
+ * 2^100. */
 typedef struct sx_kv_cache {
     void *k, *v;
     int32_t dtype;

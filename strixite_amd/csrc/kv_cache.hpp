@@ -80,8 +80,9 @@ inline std::string kv_cache_error(const sx_kv_cache &c) {
     if (!aligned(c.k, 16) || !aligned(c.v, 16)) return "the cache must be 16-byte aligned";
     if (c.k_token * e * c.page_size > 0x7fffffff || c.v_token * e * c.page_size > 0x7fffffff)
         return "a page spans more than 2^31 bytes";
-    if (c.dtype == SX_KV_E4M3 && !(std::isfinite(c.k_scale) && c.k_scale > 0.f && std::isfinite(c.v_scale) && c.v_scale > 0.f))
-        return cat("k_scale = ", c.k_scale, ", v_scale = ", c.v_scale, ", expected positive");
+    // inside them the reciprocals, and the products with a softmax's terms, stay in FP32's range
+    if (c.dtype == SX_KV_E4M3 && !(c.k_scale >= 0x1p-100f && c.k_scale <= 0x1p100f && c.v_scale >= 0x1p-100f && c.v_scale <= 0x1p100f))
+        return cat("k_scale = ", c.k_scale, ", v_scale = ", c.v_scale, ", expected 2^-100..2^100");
     return "";
 }
 

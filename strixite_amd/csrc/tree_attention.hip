@@ -819,7 +819,9 @@ int sx_tree_attention(const sx_head_rows *q, const sx_head_rows *k_new, const sx
     SX_CHECK(T >= 1 && T <= 0x7fffffff, "T = ", T, " rows of drafted tokens");
     SX_CHECK(k_new->token <= (1 << 21) && v_new->token <= (1 << 21), "token strides of k_new and v_new up to 2^21 elements (", k_new->token, ", ", v_new->token, ")");
     SX_CHECK(mask_ld >= (max_new + 63) / 64, "mask_ld = ", mask_ld, " words a token for max_new = ", max_new);
-    SX_CHECK(std::isfinite(scale) && scale > 0.f, "scale = ", scale, ", expected positive");
+    const float scale2 = scale * 1.4426950408889634f;  // the kernels work in powers of two
+    SX_CHECK(scale > 0.f && std::isnormal(scale2) && (cache->dtype != SX_KV_E4M3 || std::isnormal(scale2 * cache->k_scale)),
+             "scale = ", scale, ", expected positive and, times k_scale, a normal number");
     why = head_rows_error(*q, "q", Hq, D);
     if (why.empty()) why = head_rows_error(*k_new, "k_new", Hkv, D);
     if (why.empty()) why = head_rows_error(*v_new, "v_new", Hkv, D);
@@ -866,7 +868,7 @@ int sx_tree_attention(const sx_head_rows *q, const sx_head_rows *k_new, const sx
     a.B = (int32_t)B, a.T = (int32_t)T, a.G = (int32_t)(Hq / Hkv), a.P = (int32_t)cache->pages_per_seq;
     a.pages = (int32_t)cache->pages, a.page_shift = __builtin_ctzll((uint64_t)cache->page_size);
     a.max_new = (int32_t)max_new, a.nb = p.nb, a.heads = (int32_t)Hq;
-    a.scale = scale * 1.4426950408889634f, a.k_scale = cache->k_scale, a.v_scale = cache->v_scale;
+    a.scale = scale2, a.k_scale = cache->k_scale, a.v_scale = cache->v_scale;
     const bool f8 = cache->dtype == SX_KV_E4M3;
     hipStream_t s = stream_of(stream);
     if (D == 64) launch_rows<64>(p, a, Hkv, f8, s);

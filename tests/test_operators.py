@@ -643,3 +643,19 @@ def test_moe_verify_layer_runs_on_its_device_whichever_is_current(monkeypatch, M
     layer.Wr, layer._dev = OnGpu1, torch.device("cuda", 1)
     layer.forward(torch.zeros(M, 128))
     assert len(seen) >= 4 and set(seen) == {1} and current == [0]
+
+
+@pytest.mark.parametrize("bad", [1e-45, 2.9e-39, 2.0 ** -101, 2.0 ** 101, float("inf"), float("nan"), -1.0])
+def test_scales_of_a_cache_that_fp32_cannot_divide_by_are_refused(L, bad):
+    for kw in (dict(k_scale=bad), dict(v_scale=bad)):
+        refused(L, attention(L, c=cache(dtype=sx.KV_E4M3, **kw), ws=100), "expected 2^-100..2^100")
+        refused(L, append(L, c=cache(dtype=sx.KV_E4M3, **kw), max_count=0), "expected 2^-100..2^100")
+        refused(L, attention(L, c=cache(**kw), ws=100), "workspace of 100")  # a BF16 cache has none
+    edge = dict(k_scale=2.0 ** -100, v_scale=2.0 ** 100)
+    refused(L, attention(L, c=cache(dtype=sx.KV_E4M3, **edge), ws=100), "workspace of 100")
+
+
+@pytest.mark.parametrize("scale,k_scale,dtype", [(1e-45, 1.0, sx.KV_BF16), (3e38, 1.0, sx.KV_BF16), (1e-10, 2.0 ** -99, sx.KV_E4M3),
+                                                 (1e10, 2.0 ** 100, sx.KV_E4M3)])
+def test_a_scale_of_scores_outside_the_normal_numbers_is_refused(L, scale, k_scale, dtype):
+    refused(L, attention(L, c=cache(dtype=dtype, k_scale=k_scale), scale=scale, ws=100), "a normal number")
