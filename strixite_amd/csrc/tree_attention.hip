@@ -723,8 +723,13 @@ __global__ void __launch_bounds__(kJoinThreads) tree_attn_join_kernel(const Args
 // 64 68.4 / 75.9, 96 78.5 / 82.8, 128 83.2 / 89.2, 192 alike; FP8 at 131,072: 48 rows 81 / 96, 128 121 / 134). 256 rows, and
 // more than 64 at D = 256, take a block of eight waves (D = 256, 128 rows: 103 / 114).
 struct Plan {
-    int nt, wr, nb;
+    int nt, wr, nb, hs;  // hs: bytes of keys (of values) a stage
     int64_t rows() const { return 16 * nt * wr; }
+    // units of a sequence's row group, stages as Lay deals them
+    int64_t units(int64_t D, int e, int64_t cached, int64_t max_new) const {
+        const int64_t keys = std::min<int64_t>(hs / (D * e), 256), fresh = std::min<int64_t>(hs / (2 * D), 256);
+        return (cached + keys - 1) / keys + (max_new + fresh - 1) / fresh;
+    }
 };
 Plan plan_of(int64_t D, int64_t G, int64_t Hkv, int64_t max_new) {
     Plan p;
@@ -738,6 +743,7 @@ Plan plan_of(int64_t D, int64_t G, int64_t Hkv, int64_t max_new) {
     }
     const int per_cu = D == 256 ? (p.wr == 4 && p.nt == 1 ? 2 : 1) : p.wr == 2 || p.wr == 4 ? 2 : 1;
     p.nb = (int)std::max<int64_t>(1, (int64_t)device_cus() * per_cu / Hkv);
+    p.hs = per_cu == 2 ? 16384 : 32768;
     return p;
 }
 
@@ -837,7 +843,7 @@ int sx_tree_attention(const sx_head_rows *q, const sx_head_rows *k_new, const sx
     SX_CHECK(ws_bytes >= (size_t)sp.bytes, "workspace of ", ws_bytes, " bytes, needs ", sp.bytes);
     SX_CHECK(apart(ws, sp.bytes, out->p, out_bytes) && (lse == nullptr || (apart(lse, 4 * T * Hq, ws, sp.bytes) && apart(lse, 4 * T * Hq, out->p, out_bytes))),
              "out, lse and the workspace overlap");
-    const int64_t most = cache->pages_per_seq * cache->page_size / 64 + 6;  // stages hold 64 keys or more
+    const int64_t most = p.units(D, kv_bytes(*cache), cache->pages_per_seq * cache->page_size, max_new);
     const int64_t groups = (max_new * (Hq / Hkv) + p.rows() - 1) / p.rows();
     SX_CHECK(B * groups * most < ((int64_t)1 << 31), "more than 2^31 units of work (B = ", B, ", pages a sequence ", cache->pages_per_seq, ")");
     // blocks read all of these until the call's last one ends

@@ -659,3 +659,21 @@ def test_scales_of_a_cache_that_fp32_cannot_divide_by_are_refused(L, bad):
                                                  (1e10, 2.0 ** 100, sx.KV_E4M3)])
 def test_a_scale_of_scores_outside_the_normal_numbers_is_refused(L, scale, k_scale, dtype):
     refused(L, attention(L, c=cache(dtype=dtype, k_scale=k_scale), scale=scale, ws=100), "a normal number")
+
+
+@pytest.mark.parametrize("D,Hq,Hkv,max_new,dtype,keys", [  # keys: a stage's, by the tile that the rows take
+    (256, 8, 1, 8, sx.KV_BF16, 32), (256, 8, 1, 8, sx.KV_E4M3, 64), (256, 4, 1, 8, sx.KV_BF16, 64), (128, 4, 1, 8, sx.KV_BF16, 128),
+    (128, 8, 1, 8, sx.KV_BF16, 64), (128, 8, 1, 8, sx.KV_E4M3, 128), (64, 4, 1, 8, sx.KV_E4M3, 256), (64, 4, 1, 256, sx.KV_BF16, 256),
+])
+def test_attention_counts_the_stages_of_its_tile(L, D, Hq, Hkv, max_new, dtype, keys):
+    groups = -(-max_new * Hq // 256)
+    for pages, ok in ((2 ** 30 // 1024 // 16 * keys // groups, True), (2 ** 31 // 1024 // 16 * keys // groups, False)):
+        e, far = (1 if dtype else 2), 1 << 44
+        if pages * 16 > 2 ** 31 - 65536 - 16:
+            continue  # no sequence is that long
+        c = cache(dtype=dtype, k=BASE + far, v=BASE + 2 * far, heads=Hkv, dim=D, k_page=16 * D, v_page=16 * D, k_token=D, v_token=D,
+                  k_head=D, v_head=D, table=BASE + 3 * far, table_ld=pages, pages_per_seq=pages, lens=BASE + 4 * far, batch=1024)
+        rows = lambda o, t: ctypes.byref(sx.HeadRows(BASE + o, t, D, 0))
+        rc = L.sx_tree_attention(rows(0, Hq * D), rows(1 << 24, D), rows(2 << 24, D), 4, Hq, ctypes.byref(c), P(3 << 24), max_new,
+                                 P(4 << 24), 4, 0.1, rows(5 << 24, Hq * D), None, P(6 << 24), 1 << 40, P(1), None)
+        refused(L, rc, "4-byte aligned" if ok else "more than 2^31 units")
