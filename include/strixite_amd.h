@@ -314,7 +314,7 @@ typedef struct sx_kv_cache {
     int64_t batch;
 } sx_kv_cache;
 /* Attention of drafted tokens: sequence b's are rows starts[b] .. starts[b + 1] - 1 (device int32 [batch + 1]) of q
- * [T, Hq, dim], k_new and v_new [T, heads, dim]; none to max_new (1..256) of them, T bounds them all. Token t sees
+ * [T, Hq, dim], k_new and v_new [T, heads, dim]; none to max_new (1..256) of them, T (under 2^24) bounds them all. Token t sees
  * every cached token of its sequence and, of the drafted ones, number j of the sequence where bit j % 64 of
  * mask[t * mask_ld + j / 64] is set (its ancestors and itself for a tree; a chain: all up to itself). out = softmax(
  * scale * q k^T) v per query head h over key head h / (Hq / heads); a row that sees nothing is zero. A drafted token

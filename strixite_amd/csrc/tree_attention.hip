@@ -822,7 +822,8 @@ int sx_tree_attention(const sx_head_rows *q, const sx_head_rows *k_new, const sx
     const char *bad = shape_error(B, Hq, Hkv, D, max_new);
     SX_CHECK(bad == nullptr, bad, " (B = ", B, ", Hq = ", Hq, ", Hkv = ", Hkv, ", D = ", D, ", max_new = ", max_new, ")");
     SX_CHECK(cache->layers == 1, "layers = ", cache->layers, ": attention takes one layer's cache");
-    SX_CHECK(T >= 1 && T <= 0x7fffffff, "T = ", T, " rows of drafted tokens");
+    // a launch has fewer than 2^32 threads a dimension: the join's is T blocks (the sequences' own are 2^18 rows at most)
+    SX_CHECK(T >= 1 && T < ((int64_t)1 << 32) / kJoinThreads, "T = ", T, " rows of drafted tokens, expected 1..", ((int64_t)1 << 32) / kJoinThreads - 1);
     SX_CHECK(k_new->token <= (1 << 21) && v_new->token <= (1 << 21), "token strides of k_new and v_new up to 2^21 elements (", k_new->token, ", ", v_new->token, ")");
     SX_CHECK(mask_ld >= (max_new + 63) / 64, "mask_ld = ", mask_ld, " words a token for max_new = ", max_new);
     const float scale2 = scale * 1.4426950408889634f;  // the kernels work in powers of two

@@ -677,3 +677,8 @@ def test_attention_counts_the_stages_of_its_tile(L, D, Hq, Hkv, max_new, dtype, 
         rc = L.sx_tree_attention(rows(0, Hq * D), rows(1 << 24, D), rows(2 << 24, D), 4, Hq, ctypes.byref(c), P(3 << 24), max_new,
                                  P(4 << 24), 4, 0.1, rows(5 << 24, Hq * D), None, P(6 << 24), 1 << 40, P(1), None)
         refused(L, rc, "4-byte aligned" if ok else "more than 2^31 units")
+
+
+def test_attention_refuses_more_rows_than_its_second_launch_has_blocks(L):
+    refused(L, attention(L, T=1 << 24, ws=100), "expected 1..16777215")
+    refused(L, attention(L, T=(1 << 24) - 1, ws=100, out=(1 << 40, 256, 64)), "workspace of 100")
