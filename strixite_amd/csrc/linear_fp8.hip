@@ -40,10 +40,12 @@ __device__ __forceinline__ bf16x8 as_bf16x8(int lo, int hi) {
     return __builtin_bit_cast(bf16x8, u32x4{pair(lo, false), pair(lo, true), pair(hi, false), pair(hi, true)});
 }
 
-// A block's products of 16 rows and 16 tokens. The FP8 instructions keep fewer bits than FP32 of the products of one
-// block (1.4e-5 of the result, root mean square, on random codes): a hundredth of a BF16 output's rounding, but far
-// over an FP32 output's. FP32 outputs take the codes as BF16, exact there, whose products are summed in FP32 (a quarter
-// of the rate; they are logits of few tokens, bound by the weight's bytes).
+// A block's products of 16 rows and 16 tokens. The FP8 instruction keeps fewer bits than FP32: the products of eight
+// neighbouring codes are cut, toward zero, at 2^-13 of the largest one's power of two (2^(ex + ew), codes under 2^-6 counted
+// as 2^-6), so a block is off by 2^-10 of its sum of |products| at most, by 1.4e-5 of its result (root mean square) on random
+// codes: a hundredth of a BF16 output's rounding there, but more where large products cancel, and far over an FP32 output's
+// rounding. FP32 outputs take the codes as BF16, exact there, whose products are summed in FP32 (half the rate: a K block
+// of the tiles takes 1.5 to 1.6 times as long; these are logits of few tokens, bound by the weight's bytes).
 template <bool F32>
 __device__ __forceinline__ f32x4 block_products(i32x8 a, i32x8 b) {
     f32x4 d = {0.f, 0.f, 0.f, 0.f};

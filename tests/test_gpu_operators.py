@@ -886,3 +886,31 @@ def test_verify_attention_on_two_streams_at_once():
         torch.cuda.synchronize()
         for w, g in zip(want, got):
             assert all(torch.equal(p, q) for p, q in zip(w, g))
+
+
+@pytest.mark.parametrize("M", [6, 40, 100, 600])  # rows, rows of 32, the tiles
+def test_linear_fp8_where_large_products_cancel(M):
+    """+-448 * 448 beside small products inside a block. BF16 outputs: a product loses less than 2^-13 of the largest power of
+    two 2^(ex + ew) among its eight neighbours (codes under 2^-6 as 2^-6), so 8 of that a group, and the output's rounding; FP32
+    outputs (K / 32 + 8) u32 S, as ever. The group's own sums: (K / 8 + 8) u32 S."""
+    print(f"linear_fp8 cancelling M={M}", flush=True)
+    N, K = 256, 256
+    g = gen(M)
+    code = lambda r: (torch.randn(r, K, device="cuda", generator=g) * 100 *
+                      2.0 ** torch.randint(-12, 1, (r, K), device="cuda", generator=g)).clamp(-448, 448).to(F8).float()
+    x, w = code(M), code(N)
+    x[:, 8::32], x[:, 9::32] = 448, 448
+    w[:, 8::32], w[:, 9::32] = 448, -448
+    x[0, :], x[0, 8:10] = 7.5, 448            # one group: six of 7.5, each just under the cut beside the pair
+    w[0, :], w[0, 8], w[0, 9], w[0, 10:16] = 0, 448, -448, 1
+    one = torch.ones(N // 128, K // 128, device="cuda")
+    weight, xs = kx.Fp8Weight(w.to(F8), one), torch.ones(M, K // 128, device="cuda")
+    ref, S = x.double() @ w.double().T, x.double().abs() @ w.double().abs().T
+    power = lambda t: torch.floor(torch.log2(t.abs().clamp(min=2.0 ** -6)))
+    cut = torch.zeros(M, N, dtype=torch.float64, device="cuda")
+    for k in range(0, K, 8):
+        cut += 2.0 ** -10 * torch.exp2((power(x[:, None, k:k + 8]) + power(w[None, :, k:k + 8])).amax(2)).double()
+    y = kx.linear_fp8(x.to(F8), xs, weight).double()
+    assert ((y - ref).abs() <= U16 * ref.abs() + cut + (K / 8 + 8) * U32 * S).all()
+    y = kx.linear_fp8(x.to(F8), xs, weight, out_act=ACT_F32).double()
+    assert ((y - ref).abs() <= (K / 32 + 8) * U32 * S).all() and float(y[0, 0]) == 45.0
