@@ -46,6 +46,14 @@ def _empty(like, shape, dtype, stream, fill=None):
     return t if fill is None else t.fill_(fill)
 
 
+def _empty_like(like, stream):
+    """_empty in like's own shape and type (half of the host time)."""
+    if stream is not None:
+        with torch.cuda.stream(stream):
+            return torch.empty_like(like)
+    return torch.empty_like(like)
+
+
 class QWeight:
     """A q4 / q8 weight resident on the device (Q4Device / Q8Device, runtime/q4_device.hpp:23-36): codes uint8,
     scale / min as BF16 bits (int16 tensors), in the formats/q4.hpp / q8.hpp layout."""
@@ -506,7 +514,7 @@ def add_rms_norm_fp8(x, weight, eps=1e-6, residual=None, residual_out=None, w_ad
     if residual is not None:
         _is("residual", residual, dtype, shape)
         if residual_out is None:
-            residual_out = _empty(x, shape, dtype, stream)
+            residual_out = _empty_like(residual, stream)
         else:
             _is("residual_out", residual_out, dtype, shape)
     elif residual_out is not None:
@@ -673,7 +681,7 @@ def kv_append(k_new, v_new, k_cache, v_cache, table, lens, starts, count, path=N
     elif max_count is None:
         _refuse("max_count is needed without a path")
     if lens_out is None:
-        lens_out = _empty(lens, (B,), torch.int32, stream)
+        lens_out = _empty_like(lens, stream)
     else:
         _is("lens_out", lens_out, torch.int32, (B,))
     _is_err(err)
