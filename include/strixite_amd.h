@@ -321,7 +321,9 @@ typedef struct sx_kv_cache {
  * every cached token of its sequence and, of the drafted ones, number j of the sequence where bit j % 64 of
  * mask[t * mask_ld + j / 64] is set (its ancestors and itself for a tree; a chain: all up to itself). out = softmax(
  * scale * q k^T) v per query head h over key head h / (Hq / heads); a row that sees nothing is zero. A drafted token
- * that a row does not see does not touch it, NaN and infinities included. lse (nullable) [T, Hq] FP32: the natural
+ * that a row does not see does not touch it, NaN and infinities included (an infinite value that it sees may come out as
+ * NaN). Scores, maxima and sums are FP32; softmax terms meet BF16 values to 2^-17 where max_new * Hq / heads <= 64 and
+ * rounded to BF16 above, E4M3 values in FP16 (2^-12; 2^-32 of a row's maximum and less may be lost). lse (nullable) [T, Hq] FP32: the natural
  * logarithm of each row's sum of exp(score). Rows behind starts[batch] are left as they are. dim 64, 128 or 256; Hq a
  * multiple of heads; batch up to 1024. ws: sx_tree_attention_workspace_bytes bytes, 16-byte aligned, its contents
  * never read before they are written; one per stream. out, lse and ws lie apart from each other and from all that is read
@@ -336,7 +338,7 @@ int sx_tree_attention(const sx_head_rows *q, const sx_head_rows *k_new, const sx
                       uint32_t *err, sx_stream stream);
 /* The accepted tokens into every layer of the cache: for i < count[b] (device int32 [batch], up to max_count), drafted
  * row starts[b] + path[b * path_ld + i] (path null: starts[b] + i) goes to position lens[b] + i. BF16 rows are copied,
- * E4M3 takes the nearest code of x / scale, saturating at 448. lens is only read; lens_out (nullable, apart from all
+ * E4M3 takes the nearest code of x / scale (one FP32 division), saturating at 448. lens is only read; lens_out (nullable, apart from all
  * that is read) gets lens + count. Keys, values (in one
  * buffer, interleaved too) and k_new, v_new lie apart. The pages for
  * the new positions are the caller's to provide, each to one sequence. A sequence

@@ -368,7 +368,8 @@ __global__ void __launch_bounds__(64 * WR * WK, HS < 32768 || WR * WK > 4 ? 2 : 
     using C_ = Lay<D, F8, HS>;     // cached stages
     using N_ = Lay<D, false, HS>;  // drafted stages
     // BF16 values meet P in two terms where there are few rows and products to spare (at 16 rows and 65,536 keys the time
-    // is the same), else in one: the output's error is its own rounding, or 1.4 times that
+    // is the same), else in one, rounded as the values are: the output's error is its own rounding, or 1.4 times that (two
+    // above 64 rows too: 8 to 23 % slower, 96 rows 78.7 -> 92 us)
     constexpr int kWaves = WR * WK, ROWS = 16 * NT * WR, KEYS = C_::KEYS, FRESH = N_::KEYS, VEC = D / 16, BF16_TERMS = ROWS <= 64 ? 2 : 1;
     static_assert(WK / 2 * WR <= 4, "an array for each pair of waves that meet");
     // one array a stage and operand, so that the wait-count pass tells a stage's loads apart from the other's

@@ -15,7 +15,7 @@ class MoeVerifyLayer:
     buffer the layer owns) -> down + combine (the sequence qwen4exp.cpp:1139-1163 runs below kGroupedMinTokens). Otherwise (or fused=False): router projection -> moe_router + moe_group_routes -> grouped
     gate_up with the SwiGLU epilogue -> grouped down + combine. routing (optional): a dict of moe_router_scored's score,
     bias, groups, top_groups, group_best, renorm and factor; the layer then routes by those scores (grouped experts at
-    every width) and not by moe_router."""
+    every width) and not by moe_router. The layer has one set of buffers: forwards on different streams have to be ordered."""
 
     def __init__(self, Wr, gate_up, down, E, k, max_tokens, act_dtype=torch.bfloat16, fused=True, routing=None):
         self.Wr, self.gate_up, self.down, self.E, self.k = Wr, gate_up, down, E, k
