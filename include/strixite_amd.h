@@ -323,8 +323,8 @@ typedef struct sx_kv_cache {
  * scale * q k^T) v per query head h over key head h / (Hq / heads); a row that sees nothing is zero. A drafted token
  * that a row does not see does not touch it, NaN and infinities included (an infinite value that it sees may come out as
  * NaN). Scores, maxima and sums are FP32; softmax terms meet BF16 values to 2^-17 where max_new * Hq / heads <= 64 and
- * rounded to BF16 above, E4M3 values in FP16 (2^-12; 2^-32 of a row's maximum and less may be lost). lse (nullable) [T, Hq] FP32: the natural
- * logarithm of each row's sum of exp(score). Rows behind starts[batch] are left as they are. dim 64, 128 or 256; Hq a
+ * rounded to BF16 above, E4M3 values in FP16 (2^-12; 2^-32 of a row's maximum and less may be lost). lse (nullable) [T,
+ * Hq] FP32: the natural logarithm of each row's sum of exp(score). Rows behind starts[batch] are left as they are. dim 64, 128 or 256; Hq a
  * multiple of heads; batch up to 1024. ws: sx_tree_attention_workspace_bytes bytes, 16-byte aligned, its contents
  * never read before they are written; one per stream. out, lse and ws lie apart from each other and from all that is read
  * (out may be a slice of the buffer that holds q). A sequence with impossible words (a length its table does not
@@ -355,7 +355,8 @@ int sx_kv_append(const sx_head_rows *k_new, const sx_head_rows *v_new, int64_t T
  * in the choice. ids: the k largest c, larger first; every tie, of groups too, goes to the lower index. coef = s of
  * the chosen ones (without the bias), divided by their sum if renorm (a sum of zero leaves them zero), times factor.
  * Scores and choices are FP64, coef rounded once. ids and coef lie apart from each other and from all that is read.
- * Shared slot, errors (a non-finite logit or bias; err nullable) and layouts as sx_moe_router's; factor does not touch the shared slot. groups <= 64, k in 1..min(E, 32), E in 1..1024. */
+ * Shared slot, errors (a non-finite logit or bias; err nullable) and layouts as sx_moe_router's; factor does not touch
+ * the shared slot. groups <= 64, k in 1..min(E, 32), E in 1..1024. */
 enum sx_score { SX_SCORE_SIGMOID = 0, SX_SCORE_SOFTMAX = 1 };
 int sx_moe_router_scored(const void *logits, int64_t ld, int64_t M, int64_t E, int64_t k, int score, const float *bias,
                          int64_t groups, int64_t top_groups, int64_t group_best, int renorm, float factor,

@@ -129,8 +129,9 @@ extern "C" int sx_kv_append(const sx_head_rows *k_new, const sx_head_rows *v_new
         SX_CHECK(strided_apart(rows_block(*k_new, T, c.heads, c.dim, c.layers), kv_block(c, values)) &&
                      strided_apart(rows_block(*v_new, T, c.heads, c.dim, c.layers), kv_block(c, values)),
                  "k_new or v_new lies in the cache that is written");
-    SX_CHECK(aligned(starts, 4) && aligned(count, 4) && aligned(path, 4) && aligned(lens_out, 4) && aligned(err, 4),
-             "starts, count, path, lens_out and err must be 4-byte aligned");
+    SX_CHECK(aligned(starts, 4) && aligned(count, 4) && aligned(path, 4) && aligned(lens_out, 4) && aligned(c.lens, 4) && aligned(c.table, 4) &&
+                 aligned(err, 4),
+             "starts, count, path, lens, the table, lens_out and err must be 4-byte aligned");
     const int e = kv_bytes(*cache);
     Args a;
     a.kn = static_cast<const uint16_t *>(k_new->p), a.kn_l = k_new->layer, a.kn_t = k_new->token, a.kn_h = k_new->head;

@@ -494,7 +494,7 @@ def append_far(L, **kw):
     """kv_append with everything but the caches out of their way."""
     a = dict(k=FAR, v=FAR + 4096, strides=(128, 64, 0), starts=FAR + 8192, count=FAR + 8448, lens_out=FAR + 8704, err=None)
     a.update({n[4:]: v for n, v in kw.items() if n.startswith("new_")})
-    c = cache(table=BASE + FAR + 9216, lens=BASE + FAR + 9472, **{n: v for n, v in kw.items() if not n.startswith("new_")})
+    c = cache(**{"table": BASE + FAR + 9216, "lens": BASE + FAR + 9472, **{n: v for n, v in kw.items() if not n.startswith("new_")}})
     rows = lambda o: ctypes.byref(sx.HeadRows(BASE + o, *a["strides"]))
     p = lambda o: None if o is None else P(o)
     return L.sx_kv_append(rows(a["k"]), rows(a["v"]), 4, ctypes.byref(c), p(a["starts"]), p(a["count"]), 2, None, 0,
@@ -682,3 +682,9 @@ def test_attention_counts_the_stages_of_its_tile(L, D, Hq, Hkv, max_new, dtype, 
 def test_attention_refuses_more_rows_than_its_second_launch_has_blocks(L):
     refused(L, attention(L, T=1 << 24, ws=100), "expected 1..16777215")
     refused(L, attention(L, T=(1 << 24) - 1, ws=100, out=(1 << 40, 256, 64)), "workspace of 100")
+
+
+@pytest.mark.parametrize("kw", [dict(new_starts=FAR + 8193), dict(new_count=FAR + 8450), dict(new_lens_out=FAR + 8707), dict(table=BASE + FAR + 9218),
+                                dict(lens=BASE + FAR + 9473), dict(new_err=FAR + 9)])
+def test_append_refuses_misaligned_words(L, kw):
+    refused(L, append_far(L, v=BASE + 16384, **{"new_err": FAR + 9728, **kw}), "4-byte aligned")
