@@ -363,6 +363,108 @@ int sx_moe_router_scored(const void *logits, int64_t ld, int64_t M, int64_t E, i
                          const void *shared_logit, int64_t shared_ld, int32_t shared_id, int32_t *ids, float *coef,
                          int act, uint32_t *err, sx_stream stream);
 
+/* Acceptance of drafted tokens against the target's probabilities (rejection sampling; sx_mtp_accept compares a sample with the
+ * draft, this keeps what the draft's probabilities allow). Sequence b's rows are starts[b] .. starts[b + 1] - 1 (device int32
+ * [batch + 1], none to max_rows, 1..256) of logits [T, >= n_valid] (act, rows ld apart); drafts[t] is the token proposed behind row t
+ * (a sequence's last row has none), draft_logits [T, >= n_draft] (nullable: the draft was certain) what it was drawn from,
+ * n_draft <= n_valid (the rest of the vocabulary: probability 0). With p, q the softmax of a row of each over temperature[b] and u
+ * [T, 2] FP64 in [0, 1): draft d of row t stays if u[t, 0] q(d) < p(d). At the first that does not, a token from max(p - q, 0), behind the
+ * last draft one from p: the first place at which the running sum passes u[t, 1] times the total. temperature 0 or less: a draft
+ * stays if it is the row's largest logit (ties: the lowest place), which is the token otherwise. Probabilities and sums are FP64.
+ * tokens [batch, max_rows]: the drafts that stay, the token, then -1; count: how many; status 0. A row that counts and holds NaN or
+ * no finite largest logit, a draft outside the vocabulary or a temperature that is not finite: status 1 + the row, count and tokens
+ * the drafts before it. Impossible starts: status -1, count 0. ws: sx_mtp_accept_sampled_workspace_bytes, 16-byte aligned, never read
+ * before it is written; one per stream. T up to 32767, batch up to 1024. */
+int sx_mtp_accept_sampled_workspace_bytes(int64_t T, int64_t batch, int64_t n_valid, int64_t n_draft, size_t *bytes);
+int sx_mtp_accept_sampled(const void *logits, int64_t ld, int64_t T, int64_t n_valid, const void *draft_logits, int64_t draft_ld,
+                          int64_t n_draft, int act, const int32_t *drafts, const int32_t *starts, int64_t batch, int64_t max_rows,
+                          const double *u, const float *temperature, int32_t *tokens, int32_t *count, int32_t *status, void *ws,
+                          size_t ws_bytes, sx_stream stream);
+
+/* The norms around a block, its gate, the residual and an 8-bit output in one launch; rows of K features in act:
+ *   h = x / sqrt(mean(x^2) + eps) * (post + w_add)   over the row, or each run of `group` features (0: the row; else a power of
+ *                                                    two, 8..512, that divides K); post null: h = x
+ *   h = h * gate, h * silu(gate) or h * sigmoid(gate)   gate rows ld_gate apart (0: one row for all); null: left out
+ *   r = residual_scale * residual + branch_scale * h    rounded to act and stored to residual_out; residual null: branch_scale * h
+ *   y = r / sqrt(mean(r^2) + eps) * (pre + w_add)       pre null: y = r
+ * Outputs: residual_out (with a residual), y (nullable) [M, K] in act, q (nullable) [M, K] int8 codes of y with scale [M] FP32 =
+ * amax(|y|) / 127, the activations sx_linear_int8 takes. A code is the nearest one, ties to even, of the exact y / scale (FP64: off
+ * where they lie 1e-13 from a border). A row of zeros has scale 0 and codes 0, one that holds NaN or an infinity scale NaN and
+ * codes 0. post has post_len values: K (0 says so too) or the group's. K a multiple of 8, up to 16384. residual_out and y may be x,
+ * the residual or the gate, row for row. No reference counterpart. */
+enum sx_gate_act { SX_GATE_NONE = 0, SX_GATE_SILU = 1, SX_GATE_SIGMOID = 2 };
+typedef struct sx_block_norm {
+    const void *x, *post, *gate, *residual, *pre;
+    void *residual_out, *y;
+    int8_t *q;
+    float *scale;
+    int64_t ldx, ld_gate, group, post_len;
+    int32_t gate_act;
+    float eps, w_add, residual_scale, branch_scale;
+} sx_block_norm;
+int sx_block_norm_int8(const sx_block_norm *p, int64_t M, int64_t K, int act, sx_stream stream);
+
+/* An 8-bit integer weight: q [N, K] int8 row-major, 16-byte aligned, scale [N] FP32, one for each channel; w = code * scale. K a
+ * multiple of 16, up to 131056. */
+typedef struct sx_int8_view {
+    const int8_t *q;
+    const float *scale;
+    int64_t N, K;
+} sx_int8_view;
+/* y[M, N] (out_act) = x * w^T with x [M, K] int8 codes (16-byte aligned) and x_scale [M] FP32, one for each token: the codes' sum
+ * is exact (32-bit integers), then rounded to FP32, times x_scale, times scale, one more rounding at a BF16 store. No reference
+ * counterpart. */
+int sx_linear_int8(const int8_t *x, const float *x_scale, const sx_int8_view *w, void *y, int64_t M, int out_act,
+                   sx_stream stream);
+
+/* ---- the gated delta rule: layers whose memory is a state and not a cache (no reference counterparts here; its
+ * kernels/gdn.hpp runs chains of tokens). A state S [key_dim, dim] FP32 for each of `heads` value heads; for each token
+ *   S <- e^g S;  u = beta (v - S^T k);  S <- S + k u^T;  o = S^T q.
+ * q, k [T, key_heads, key_dim], v [T, heads, dim] BF16; value head h goes with key head h / (heads / key_heads). normalize: k
+ * and q are divided by sqrt(sum of squares + 1e-6) first; q is then multiplied by scale. Gates a, b [T, heads] in gate_act, rows
+ * a_token and b_token elements apart: with A_log and dt_bias (FP32 [heads]) g = -exp(A_log) softplus(a + dt_bias) and beta =
+ * sigmoid(b); without (both null) g = a (0 or less; -1e4 and less all say: forget everything) and beta = b.
+ * Sequence b's tokens are rows starts[b] .. starts[b + 1] - 1 (device int32 [batch + 1]); its state is number slot[b] (null: b)
+ * of `slots` states, state_slot floats apart, each [heads, key_dim, dim] dense. key_dim 64 or 128, dim a multiple of 16 up to
+ * 1024, batch up to 1024. States, sums and norms are FP32; products of states and corrections are exact in BF16 thirds. A sequence
+ * whose run of tokens is impossible (negative, over the call's limit, outside T) is left alone; one with tokens whose slot is none
+ * of the states, or (where states are written) is another such sequence's too, keeps its state and its rows come out NaN. err
+ * (nullable) is then {1, the first row or the slot, the sequence}. Sequences of no tokens need no slot. Rows behind
+ * starts[batch] are left as they are. */
+typedef struct sx_delta {
+    sx_head_rows q, k, v;
+    const void *a, *b;
+    int64_t a_token, b_token;
+    const float *A_log, *dt_bias;
+    float *state;
+    const int32_t *slot, *starts;
+    int64_t T, key_heads, heads, key_dim, dim, slots, state_slot, batch;
+    int32_t gate_act, normalize;
+    float scale;
+} sx_delta;
+/* Tokens through the states, which are updated in place; out [T, heads, dim] BF16. max_len bounds a sequence's tokens: up to 16
+ * they go one by one, in one launch without a workspace (sx_gated_delta_workspace_bytes says 0; ws may be null); above in chunks
+ * of 64, two launches, ws 16-byte aligned, its contents never read before they are written, one per stream. A token that is no
+ * number makes the rows from it on NaN (a value: its column of them), and the state. */
+int sx_gated_delta_workspace_bytes(int64_t T, int64_t B, int64_t Hk, int64_t Hv, int64_t Dk, int64_t max_len, size_t *bytes);
+int sx_gated_delta(const sx_delta *d, int64_t max_len, const sx_head_rows *out, void *ws, size_t ws_bytes, uint32_t *err,
+                   sx_stream stream);
+/* The same for drafted tokens, whose states must not be kept before it is known which are accepted: the states are only read. A
+ * sequence's tokens (none to max_new, 1..64) are a tree, parents first: bit j of mask[t * mask_ld] says that token t goes on from
+ * token j of its sequence (bits at and above its own number are not looked at). out as above; u [T, heads, dim] and decay [T, heads]
+ * FP32 are what sx_gated_delta_commit takes: u / |k| and g. A token touches only those that see it, NaN included. */
+int sx_gated_delta_verify(const sx_delta *d, int64_t max_new, const uint64_t *mask, int64_t mask_ld, const sx_head_rows *out,
+                          float *u, float *decay, uint32_t *err, sx_stream stream);
+/* The accepted path into the states of all layers: for tokens i < count[b] (device int32 [batch], up to max_count), number
+ * path[b * path_ld + i] of the sequence (path null: i), a path from a root down, S <- e^g S + k u^T. k as the verify had it (layer
+ * stride: `layer`), u [layers, T, Hv, Dv], decay [layers, T, Hv]; states state_layer floats apart. A sequence with an impossible
+ * word (as above; a count below 0 or over max_count or its tokens, a path entry outside them) keeps its states; err (nullable) is
+ * then {1, the word, the sequence}. */
+int sx_gated_delta_commit(const sx_head_rows *k, const float *u, const float *decay, int64_t layers, int64_t T, int64_t Hk,
+                          int64_t Hv, int64_t Dk, int64_t Dv, float *state, int64_t state_layer, int64_t state_slot,
+                          int64_t slots, const int32_t *slot, const int32_t *starts, int64_t batch, const int32_t *count,
+                          int64_t max_count, const int32_t *path, int64_t path_ld, uint32_t *err, sx_stream stream);
+
 /* ---- strixw weight files: formats/strixw.hpp (the reader, StrixwFile :86-112) and runtime/strixw_loader.hpp (the
  * upload, StrixwDevice :22-52) ----
  * A file is a 128-byte header (magic "STRIXWT\0", format version 1..4, index and data-region offsets, file size, the

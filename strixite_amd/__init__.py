@@ -14,6 +14,7 @@ ACT_F32, ACT_BF16 = 0, 1
 MOE_F32, MOE_WMMA_BF16, MOE_WMMA_F16 = 0, 1, 2
 KV_BF16, KV_E4M3 = 0, 1
 SCORE_SIGMOID, SCORE_SOFTMAX = 0, 1
+GATE_NONE, GATE_SILU, GATE_SIGMOID = 0, 1, 2
 
 
 class SxError(RuntimeError):
@@ -47,6 +48,18 @@ class Fp8View(ctypes.Structure):
     _fields_ = [("q", ctypes.c_void_p), ("scale", ctypes.c_void_p), ("N", ctypes.c_int64), ("K", ctypes.c_int64)]
 
 
+class Int8View(ctypes.Structure):
+    """sx_int8_view: an int8 weight [N, K] with one FP32 scale for each channel."""
+    _fields_ = [("q", ctypes.c_void_p), ("scale", ctypes.c_void_p), ("N", ctypes.c_int64), ("K", ctypes.c_int64)]
+
+
+class BlockNormC(ctypes.Structure):
+    """sx_block_norm: the norms around a block."""
+    _fields_ = [(n, ctypes.c_void_p) for n in ("x", "post", "gate", "residual", "pre", "residual_out", "y", "q", "scale")] + [
+        (n, ctypes.c_int64) for n in ("ldx", "ld_gate", "group", "post_len")] + [("gate_act", ctypes.c_int32)] + [
+        (n, ctypes.c_float) for n in ("eps", "w_add", "residual_scale", "branch_scale")]
+
+
 class HeadRows(ctypes.Structure):
     """sx_head_rows: BF16 rows of heads, strides in elements."""
     _fields_ = [("p", ctypes.c_void_p), ("token", ctypes.c_int64), ("head", ctypes.c_int64), ("layer", ctypes.c_int64)]
@@ -62,6 +75,17 @@ class KvCacheC(ctypes.Structure):
                 ("v_head", ctypes.c_int64), ("v_layer", ctypes.c_int64), ("table", ctypes.c_void_p),
                 ("table_ld", ctypes.c_int64), ("pages_per_seq", ctypes.c_int64), ("lens", ctypes.c_void_p),
                 ("batch", ctypes.c_int64)]
+
+
+class DeltaC(ctypes.Structure):
+    """sx_delta: tokens, gates and states of the gated delta rule."""
+    _fields_ = [("q", HeadRows), ("k", HeadRows), ("v", HeadRows), ("a", ctypes.c_void_p), ("b", ctypes.c_void_p),
+                ("a_token", ctypes.c_int64), ("b_token", ctypes.c_int64), ("A_log", ctypes.c_void_p),
+                ("dt_bias", ctypes.c_void_p), ("state", ctypes.c_void_p), ("slot", ctypes.c_void_p),
+                ("starts", ctypes.c_void_p), ("T", ctypes.c_int64), ("key_heads", ctypes.c_int64), ("heads", ctypes.c_int64),
+                ("key_dim", ctypes.c_int64), ("dim", ctypes.c_int64), ("slots", ctypes.c_int64),
+                ("state_slot", ctypes.c_int64), ("batch", ctypes.c_int64), ("gate_act", ctypes.c_int32),
+                ("normalize", ctypes.c_int32), ("scale", ctypes.c_float)]
 
 
 class StrixwComponentC(ctypes.Structure):
@@ -134,6 +158,16 @@ SIGNATURES = {
     "sx_kv_append": [_HR, _HR, _I64, _KV, _P, _P, _I64, _P, _I64, _P, _P, _P],
     "sx_moe_router_scored": [_P, _I64, _I64, _I64, _I64, _INT, _P, _I64, _I64, _I64, _INT, _F, _P, _I64, ctypes.c_int32,
                              _P, _P, _INT, _P, _P],
+    "sx_mtp_accept_sampled_workspace_bytes": [_I64, _I64, _I64, _I64, _SZP],
+    "sx_mtp_accept_sampled": [_P, _I64, _I64, _I64, _P, _I64, _I64, _INT, _P, _P, _I64, _I64, _P, _P, _P, _P, _P, _P,
+                              ctypes.c_size_t, _P],
+    "sx_block_norm_int8": [_P, _I64, _I64, _INT, _P],
+    "sx_linear_int8": [_P, _P, ctypes.POINTER(Int8View), _P, _I64, _INT, _P],
+    "sx_gated_delta_workspace_bytes": [_I64, _I64, _I64, _I64, _I64, _I64, _SZP],
+    "sx_gated_delta": [_P, _I64, _HR, _P, ctypes.c_size_t, _P, _P],
+    "sx_gated_delta_verify": [_P, _I64, _P, _I64, _HR, _P, _P, _P, _P],
+    "sx_gated_delta_commit": [_HR, _P, _P, _I64, _I64, _I64, _I64, _I64, _I64, _P, _I64, _I64, _I64, _P, _P, _I64, _P, _I64, _P,
+                              _I64, _P, _P],
     "sx_strix_hash64": [_P, _U64],
     "sx_strixw_open": [_CP, ctypes.POINTER(_P)],
     "sx_strixw_close": [_P],

@@ -9,8 +9,8 @@ import struct
 
 import torch
 
-from . import (ACT_BF16, ACT_F32, KV_BF16, KV_E4M3, MOE_F32, SCORE_SIGMOID, SCORE_SOFTMAX, SX_EINVAL, Fp8View,
-               LogitCand, MtpPick, QView, SxError, check, lib)
+from . import (ACT_BF16, ACT_F32, GATE_NONE, GATE_SIGMOID, GATE_SILU, KV_BF16, KV_E4M3, MOE_F32, SCORE_SIGMOID, SCORE_SOFTMAX, SX_EINVAL, Fp8View,
+               Int8View, LogitCand, MtpPick, QView, SxError, check, lib)
 
 _c = ctypes.c_void_p
 
@@ -726,3 +726,307 @@ def moe_router_scored(logits, E, k, score="sigmoid", bias=None, groups=1, top_gr
          SCORES[score], _a(bias), groups, top_groups if groups > 1 else 1, group_best if groups > 1 else 1, int(renorm),
          factor, _a(shared), shared_ld, shared_id, ids.data_ptr(), coef.data_ptr(), act, _a(err), stream=stream)
     return ids, coef, err
+
+
+# ---------------- 8-bit integer activations and linear ----------------
+
+GATES = {"none": GATE_NONE, "silu": GATE_SILU, "sigmoid": GATE_SIGMOID}
+_NORM = struct.Struct("@9P4qi4f4x").pack  # sx_block_norm as bytes
+
+
+def block_norm_int8(x, post=None, gate=None, residual=None, pre=None, eps=1e-6, w_add=0.0, group=None, gate_act="none",
+                    residual_scale=1.0, branch_scale=1.0, residual_out=None, y=None, q=None, scale=None, codes=True, stream=None):
+    """h = x / rms(x) * (post + w_add), over the row or each run of `group` features; h *= act(gate), act none, silu or sigmoid;
+    r = residual_scale * residual + branch_scale * h (with a residual: rounded, residual_out); y = r / rms(r) * (pre + w_add); and y as
+    int8 codes q [M, K] with an FP32 scale for each row [M], the activations linear_int8 takes. Each of post, gate, residual and pre
+    may be None and is then left out. x [M, K] (any row stride) in FP32 or BF16, the others in its type: gate [M, K], its rows any
+    stride apart (expanded: one for all), post [K] or [group], pre [K], y (optional): a buffer that receives y itself. codes False: no
+    q and scale. Returns (q, scale, residual_out or None); residual_out may be the residual."""
+    act, dtype, dev = act_of(x), x.dtype, x.get_device()
+    if x.dim() != 2 or x.stride(1) != 1:
+        _refuse("x must be [M, K] with dense rows and is", tuple(x.shape), x.stride())
+    M, K = shape = x.shape
+    _together(dev, (post, gate, residual, pre, residual_out, y, q, scale))
+    post_len = 0
+    if post is not None:
+        post_len = post.numel()
+        _is("post", post, dtype, (group if group is not None and post_len == group else K,))
+    if gate is not None and (gate.dtype != dtype or gate.shape != shape or gate.stride(1) != 1):
+        _refuse("gate must be", dtype, tuple(shape), "with dense rows and is", gate.dtype, tuple(gate.shape), gate.stride())
+    if gate_act not in GATES:
+        _refuse("gate_act is", repr(gate_act), "and not one of", list(GATES))
+    if pre is not None:
+        _is("pre", pre, dtype, (K,))
+    if residual is not None:
+        _is("residual", residual, dtype, shape)
+        if residual_out is None:
+            residual_out = _empty_like(residual, stream)
+        else:
+            _is("residual_out", residual_out, dtype, shape)
+    elif residual_out is not None:
+        _refuse("residual_out without a residual")
+    if y is not None:
+        _is("y", y, dtype, shape)
+    if not codes:
+        if q is not None or scale is not None:
+            _refuse("q or scale without codes")
+    else:
+        if q is None:
+            q = _empty(x, shape, torch.int8, stream)
+        else:
+            _is("q", q, torch.int8, shape)
+        if scale is None:
+            scale = _empty(x, (M,), torch.float32, stream)
+        else:
+            _is("scale", scale, torch.float32, (M,))
+    a = lambda t: 0 if t is None else t.data_ptr()
+    n = _NORM(x.data_ptr(), a(post), a(gate), a(residual), a(pre), a(residual_out), a(y), a(q), a(scale), x.stride(0) if M > 1 else K,
+              0 if gate is None else gate.stride(0) if M > 1 else K, group or 0, post_len, GATES[gate_act], eps, w_add, residual_scale,
+              branch_scale)
+    _run(dev, lib().sx_block_norm_int8, n, M, K, act, stream=stream)
+    return q, scale, residual_out
+
+
+
+class Int8Weight:
+    """An int8 weight resident on the device: q [N, K] torch.int8, scale [N] FP32, one for each channel (w = code * scale)."""
+
+    def __init__(self, q, scale):
+        if q.dim() != 2 or q.shape[1] % 16:
+            _refuse("an int8 weight is [N, K], K a multiple of 16, and not", tuple(q.shape))
+        self.N, self.K = (int(n) for n in q.shape)
+        _is("q", q, torch.int8, (self.N, self.K))
+        _is("scale", scale, torch.float32, (self.N,))
+        if scale.device != q.device:
+            _refuse("q is on", q.device, "and scale on", scale.device)
+        self.q, self.scale = q, scale
+        self._view = Int8View(q.data_ptr(), scale.data_ptr(), self.N, self.K)
+
+    def view(self):
+        return ctypes.byref(self._view)
+
+    def nbytes(self):
+        return self.q.numel() + 4 * self.scale.numel()
+
+
+def linear_int8(x, x_scale, w, out_act=ACT_BF16, y=None, stream=None):
+    """y[M, N] = (x * x_scale) * w^T: x int8 codes [M, K] with an FP32 scale for each token [M] (block_norm_int8's outputs), w an
+    Int8Weight; y BF16 or (out_act ACT_F32) FP32."""
+    dev, M, dtype = x.get_device(), x.shape[0], dtype_of(out_act)
+    _together(dev, (x_scale, w.q, y))
+    _is("x", x, torch.int8, (M, w.K))
+    _is("x_scale", x_scale, torch.float32, (M,))
+    if y is None:
+        y = _empty(x, (M, w.N), dtype, stream)
+    else:
+        _is("y", y, dtype, (M, w.N))
+    _run(dev, lib().sx_linear_int8, x.data_ptr(), x_scale.data_ptr(), w.view(), y.data_ptr(), M, out_act, stream=stream)
+    return y
+
+
+# ---------------- the gated delta rule ----------------
+
+# sx_delta as bytes
+_DELTA = struct.Struct("@Pqqq Pqqq Pqqq PP qq PPPPP qqqqqqqq iif4x".replace(" ", "")).pack
+
+
+def _rows_of(name, t, heads, dim):
+    """A BF16 tensor [T, heads, dim]'s data pointer and strides (token, head, none) as _DELTA takes them."""
+    if t.dtype != torch.bfloat16 or t.dim() != 3 or t.shape[1:] != (heads, dim) or t.stride(2) != 1:
+        _refuse(name, f"must be BF16 [tokens, {heads}, {dim}] with dense rows and is", t.dtype, tuple(t.shape), t.stride())
+    return t.data_ptr(), t.stride(0), t.stride(1), 0
+
+
+def _delta(q, k, v, a, b, state, starts, slots, A_log, dt_bias, normalize, scale):
+    """The sx_delta of these tensors, and (T, Hk, Hv, Dk, Dv, batch)."""
+    if q.dim() != 3 or v.dim() != 3:
+        _refuse("q, k and v are [tokens, heads, dim]")
+    (T, Hk, Dk), (Hv, Dv) = q.shape, v.shape[1:]
+    if k.shape[0] != T or v.shape[0] != T:
+        _refuse("q", tuple(q.shape), "k", tuple(k.shape), "v", tuple(v.shape))
+    for name, t in (("a", a), ("b", b)):
+        if t.shape != (T, Hv) or t.stride(1) != 1 and Hv > 1 or t.dtype != a.dtype:
+            _refuse(name, f"must be [{T}, {Hv}] with dense rows, a and b of one type, and is", t.dtype, tuple(t.shape), t.stride())
+    if state.dtype != torch.float32 or state.dim() != 4 or state.shape[1:] != (Hv, Dk, Dv) or state.stride()[1:] != (Dk * Dv, Dv, 1):
+        _refuse(f"state must be FP32 [states, {Hv}, {Dk}, {Dv}], each dense, and is", state.dtype, tuple(state.shape), state.stride())
+    if starts.dim() != 1 or starts.numel() < 2:
+        _refuse("starts must be [batch + 1] and is", tuple(starts.shape))
+    B = starts.numel() - 1
+    _is("starts", starts, torch.int32, (B + 1,))
+    if slots is not None:
+        _is("slots", slots, torch.int32, (B,))
+    if A_log is not None:
+        _is("A_log", A_log, torch.float32, (Hv,))
+    if dt_bias is not None:
+        _is("dt_bias", dt_bias, torch.float32, (Hv,))
+    one = Hv * Dk * Dv
+    d = _DELTA(*_rows_of("q", q, Hk, Dk), *_rows_of("k", k, Hk, Dk), *_rows_of("v", v, Hv, Dv), a.data_ptr(), b.data_ptr(),
+               a.stride(0) if T > 1 else Hv, b.stride(0) if T > 1 else Hv, _a(A_log) or 0, _a(dt_bias) or 0, state.data_ptr(),
+               _a(slots) or 0, starts.data_ptr(), T, Hk, Hv, Dk, Dv, state.shape[0],
+               state.stride(0) if state.shape[0] > 1 else one, B, act_of(a), int(normalize), Dk ** -0.5 if scale is None else scale)
+    return d, (T, Hk, Hv, Dk, Dv, B)
+
+
+def gated_delta_workspace_bytes(T, B, Hk, Hv, Dk, max_len):
+    n = ctypes.c_size_t()
+    check(lib().sx_gated_delta_workspace_bytes(T, B, Hk, Hv, Dk, max_len, ctypes.byref(n)))
+    return n.value
+
+
+def gated_delta_workspace(q, v, starts, max_len):
+    """A workspace for gated_delta calls of these shapes (one per stream; nothing in it outlives a call); None where such
+    calls need none."""
+    n = gated_delta_workspace_bytes(q.shape[0], starts.numel() - 1, q.shape[1], v.shape[1], q.shape[2], max_len)
+    return torch.empty((n + 7) // 8, dtype=torch.int64, device=q.device) if n else None
+
+
+def gated_delta(q, k, v, a, b, state, starts, max_len, slots=None, A_log=None, dt_bias=None, normalize=True, scale=None, out=None,
+                ws=None, err=None, stream=None):
+    """The gated delta rule: for each token of a sequence and value head S <- e^g S, u = beta (v - S^T k), S <- S + k u^T, o = S^T q.
+    q, k [T, Hk, Dk] and v [T, Hv, Dv] BF16 (any token and head strides; Hv a multiple of Hk), divided by their lengths first
+    (normalize), q times scale (1 / sqrt(Dk) unless given). Gates a, b [T, Hv] in BF16 or FP32: with A_log and dt_bias (FP32 [Hv])
+    g = -exp(A_log) softplus(a + dt_bias), beta = sigmoid(b), else g = a and beta = b. starts int32 [B + 1]: sequence b's tokens
+    are rows starts[b] .. starts[b + 1] - 1, at most max_len; state FP32 [states, Hv, Dk, Dv], number slots[b] (int32 [B]; None: b)
+    its own, updated in place (zeros: a new sequence). Up to 16 tokens a sequence go one by one, more in chunks. ws:
+    gated_delta_workspace(), made for the call unless given. Returns (out [T, Hv, Dv] BF16, err)."""
+    dev = q.get_device()
+    _together(dev, (k, v, a, b, state, starts, slots, A_log, dt_bias, out, ws, err))
+    d, (T, Hk, Hv, Dk, Dv, B) = _delta(q, k, v, a, b, state, starts, slots, A_log, dt_bias, normalize, scale)
+    if out is None:
+        out = _empty(q, (T, Hv, Dv), torch.bfloat16, stream)
+    elif out.dim() != 3 or out.shape[0] != T:
+        _refuse("out is", tuple(out.shape))
+    if ws is None:
+        n = gated_delta_workspace_bytes(T, B, Hk, Hv, Dk, max_len)
+        ws = _empty(q, ((n + 7) // 8,), torch.int64, stream) if n else None
+    elif not ws.is_contiguous():
+        _refuse("ws must be contiguous and has strides", ws.stride())
+    _is_err(err)
+    _run(dev, lib().sx_gated_delta, d, max_len, _head_rows("out", out, Hv, Dv), _a(ws), 0 if ws is None else ws.numel() * ws.element_size(),
+         _a(err), stream=stream)
+    return out, err
+
+
+def gated_delta_verify(q, k, v, a, b, state, starts, mask, max_new, slots=None, A_log=None, dt_bias=None, normalize=True, scale=None,
+                       out=None, u=None, decay=None, err=None, stream=None):
+    """gated_delta of drafted tokens, whose states must wait for the accepted path: state is only read. A sequence's tokens, at
+    most max_new (up to 64), are a tree; mask int64 [T, 1] as tree_mask makes it. Returns (out [T, Hv, Dv] BF16, u FP32 [T, Hv, Dv],
+    decay FP32 [T, Hv], err); u and decay (and k) are what gated_delta_commit takes."""
+    dev = q.get_device()
+    _together(dev, (k, v, a, b, state, starts, mask, slots, A_log, dt_bias, out, u, decay, err))
+    d, (T, Hk, Hv, Dk, Dv, B) = _delta(q, k, v, a, b, state, starts, slots, A_log, dt_bias, normalize, scale)
+    if mask.dtype != torch.int64 or mask.dim() != 2 or mask.shape[0] != T or mask.shape[1] < 1:
+        _refuse("mask must be int64 [T, 1] and is", mask.dtype, tuple(mask.shape))
+    if out is None:
+        out = _empty(q, (T, Hv, Dv), torch.bfloat16, stream)
+    elif out.dim() != 3 or out.shape[0] != T:
+        _refuse("out is", tuple(out.shape))
+    if u is None:
+        u = _empty(q, (T, Hv, Dv), torch.float32, stream)
+    else:
+        _is("u", u, torch.float32, (T, Hv, Dv))
+    if decay is None:
+        decay = _empty(q, (T, Hv), torch.float32, stream)
+    else:
+        _is("decay", decay, torch.float32, (T, Hv))
+    _is_err(err)
+    _run(dev, lib().sx_gated_delta_verify, d, max_new, mask.data_ptr(), mask.stride(0) if T > 1 else 1, _head_rows("out", out, Hv, Dv),
+         u.data_ptr(), decay.data_ptr(), _a(err), stream=stream)
+    return out, u, decay, err
+
+
+def gated_delta_commit(k, u, decay, state, starts, count, path=None, max_count=None, slots=None, err=None, stream=None):
+    """The accepted path of a gated_delta_verify into the states, in place: its first count[b] (int32 [B]) tokens, number path[b, i]
+    of the sequence (int32 [B, at most]; None: i) the i-th of them. k [T, Hk, Dk], u and decay as the verify had and gave them; all
+    layers in one launch with k [layers, T, Hk, Dk], u [layers, T, Hv, Dv], decay [layers, T, Hv], state [layers, states, Hv, Dk,
+    Dv]. Without a path max_count bounds the counts. Returns err. A sequence that cannot be committed as asked keeps its states."""
+    dev, layered = k.get_device(), k.dim() == 4
+    _together(dev, (u, decay, state, starts, count, path, slots, err))
+    if k.dim() not in (3, 4) or u.dim() != k.dim() or k.dtype != torch.bfloat16 or k.stride(-1) != 1 or u.shape[:-2] != k.shape[:-2]:
+        _refuse("k must be BF16 [tokens, heads, dim] with dense rows, with or without layers as u is:", k.dtype, tuple(k.shape), k.stride(), tuple(u.shape))
+    T, Hk, Dk = k.shape[-3:]
+    Hv, Dv = u.shape[-2:]
+    layers = k.shape[0] if layered else 1
+    _is("u", u, torch.float32, u.shape)
+    _is("decay", decay, torch.float32, u.shape[:-1])
+    if (state.dtype != torch.float32 or state.dim() != 4 + layered or state.shape[-3:] != (Hv, Dk, Dv) or
+            state.stride()[-3:] != (Dk * Dv, Dv, 1) or layered and state.shape[0] != layers):
+        _refuse(f"state must be FP32 [{'layers, ' if layered else ''}states, {Hv}, {Dk}, {Dv}], each dense, and is", state.dtype, tuple(state.shape), state.stride())
+    B = starts.numel() - 1
+    _is("starts", starts, torch.int32, (B + 1,))
+    _is("count", count, torch.int32, (B,))
+    if slots is not None:
+        _is("slots", slots, torch.int32, (B,))
+    ld = 0
+    if path is not None:
+        if path.dtype != torch.int32 or path.dim() != 2 or path.shape[0] != B or path.stride(1) != 1:
+            _refuse("path must be int32 [batch, most tokens kept] with dense rows")
+        max_count = path.shape[1] if max_count is None else max_count
+        ld = path.stride(0) if B > 1 else path.shape[1]
+        if max_count > path.shape[1]:
+            _refuse("max_count =", max_count, "is over the path's", path.shape[1])
+    elif max_count is None:
+        _refuse("max_count is needed without a path")
+    _is_err(err)
+    states, one = state.shape[-4], Hv * Dk * Dv
+    _run(dev, lib().sx_gated_delta_commit, _ROWS(k.data_ptr(), k.stride(-3), k.stride(-2), k.stride(0) if layered else 0), u.data_ptr(),
+         decay.data_ptr(), layers, T, Hk, Hv, Dk, Dv, state.data_ptr(), state.stride(0) if layered else 0,
+         state.stride(-4) if states > 1 else one, states, _a(slots), starts.data_ptr(), B, count.data_ptr(), max_count, _a(path), ld,
+         _a(err), stream=stream)
+    return err
+
+
+# ---------------- acceptance by the target's probabilities ----------------
+
+def mtp_accept_sampled_workspace_bytes(T, B, n_valid, n_draft):
+    n = ctypes.c_size_t()
+    check(lib().sx_mtp_accept_sampled_workspace_bytes(T, B, n_valid, n_draft, ctypes.byref(n)))
+    return n.value
+
+
+def mtp_accept_sampled(logits, drafts, starts, u, temperature, max_rows, draft_logits=None, n_valid=None, tokens=None, count=None,
+                       status=None, ws=None, stream=None):
+    """Acceptance of drafted tokens by rejection sampling. Sequence b's rows are starts[b] .. starts[b + 1] - 1 (int32 [B + 1], at
+    most max_rows) of logits [T, >= n_valid] (FP32 or BF16, any row stride); drafts int32 [T]: the token proposed behind a row (a
+    sequence's last row has none); draft_logits [T, n_draft] in the logits' type: what it was drawn from (None: it was certain). Draft
+    d of row t stays if u[t, 0] q(d) < p(d), p and q the softmax over temperature[b] (FP32 [B]); the first that does not is replaced by a
+    token from max(p - q, 0), and behind the last comes one from p, both by u[t, 1]. u FP64 [T, 2] in [0, 1). temperature 0: the
+    largest logits. Returns (tokens int32 [B, max_rows]: what is committed, then -1; count int32 [B], as kv_append and
+    gated_delta_commit take it; status int32 [B]: 0, 1 + the row that has no distribution or draft, -1 impossible starts)."""
+    dev, act = logits.get_device(), act_of(logits)
+    if logits.dim() != 2 or logits.stride(1) != 1:
+        _refuse("logits must be [T, vocabulary] with dense rows and are", tuple(logits.shape), logits.stride())
+    T, n_valid, n_draft, dld = logits.shape[0], logits.shape[1] if n_valid is None else n_valid, 0, 0
+    _together(dev, (drafts, starts, u, temperature, draft_logits, tokens, count, status, ws))
+    if n_valid > logits.shape[1]:
+        _refuse("n_valid =", n_valid, "is over the logits'", logits.shape[1])
+    B = starts.numel() - 1
+    _is("drafts", drafts, torch.int32, (T,))
+    _is("starts", starts, torch.int32, (B + 1,))
+    _is("u", u, torch.float64, (T, 2))
+    _is("temperature", temperature, torch.float32, (B,))
+    if draft_logits is not None:
+        if draft_logits.dtype != logits.dtype or draft_logits.dim() != 2 or draft_logits.shape[0] != T or draft_logits.stride(1) != 1:
+            _refuse("draft_logits must be", logits.dtype, f"[{T}, vocabulary] with dense rows and are", draft_logits.dtype, tuple(draft_logits.shape))
+        n_draft = draft_logits.shape[1]
+        dld = draft_logits.stride(0) if T > 1 else n_draft
+    if tokens is None:
+        tokens = _empty(drafts, (B, max_rows), torch.int32, stream)
+    else:
+        _is("tokens", tokens, torch.int32, (B, max_rows))
+    if count is None:
+        count = _empty(drafts, (B,), torch.int32, stream)
+    else:
+        _is("count", count, torch.int32, (B,))
+    if status is None:
+        status = _empty(drafts, (B,), torch.int32, stream)
+    else:
+        _is("status", status, torch.int32, (B,))
+    if ws is None:
+        ws = _empty(drafts, ((mtp_accept_sampled_workspace_bytes(T, B, n_valid, n_draft) + 7) // 8,), torch.int64, stream)
+    elif not ws.is_contiguous():
+        _refuse("ws must be contiguous and has strides", ws.stride())
+    _run(dev, lib().sx_mtp_accept_sampled, logits.data_ptr(), logits.stride(0) if T > 1 else logits.shape[1], T, n_valid,
+         _a(draft_logits), dld, n_draft, act, drafts.data_ptr(), starts.data_ptr(), B, max_rows, u.data_ptr(), temperature.data_ptr(),
+         tokens.data_ptr(), count.data_ptr(), status.data_ptr(), ws.data_ptr(), ws.numel() * ws.element_size(), stream=stream)
+    return tokens, count, status
