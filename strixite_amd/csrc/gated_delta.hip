@@ -447,7 +447,7 @@ std::string delta_error(const sx_delta &d) {
         return "starts, slot and the gates must be aligned to their elements";
     const int64_t s[6] = {d.q.token, d.q.head, d.k.token, d.k.head, d.v.token, d.v.head};
     for (int64_t x : s)
-        if (x < 0 || x > (int64_t)1 << 32 || x % 8 != 0) return cat("strides of q, k and v must be multiples of 8 (", x, ")");
+        if (x < 0 || x > (int64_t)1 << 24 || x % 8 != 0) return cat("strides of q, k and v must be multiples of 8 up to 2^24 (", x, ")");
     if (d.a_token < 0 || d.b_token < 0 || d.a_token > (int64_t)1 << 32 || d.b_token > (int64_t)1 << 32) return cat("gate strides ", d.a_token, ", ", d.b_token);
     if (!std::isfinite(d.scale)) return cat("scale = ", d.scale);
     return "";
@@ -471,8 +471,8 @@ std::string output_error(const sx_delta &d, const void *o, int64_t n) {
 
 std::string out_error(const sx_delta &d, const sx_head_rows &o) {
     if (o.p == nullptr) return "null pointer";
-    if (!aligned(o.p, 8) || o.token < 0 || o.head < 0 || o.token % 4 != 0 || o.head % 4 != 0 || o.token > (int64_t)1 << 32 || o.head > (int64_t)1 << 32)
-        return cat("must be 8-byte aligned with strides that are multiples of 4 (", o.token, ", ", o.head, ")");
+    if (!aligned(o.p, 8) || o.token < 0 || o.head < 0 || o.token % 4 != 0 || o.head % 4 != 0 || o.token > (int64_t)1 << 24 || o.head > (int64_t)1 << 24)
+        return cat("must be 8-byte aligned with strides that are multiples of 4, up to 2^24 (", o.token, ", ", o.head, ")");
     if (!rows_apart(d.dim, {{d.T, o.token}, {d.heads, o.head}})) return "has heads that overlap";
     const std::string e = output_error(d, o.p, span(o, d.T, d.heads, d.dim));
     if (!e.empty()) return e;

@@ -19,6 +19,8 @@
 // out and everything from them on (a value's: in its column) is NaN, as the rule has it.
 #include "gated_delta.hpp"
 
+#include <type_traits>
+
 namespace sx {
 namespace delta {
 namespace {
@@ -228,212 +230,299 @@ __global__ void __launch_bounds__(256) delta_prepare_kernel(const Args a, const 
         }
 }
 
-// What a wave needs of a chunk from memory.
+// What a state wave needs of a chunk from memory.
 template <int TS>
-struct Chunk {
-    bf16x8 K[4], Q[4];       // 4 TS of a token's values
-    bf16x8 T[2][3], P[2][2];
+struct StateChunk {
+    bf16x8 K[4];             // 4 TS values of a token
+    bf16x8 T[2][3];
     bf16x8 KT[TS][2];
-    f32x4 in, out, keep;     // of the wave's four tokens a lane
+    f32x4 in, keep;          // of the wave's four tokens a lane
     uint16_t v[4];
     float fade;
     int32_t bad;
     uint64_t use;
 };
+// And an output wave.
+struct OutChunk {
+    bf16x8 Q[4], P[2][2];
+    f32x4 out;
+};
 
+__device__ __forceinline__ u32x4 load16(const void *base, uint32_t off) { return *reinterpret_cast<const u32x4 *>(static_cast<const uint8_t *>(base) + off); }
+__device__ __forceinline__ u32x2 load8(const void *base, uint32_t off) { return *reinterpret_cast<const u32x2 *>(static_cast<const uint8_t *>(base) + off); }
+template <int TS>
+__device__ __forceinline__ bf16x8 load_piece(const void *base, uint32_t off) {  // 4 TS values, the rest zero
+    if constexpr (TS == 2) {
+        return __builtin_bit_cast(bf16x8, load16(base, off));
+    } else {
+        const u32x2 x = load8(base, off);
+        return __builtin_bit_cast(bf16x8, u32x4{x[0], x[1], 0u, 0u});
+    }
+}
+
+// Eight tokens of a column from two tiles of four, as an operand.
+__device__ __forceinline__ bf16x8 pair_of(const u32x2 (*from)[64], int p) {
+    const u32x2 x = from[2 * p][threadIdx.x & 63], y = from[2 * p + 1][threadIdx.x & 63];
+    return __builtin_bit_cast(bf16x8, u32x4{x[0], x[1], y[0], y[1]});
+}
+
+// Waves 0 to 3 carry the state, waves 4 to 7 make the outputs from what those leave in LDS, a chunk's products of Q and P beside
+// the next one's of K: alone on its SIMD a wave that did both took twice as long for a chunk.
 template <int DK>
-__global__ void __launch_bounds__(256, 1) delta_scan_kernel(const Args a, const Work w, int pairs8) {
-    constexpr int TS = DK / 64;  // tiles of the state's rows a wave has
-    __shared__ __attribute__((aligned(16))) f32x4 xs[4][4][64], ys[4][4][64];  // [wave][tile]
+__global__ void __launch_bounds__(512) delta_scan_kernel(const Args a, const Work w, int pairs8) {
+    constexpr int TS = DK / 64;  // tiles of the state's rows a state wave has
+    __shared__ __attribute__((aligned(16))) f32x4 xs[4][4][64];  // [wave][tile]: K S over the wave's rows
+    __shared__ __attribute__((aligned(16))) u32x4 ss[4][2][64];  // the state's rows of each wave as operands
     __shared__ __attribute__((aligned(16))) u32x2 rs[3][4][64], us[2][4][64], ks[3][4][64];
     __shared__ int poison[16];
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), n16 = lane & 15, g4 = lane >> 4;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wt = wave & 3, n16 = lane & 15, g4 = lane >> 4;
     const int pair = blockIdx.x % pairs8, b = pair / a.Hv, h = pair % a.Hv, hk = h / a.rep;
     if (b >= a.B) return;
     const int col = (int)(blockIdx.x / pairs8) * 16 + n16;
     const Seq s = sequence(a.starts, a.slot, b, a.B, a.T, a.max_len, a.slots, true);
     if (blockIdx.x / pairs8 == 0 && h == 0 && threadIdx.x == 0) tell(s, b, a.err);
     if (s.n == 0) return;
+    uint16_t *const op = a.out + s.t0 * a.o_t + h * a.o_h;
     if (!s.ok) {
-        for (int i = threadIdx.x >> 4; i < s.n; i += 16) a.out[(int64_t)(s.t0 + i) * a.o_t + h * a.o_h + col] = 0x7fc0;
+        for (int i = threadIdx.x >> 4; i < s.n; i += 32) op[i * a.o_t + col] = 0x7fc0;
         return;
     }
     if (threadIdx.x < 16) poison[threadIdx.x] = 0x7fffffff;
-    float *state = a.state + s.slot * a.s_slot + ((int64_t)h * DK + 16 * TS * wave + 4 * TS * g4) * a.Dv + col;
-    f32x4 S[TS];
-#pragma unroll
-    for (int t = 0; t < TS; ++t)
-#pragma unroll
-        for (int r = 0; r < 4; ++r) S[t][r] = state[(int64_t)(4 * t + r) * a.Dv];
     const int chunks = (s.n + kC - 1) / kC;
     const int64_t slot0 = first_slot(s.t0, b);
-    const uint16_t *kp = a.k + s.t0 * a.k_t + hk * a.k_h + 16 * TS * wave + 4 * TS * g4, *qp = a.q + s.t0 * a.q_t + hk * a.q_h + 16 * TS * wave + 4 * TS * g4;
-    const uint16_t *vp = a.v + s.t0 * a.v_t + h * a.v_h + col;
-    auto fetch = [&](int c, Chunk<TS> &o) __attribute__((always_inline)) {  // past the last one: the last one again, not used
-        c = min(c, chunks - 1);
-        const uint8_t *head = w.heads + ((slot0 + c) * a.Hv + h) * kHeadBytes, *keys = w.keys + ((slot0 + c) * a.Hk + hk) * (DK / 16 * 2048);
-        const Words *words = reinterpret_cast<const Words *>(head + kTBytes + kPBytes);
-#pragma unroll
-        for (int t = 0; t < 4; ++t) {
-            const int64_t at = min(c * kC + token_at(t, n16), s.n - 1);
-            if constexpr (TS == 2) {
-                o.K[t] = *reinterpret_cast<const bf16x8 *>(kp + at * a.k_t);
-                o.Q[t] = *reinterpret_cast<const bf16x8 *>(qp + at * a.q_t);
-            } else {
-                const u32x2 x = *reinterpret_cast<const u32x2 *>(kp + at * a.k_t), y = *reinterpret_cast<const u32x2 *>(qp + at * a.q_t);
-                o.K[t] = __builtin_bit_cast(bf16x8, u32x4{x[0], x[1], 0u, 0u}), o.Q[t] = __builtin_bit_cast(bf16x8, u32x4{y[0], y[1], 0u, 0u});
-            }
-        }
-#pragma unroll
-        for (int p = 0; p < 2; ++p) {
-            if (p <= wave >> 1) {
-                const int blk = block_of(wave, p);
-#pragma unroll
-                for (int i = 0; i < 3; ++i) o.T[p][i] = *reinterpret_cast<const bf16x8 *>(head + (blk * 3 + i) * 1024 + lane * 16);
-#pragma unroll
-                for (int i = 0; i < 2; ++i) o.P[p][i] = *reinterpret_cast<const bf16x8 *>(head + kTBytes + (blk * 2 + i) * 1024 + lane * 16);
-            }
-#pragma unroll
-            for (int t = 0; t < TS; ++t) o.KT[t][p] = *reinterpret_cast<const bf16x8 *>(keys + ((wave * TS + t) * 2 + p) * 1024 + lane * 16);
-        }
-        const int at = token_of(wave, g4, 0);
-        o.in = *reinterpret_cast<const f32x4 *>(&words->in[at]);
-        o.out = *reinterpret_cast<const f32x4 *>(&words->out[at]);
-        o.keep = *reinterpret_cast<const f32x4 *>(&words->keep[at]);
-        o.fade = words->fade, o.bad = words->bad, o.use = words->use;
-#pragma unroll
-        for (int r = 0; r < 4; ++r) o.v[r] = vp[(int64_t)min(c * kC + at + r, s.n - 1) * a.v_t];
-    };
+    const uint8_t *const heads = w.heads + (slot0 * a.Hv + h) * kHeadBytes, *const keys = w.keys + (slot0 * a.Hk + hk) * (DK / 16 * 2048);
+    const uint16_t *const kp = a.k + s.t0 * a.k_t + hk * a.k_h, *const qp = a.q + s.t0 * a.q_t + hk * a.q_h, *const vp = a.v + s.t0 * a.v_t + h * a.v_h;
     const f32x4 zero = {0.f, 0.f, 0.f, 0.f};
-    auto put3 = [&](u32x2 (*to)[4][64], const f32x4 &x) __attribute__((always_inline)) {
-        float r[4] = {x[0], x[1], x[2], x[3]};
-#pragma unroll
-        for (int i = 0; i < 3; ++i) {
-            to[i][wave][lane] = u32x2{tops(__float_as_uint(r[0]), __float_as_uint(r[1])), tops(__float_as_uint(r[2]), __float_as_uint(r[3]))};
-#pragma unroll
-            for (int j = 0; j < 4; ++j) r[j] -= __uint_as_float(__float_as_uint(r[j]) & 0xFFFF0000u);
-        }
-    };
-    auto get = [&](const u32x2 (*from)[64], int p) __attribute__((always_inline)) {
-        const u32x2 x = from[2 * p][lane], y = from[2 * p + 1][lane];
-        return __builtin_bit_cast(bf16x8, u32x4{x[0], x[1], y[0], y[1]});
-    };
-    auto chunk = [&](int c, Chunk<TS> &now, Chunk<TS> &next) __attribute__((always_inline)) {
-        fetch(c + 1, next);
-        if (now.use != ~0ull) {
-            const u32x4 none = {0u, 0u, 0u, 0u};
-#pragma unroll
-            for (int t = 0; t < 4; ++t)
-                if (!(now.use >> token_at(t, n16) & 1)) now.K[t] = __builtin_bit_cast(bf16x8, none);
-        }
-        // K S and Q S over this wave's rows of the state
-        float s8[8];
-#pragma unroll
-        for (int j = 0; j < 4; ++j) s8[j] = S[0][j], s8[4 + j] = TS == 2 ? S[TS - 1][j] : 0.f;
-        bf16x8 so[3];
-        split(s8, so);
-        f32x4 X[4], Y[4];
-#pragma unroll
-        for (int t = 0; t < 4; ++t) X[t] = mfma(now.K[t], so[2], zero);
-#pragma unroll
-        for (int t = 0; t < 4; ++t) X[t] = mfma(now.K[t], so[1], X[t]);
-#pragma unroll
-        for (int t = 0; t < 4; ++t) X[t] = mfma(now.K[t], so[0], X[t]);
-#pragma unroll
-        for (int t = 0; t < 4; ++t) Y[t] = mfma(now.Q[t], so[1], zero);
-#pragma unroll
-        for (int t = 0; t < 4; ++t) Y[t] = mfma(now.Q[t], so[0], Y[t]);
-#pragma unroll
-        for (int t = 0; t < 4; ++t) xs[wave][t][lane] = X[t], ys[wave][t][lane] = Y[t];
-        lds_barrier();
-        // this wave's 16 tokens: what the state does not explain of them
-        f32x4 x = xs[0][wave][lane] + xs[1][wave][lane] + xs[2][wave][lane] + xs[3][wave][lane];
-        const f32x4 y = ys[0][wave][lane] + ys[1][wave][lane] + ys[2][wave][lane] + ys[3][wave][lane];
-        bool odd = now.bad < kC;
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-            const int at = token_of(wave, g4, r);
-            float v = bf16_to_f32(now.v[r]);
-            const bool use = now.use >> at & 1, num = finite(v);
-            odd |= use && !num;
-            x[r] = use && num ? v - now.in[r] * x[r] : use ? -now.in[r] * x[r] : 0.f;
-        }
-        if (__any(odd)) {
-            int at = now.bad;
-#pragma unroll
-            for (int r = 3; r >= 0; --r) {
-                const int i = token_of(wave, g4, r);
-                if ((now.use >> i & 1) && !finite(bf16_to_f32(now.v[r]))) at = min(at, i);
-            }
-            if (at < kC) atomicMin(&poison[n16], c * kC + at);
-        }
-        put3(rs, x);
-        lds_barrier();
-        // U = T x
-        f32x4 u = zero;
-#pragma unroll
-        for (int p = 0; p < 2; ++p)
-            if (p <= wave >> 1) {
-                const bf16x8 r0 = get(rs[0], p), r1 = get(rs[1], p), r2 = get(rs[2], p);
-                u = mfma(now.T[p][2], r0, u);
-                u = mfma(now.T[p][1], r1, u);
-                u = mfma(now.T[p][0], r2, u);
-                u = mfma(now.T[p][1], r0, u);
-                u = mfma(now.T[p][0], r1, u);
-                u = mfma(now.T[p][0], r0, u);
-            }
-        f32x4 uk = u;
-#pragma unroll
-        for (int r = 0; r < 4; ++r) uk[r] *= now.keep[r];
-        put3(ks, uk);
-        float lo[4];
-#pragma unroll
-        for (int j = 0; j < 4; ++j) lo[j] = u[j] - __uint_as_float(__float_as_uint(u[j]) & 0xFFFF0000u);
-        us[0][wave][lane] = u32x2{tops(__float_as_uint(u[0]), __float_as_uint(u[1])), tops(__float_as_uint(u[2]), __float_as_uint(u[3]))};
-        us[1][wave][lane] = u32x2{tops(__float_as_uint(lo[0]), __float_as_uint(lo[1])), tops(__float_as_uint(lo[2]), __float_as_uint(lo[3]))};
-        lds_barrier();
+    const uint32_t at16 = lane * 16;
+    const int mine = token_of(wt, g4, 0);  // the first of this lane's four tokens
+    __syncthreads();                        // poison
+    // The barriers of a chunk, which all eight waves pass: behind the first xs and ss are there, behind the second rs, behind the
+    // third us and ks. What they hold is read before the next barrier but one, and written again behind it.
+    // PAIRS: of column tiles in the wave's rows of T and P. Each piece of a chunk is requested as soon as the one two chunks before
+    // it has been used, into its registers: one chunk ahead, the loads' latency was on the way of every chunk.
+    auto carry = [&](auto count) __attribute__((always_inline)) {
+        constexpr int PAIRS = decltype(count)::value;
+        float *state = a.state + s.slot * a.s_slot + ((int64_t)h * DK + 16 * TS * wave + 4 * TS * g4) * a.Dv + col;
+        f32x4 S[TS];
 #pragma unroll
         for (int t = 0; t < TS; ++t)
 #pragma unroll
-            for (int r = 0; r < 4; ++r) S[t][r] *= now.fade;
+            for (int r = 0; r < 4; ++r) S[t][r] = state[(int64_t)(4 * t + r) * a.Dv];
+        // byte offsets of a whole chunk's rows from its first
+        const uint32_t kstep = (uint32_t)a.k_t * 2, vstep = (uint32_t)a.v_t * 2, kcol = (16 * TS * wave + 4 * TS * g4) * 2, vcol = col * 2;
+        uint32_t ko[4], vo[4];
 #pragma unroll
-        for (int p = 0; p < 2; ++p)
+        for (int i = 0; i < 4; ++i) ko[i] = token_at(i, n16) * kstep + kcol, vo[i] = (mine + i) * vstep + vcol;
+        StateChunk<TS> now;
+        // past the last chunk: the last one again, not used
+        auto fetch_k = [&](int c, StateChunk<TS> &o) __attribute__((always_inline)) {
+            c = min(c, chunks - 1);
+            const uint16_t *kc = kp + (int64_t)c * kC * a.k_t;
+            const int left = s.n - 1 - c * kC;
+            if (left >= kC - 1) {
 #pragma unroll
-            for (int i = 2; i >= 0; --i) {
-                const bf16x8 o = get(ks[i], p);
+                for (int i = 0; i < 4; ++i) o.K[i] = load_piece<TS>(kc, ko[i]);
+            } else {
 #pragma unroll
-                for (int t = 0; t < TS; ++t) S[t] = mfma(now.KT[t][p], o, S[t]);
+                for (int i = 0; i < 4; ++i) o.K[i] = load_piece<TS>(kc, min(token_at(i, n16), left) * kstep + kcol);
             }
-        f32x4 O;
+        };
+        auto fetch_v = [&](int c, StateChunk<TS> &o) __attribute__((always_inline)) {
+            c = min(c, chunks - 1);
+            const uint8_t *vc = reinterpret_cast<const uint8_t *>(vp + (int64_t)c * kC * a.v_t);
+            const int left = s.n - 1 - c * kC;
+            if (left >= kC - 1) {
 #pragma unroll
-        for (int r = 0; r < 4; ++r) O[r] = now.out[r] * y[r];
+                for (int i = 0; i < 4; ++i) o.v[i] = *reinterpret_cast<const uint16_t *>(vc + vo[i]);
+            } else {
 #pragma unroll
-        for (int p = 0; p < 2; ++p)
-            if (p <= wave >> 1) {
-                const bf16x8 u0 = get(us[0], p), u1 = get(us[1], p);
-                O = mfma(now.P[p][1], u0, O);
-                O = mfma(now.P[p][0], u1, O);
-                O = mfma(now.P[p][0], u0, O);
+                for (int i = 0; i < 4; ++i) o.v[i] = *reinterpret_cast<const uint16_t *>(vc + min(mine + i, left) * vstep + vcol);
             }
-        const int from = poison[n16];
+            const Words *words = reinterpret_cast<const Words *>(heads + (int64_t)c * a.Hv * kHeadBytes + kTBytes + kPBytes);
+            o.in = __builtin_bit_cast(f32x4, load16(words->in, mine * 4));
+            o.keep = __builtin_bit_cast(f32x4, load16(words->keep, mine * 4));
+            o.fade = words->fade, o.bad = words->bad, o.use = words->use;
+        };
+        auto fetch_t = [&](int c, StateChunk<TS> &o) __attribute__((always_inline)) {
+            c = min(c, chunks - 1);
 #pragma unroll
-        for (int r = 0; r < 4; ++r) {
-            const int i = c * kC + token_of(wave, g4, r);
-            if (i < s.n) a.out[(int64_t)(s.t0 + i) * a.o_t + h * a.o_h + col] = i >= from ? (uint16_t)0x7fc0 : (uint16_t)f32_to_bf16(O[r]);
-        }
+            for (int p = 0; p < PAIRS; ++p) {
+                const uint8_t *blk = heads + (int64_t)c * a.Hv * kHeadBytes + block_of(wave, p) * 3072;
+#pragma unroll
+                for (int i = 0; i < 3; ++i) o.T[p][i] = __builtin_bit_cast(bf16x8, load16(blk, at16 + i * 1024));
+            }
+        };
+        auto fetch_kt = [&](int c, StateChunk<TS> &o) __attribute__((always_inline)) {
+            c = min(c, chunks - 1);
+            const uint8_t *key = keys + (int64_t)c * a.Hk * (DK / 16 * 2048) + wave * TS * 2048;
+#pragma unroll
+            for (int t = 0; t < TS; ++t)
+#pragma unroll
+                for (int p = 0; p < 2; ++p) o.KT[t][p] = __builtin_bit_cast(bf16x8, load16(key + t * 2048, at16 + p * 1024));
+        };
+        auto put = [&](u32x2 (*to)[4][64], int i, float (&r)[4]) __attribute__((always_inline)) {  // the leading bits; r: what is left
+            to[i][wave][lane] = u32x2{tops(__float_as_uint(r[0]), __float_as_uint(r[1])), tops(__float_as_uint(r[2]), __float_as_uint(r[3]))};
+#pragma unroll
+            for (int j = 0; j < 4; ++j) r[j] -= __uint_as_float(__float_as_uint(r[j]) & 0xFFFF0000u);
+        };
+        auto chunk = [&](int c, StateChunk<TS> &now) __attribute__((always_inline)) {
+            float s8[8];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) s8[j] = S[0][j], s8[4 + j] = TS == 2 ? S[TS - 1][j] : 0.f;
+            bf16x8 so[3];
+            split(s8, so);
+            ss[wave][0][lane] = __builtin_bit_cast(u32x4, so[0]), ss[wave][1][lane] = __builtin_bit_cast(u32x4, so[1]);
+            if (now.use != ~0ull) {
+                const u32x4 none = {0u, 0u, 0u, 0u};
+#pragma unroll
+                for (int t = 0; t < 4; ++t)
+                    if (!(now.use >> token_at(t, n16) & 1)) now.K[t] = __builtin_bit_cast(bf16x8, none);
+            }
+            f32x4 X[4];
+#pragma unroll
+            for (int t = 0; t < 4; ++t) X[t] = mfma(now.K[t], so[2], zero);
+#pragma unroll
+            for (int t = 0; t < 4; ++t) X[t] = mfma(now.K[t], so[1], X[t]);
+#pragma unroll
+            for (int t = 0; t < 4; ++t) X[t] = mfma(now.K[t], so[0], X[t]);
+            fetch_k(c + 1, now);
+#pragma unroll
+            for (int t = 0; t < 4; ++t) xs[wave][t][lane] = X[t];
+            lds_barrier();
+            // this wave's 16 tokens: what the state does not explain of them
+            const f32x4 x = (xs[0][wave][lane] + xs[1][wave][lane]) + (xs[2][wave][lane] + xs[3][wave][lane]);
+            float r[4], v[4];
+            bool odd = now.bad < kC;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                v[j] = bf16_to_f32(now.v[j]);
+                odd |= !finite(v[j]);
+                r[j] = v[j] - now.in[j] * x[j];
+            }
+            if (now.use != ~0ull || __any(odd)) {
+                int at = now.bad;
+#pragma unroll
+                for (int j = 3; j >= 0; --j) {
+                    const bool use = now.use >> (mine + j) & 1;
+                    if (use && !finite(v[j])) at = min(at, mine + j);
+                    r[j] = !use ? 0.f : finite(v[j]) ? r[j] : -now.in[j] * x[j];
+                }
+                if (at < kC) atomicMin(&poison[n16], c * kC + at);
+            }
+            const float fade = now.fade;
+            const f32x4 keep = now.keep;
+            fetch_v(c + 1, now);
+#pragma unroll
+            for (int i = 0; i < 3; ++i) put(rs, i, r);
+            lds_barrier();
+            // U = T r
+            f32x4 u = zero, u2 = zero;
+#pragma unroll
+            for (int p = 0; p < PAIRS; ++p) {
+                const bf16x8 r0 = pair_of(rs[0], p), r1 = pair_of(rs[1], p), r2 = pair_of(rs[2], p);
+                u2 = mfma(now.T[p][2], r0, u2), u = mfma(now.T[p][1], r0, u);
+                u2 = mfma(now.T[p][1], r1, u2), u = mfma(now.T[p][0], r1, u);
+                u2 = mfma(now.T[p][0], r2, u2), u = mfma(now.T[p][0], r0, u);
+            }
+            fetch_t(c + 1, now);
+            u += u2;
+            float uu[4], uk[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) uu[j] = u[j], uk[j] = u[j] * keep[j];
+#pragma unroll
+            for (int i = 0; i < 3; ++i) put(ks, i, uk);
+#pragma unroll
+            for (int i = 0; i < 2; ++i) put(us, i, uu);
+            lds_barrier();
+#pragma unroll
+            for (int t = 0; t < TS; ++t)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) S[t][j] *= fade;
+#pragma unroll
+            for (int i = 2; i >= 0; --i)
+#pragma unroll
+                for (int p = 0; p < 2; ++p) {
+                    const bf16x8 o = pair_of(ks[i], p);
+#pragma unroll
+                    for (int t = 0; t < TS; ++t) S[t] = mfma(now.KT[t][p], o, S[t]);
+                }
+            fetch_kt(c + 1, now);
+        };
+        auto fetch = [&](int c, StateChunk<TS> &o) __attribute__((always_inline)) { fetch_k(c, o), fetch_v(c, o), fetch_t(c, o), fetch_kt(c, o); };
+        fetch(0, now);
+        for (int c = 0; c < chunks; ++c) chunk(c, now);
+        const bool lost = poison[n16] != 0x7fffffff;
+#pragma unroll
+        for (int t = 0; t < TS; ++t)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) state[(int64_t)(4 * t + r) * a.Dv] = lost ? qnan() : S[t][r];
     };
-    Chunk<TS> even, other;
-    fetch(0, even);
-    __syncthreads();  // poison
-    for (int c = 0; c < chunks; c += 2) {
-        chunk(c, even, other);
-        if (c + 1 < chunks) chunk(c + 1, other, even);
-    }
-    const bool lost = poison[n16] != 0x7fffffff;
+    auto output = [&](auto count) __attribute__((always_inline)) {
+        constexpr int PAIRS = decltype(count)::value;
+        const uint32_t qstep = (uint32_t)a.q_t * 2, ostep = (uint32_t)a.o_t * 2, qcol = 4 * TS * g4 * 2;
+        const uint32_t qo = token_at(wt, n16) * qstep + qcol;
+        uint32_t oo[4];
 #pragma unroll
-    for (int t = 0; t < TS; ++t)
+        for (int r = 0; r < 4; ++r) oo[r] = (mine + r) * ostep + col * 2;
+        OutChunk now;
+        auto fetch_q = [&](int c, OutChunk &o) __attribute__((always_inline)) {
+            c = min(c, chunks - 1);
+            const uint16_t *qc = qp + (int64_t)c * kC * a.q_t;
+            const int left = s.n - 1 - c * kC;
+            const uint32_t off = left >= kC - 1 ? qo : min(token_at(wt, n16), left) * qstep + qcol;
 #pragma unroll
-        for (int r = 0; r < 4; ++r) state[(int64_t)(4 * t + r) * a.Dv] = lost ? qnan() : S[t][r];
+            for (int i = 0; i < 4; ++i) o.Q[i] = load_piece<TS>(qc, off + 32 * TS * i);
+            o.out = __builtin_bit_cast(f32x4, load16(reinterpret_cast<const Words *>(heads + (int64_t)c * a.Hv * kHeadBytes + kTBytes + kPBytes)->out, mine * 4));
+        };
+        auto fetch_p = [&](int c, OutChunk &o) __attribute__((always_inline)) {
+            c = min(c, chunks - 1);
+#pragma unroll
+            for (int p = 0; p < PAIRS; ++p) {
+                const uint8_t *blk = heads + (int64_t)c * a.Hv * kHeadBytes + kTBytes + block_of(wt, p) * 2048;
+#pragma unroll
+                for (int i = 0; i < 2; ++i) o.P[p][i] = __builtin_bit_cast(bf16x8, load16(blk, at16 + i * 1024));
+            }
+        };
+        auto chunk = [&](int c, OutChunk &now) __attribute__((always_inline)) {
+            lds_barrier();
+            f32x4 Y = zero, Y2 = zero;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                Y2 = mfma(now.Q[i], __builtin_bit_cast(bf16x8, ss[i][1][lane]), Y2);
+                Y = mfma(now.Q[i], __builtin_bit_cast(bf16x8, ss[i][0][lane]), Y);
+            }
+            lds_barrier();
+            f32x4 O, O2 = zero;
+#pragma unroll
+            for (int r = 0; r < 4; ++r) O[r] = now.out[r] * (Y[r] + Y2[r]);
+            fetch_q(c + 1, now);
+            lds_barrier();
+            const int from = poison[n16] - c * kC, left = s.n - c * kC;
+#pragma unroll
+            for (int p = 0; p < PAIRS; ++p) {
+                const bf16x8 u0 = pair_of(us[0], p), u1 = pair_of(us[1], p);
+                O2 = mfma(now.P[p][1], u0, O2);
+                O = mfma(now.P[p][0], u0, O);
+                O2 = mfma(now.P[p][0], u1, O2);
+            }
+            fetch_p(c + 1, now);
+            uint8_t *oc = reinterpret_cast<uint8_t *>(op + (int64_t)c * kC * a.o_t);
+            // Always four stores, of rows past the sequence's end too, which the buffer's size leaves out: stores that a branch skips
+            // would make the next chunk's Q wait for all that is in flight.
+            const auto rows = __builtin_amdgcn_make_buffer_rsrc(oc, 0, min(left, kC) * (int)ostep, 0x00020000);
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                const float o = mine + r >= from ? qnan() : O[r] + O2[r];
+                __builtin_amdgcn_raw_buffer_store_b16(__builtin_bit_cast(uint16_t, (__bf16)o), rows, (int)oo[r], 0, 0);
+            }
+        };
+        fetch_q(0, now), fetch_p(0, now);
+        for (int c = 0; c < chunks; ++c) chunk(c, now);
+    };
+    if (wave < 2) carry(std::integral_constant<int, 1>{});
+    else if (wave < 4) carry(std::integral_constant<int, 2>{});
+    else if (wave < 6) output(std::integral_constant<int, 1>{});
+    else output(std::integral_constant<int, 2>{});
 }
 
 }  // namespace
@@ -450,10 +539,10 @@ void prefill(const Args &a, int Dk, void *ws, hipStream_t s) {
     const unsigned prep = (unsigned)(a.Hv * slots);
     if (Dk == 64) {
         delta_prepare_kernel<64><<<prep, 256, 0, s>>>(a, w);
-        delta_scan_kernel<64><<<(unsigned)(pairs8 * (a.Dv / 16)), 256, 0, s>>>(a, w, pairs8);
+        delta_scan_kernel<64><<<(unsigned)(pairs8 * (a.Dv / 16)), 512, 0, s>>>(a, w, pairs8);
     } else {
         delta_prepare_kernel<128><<<prep, 256, 0, s>>>(a, w);
-        delta_scan_kernel<128><<<(unsigned)(pairs8 * (a.Dv / 16)), 256, 0, s>>>(a, w, pairs8);
+        delta_scan_kernel<128><<<(unsigned)(pairs8 * (a.Dv / 16)), 512, 0, s>>>(a, w, pairs8);
     }
 }
 
