@@ -4,10 +4,10 @@
 // logits q is all on the draft (a head that proposes its best token).
 //
 // The results are whole numbers that a border decides, and a token is picked out of sums over a vocabulary: probabilities and sums
-// are FP64. All logits are read once, by as many blocks as they need: rows in chunks of 2048, a chunk's largest value, its
+// are FP64. All logits are read once, by as many blocks as they need: rows in chunks of 4096, a chunk's largest value, its
 // place and its sum of exponentials. Then a wave combines a row's chunks, the rows of a sequence at once, which tells the last row that
-// counts; that one's chunks of max(p - q, 0) are summed (second launch, with draft logits only), and one block a sequence
-// finds the chunk, and in it the token, at which the running sum passes u times the total. Sums are taken in one order, whatever
+// counts; that one's chunks of max(p - q, 0) are summed where there are draft logits, and one block a sequence finds the chunk,
+// and in it the token, at which the running sum passes u times the total (second launch). Sums are taken in one order, whatever
 // the schedule.
 #include "common.hpp"
 
@@ -16,7 +16,7 @@
 namespace sx {
 namespace {
 
-constexpr int kChunk = 2048, kThreads = 256, kEach = kChunk / kThreads, kMaxRows = 256, kMaxSeqs = 1024;
+constexpr int kChunk = 4096, kThreads = 256, kEach = kChunk / kThreads, kDrawThreads = 512, kDrawEach = kChunk / kDrawThreads, kMaxRows = 256, kMaxSeqs = 1024;
 
 struct Part {
     double sum;  // of exp((x - top) / temperature)
@@ -26,11 +26,13 @@ struct Part {
 
 // What a sequence's rows come to.
 struct Verdict {
-    double m, z, mq, zq;  // of the row a token is drawn from: largest logit and sum, the target's and the draft's
+    double m, z, mq, zq;  // of the row a token is drawn from: largest logit and 1 / sum, the target's and the draft's
     int32_t kept;         // drafts that stay
     int32_t status;
     int32_t kind;         // below
     int32_t best;         // the row's largest logit's place
+    int32_t t0, draft;    // the sequence's first row; the row's draft
+    double draw;          // the row's second number
 };
 enum { kNone, kTarget, kHole, kRest, kGreedy };  // nothing; from p; from p without the draft; from max(p - q, 0); the best
 
@@ -42,6 +44,7 @@ struct Args {
     int32_t *tokens, *count, *status;
     Part *parts, *draft_parts;  // [T][chunks]
     double *rest;               // [B][chunks]
+    int32_t *arrived;           // [B]: blocks whose sum is there
     Verdict *verdicts;          // [B]
     int64_t ld, draft_ld;
     int32_t T, V, Vd, B, max_rows, chunks, draft_chunks;
@@ -50,116 +53,201 @@ struct Args {
 __device__ __forceinline__ float load(const float *p) { return *p; }
 __device__ __forceinline__ float load(const uint16_t *p) { return bf16_to_f32(*p); }
 
+// N neighbouring logits in 16-byte loads; rows start at any element. Places from `left` on are -inf.
+typedef float f32x4 __attribute__((ext_vector_type(4), aligned(4)));
+typedef uint16_t u16x8 __attribute__((ext_vector_type(8), aligned(2)));
+template <int N>
+__device__ __forceinline__ void load_run(const float *p, int left, float (&x)[N]) {
+    if (left >= N) {
+#pragma unroll
+        for (int i = 0; i < N; i += 4) {
+            const f32x4 v = *reinterpret_cast<const f32x4 *>(p + i);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) x[i + j] = v[j];
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < N; ++i) x[i] = i < left ? p[i] : -INFINITY;
+    }
+}
+template <int N>
+__device__ __forceinline__ void load_run(const uint16_t *p, int left, float (&x)[N]) {
+    if (left >= N) {
+#pragma unroll
+        for (int i = 0; i < N; i += 8) {
+            const u16x8 v = *reinterpret_cast<const u16x8 *>(p + i);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) x[i + j] = bf16_to_f32(v[j]);
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < N; ++i) x[i] = i < left ? bf16_to_f32(p[i]) : -INFINITY;
+    }
+}
+
 __device__ __forceinline__ bool usable(const Args &a, int b, int &t0, int &n) {
     t0 = a.starts[b];
     n = a.starts[b + 1] - t0;
     return t0 >= 0 && n >= 0 && (int64_t)t0 + n <= a.T && n <= a.max_rows;
 }
 
+// Across a wave, the result in all lanes: neighbours by DPP, then halves of 32 and of 64 lanes.
+template <int CTRL>
+__device__ __forceinline__ uint32_t dpp(uint32_t v) { return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, 0xF, 0xF, false); }
+template <int STEP>
+__device__ __forceinline__ uint32_t other(uint32_t v) {
+    if constexpr (STEP == 0) return dpp<0xB1>(v);
+    else if constexpr (STEP == 1) return dpp<0x4E>(v);
+    else if constexpr (STEP == 2) return dpp<0x141>(v);
+    else if constexpr (STEP == 3) return dpp<0x140>(v);
+    else {
+        const bool up = threadIdx.x & (STEP == 4 ? 16 : 32);
+        const auto x = STEP == 4 ? __builtin_amdgcn_permlane16_swap(v, v, false, false) : __builtin_amdgcn_permlane32_swap(v, v, false, false);
+        return up ? x[0] : x[1];
+    }
+}
+template <int STEP>
+__device__ __forceinline__ double other(double v) {
+    const uint64_t u = (uint64_t)__double_as_longlong(v);
+    return __longlong_as_double((long long)((uint64_t)other<STEP>((uint32_t)(u >> 32)) << 32 | other<STEP>((uint32_t)u)));
+}
 __device__ __forceinline__ double wave_sum(double v) {
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) v += __shfl_xor(v, d);
-    return v;
+    v += other<0>(v), v += other<1>(v), v += other<2>(v);
+    v += other<3>(v), v += other<4>(v);
+    return v + other<5>(v);
+}
+// The largest value and its lowest place.
+template <int STEP>
+__device__ __forceinline__ void best_step(float &top, int &at) {
+    const float o = __uint_as_float(other<STEP>(__float_as_uint(top)));
+    const int oa = (int)other<STEP>((uint32_t)at);
+    if (o > top || (o == top && oa < at)) top = o, at = oa;
+}
+__device__ __forceinline__ void wave_best(float &top, int &at) {
+    best_step<0>(top, at), best_step<1>(top, at), best_step<2>(top, at);
+    best_step<3>(top, at), best_step<4>(top, at), best_step<5>(top, at);
 }
 
-// exp(x / t) for x <= 0 (x -inf: 0).
-__device__ __forceinline__ double weight(double x, double over_t) { return exp(x * over_t); }
+// exp(y) for y <= 0 (-inf: 0) in FP64: 2^n times the power series of e^r, |r| <= ln(2) / 2, to the eleventh power (6e-15 is left).
+// The library's takes more instructions for ranges that a softmax does not reach; of these a chunk's launch consists.
+__device__ __forceinline__ double weight(double y) {
+    y = fmax(y, -800.0);  // 0 from there on
+    const double n = rint(y * 1.4426950408889634);
+    const double r = fma(n, -4.7493250390316726e-07, fma(n, -0.6931467056274414, y));  // ln(2): 21 bits, whose multiples are exact, and the rest
+    double p = 1.0 / 39916800.0;
+    p = fma(p, r, 1.0 / 3628800.0);
+    p = fma(p, r, 1.0 / 362880.0);
+    p = fma(p, r, 1.0 / 40320.0);
+    p = fma(p, r, 1.0 / 5040.0);
+    p = fma(p, r, 1.0 / 720.0);
+    p = fma(p, r, 1.0 / 120.0);
+    p = fma(p, r, 1.0 / 24.0);
+    p = fma(p, r, 1.0 / 6.0);
+    p = fma(p, r, 0.5);
+    p = fma(p, r, 1.0);
+    p = fma(p, r, 1.0);
+    return ldexp(p, (int)n);
+}
 
 template <typename T>
 __global__ void __launch_bounds__(kThreads) accept_parts_kernel(const Args a) {
-    __shared__ int found;
     __shared__ float tops[4];
-    __shared__ int ats[4];
+    __shared__ int ats[4], owners[4];
     __shared__ double sums[4];
-    const int chunk = blockIdx.x;
+    const int chunk = blockIdx.x, wave = threadIdx.x >> 6;
     const int64_t row = blockIdx.y % a.T;
     const bool draft = blockIdx.y >= (unsigned)a.T;
     if (chunk >= (draft ? a.draft_chunks : a.chunks)) return;
-    if (threadIdx.x == 0) found = -1;
-    __syncthreads();
-    for (int b = threadIdx.x; b < a.B; b += kThreads) {
-        int t0, n;
-        if (usable(a, b, t0, n) && row >= t0 && row < t0 + n - (draft ? 1 : 0)) found = b;  // a last row has no draft
-    }
-    __syncthreads();
-    if (found < 0) return;
-    const float temp = a.temperature[found];
     const int V = draft ? a.Vd : a.V, first = chunk * kChunk;
     const T *p = static_cast<const T *>(draft ? a.draft_logits : a.logits) + row * (draft ? a.draft_ld : a.ld) + first;
     float x[kEach];
 #pragma unroll
-    for (int i = 0; i < kEach; ++i) {
-        const int at = threadIdx.x + i * kThreads;
-        x[i] = first + at < V ? load(p + at) : -INFINITY;
+    for (int i = 0; i < kEach / 8; ++i) {
+        const int k = ((int)threadIdx.x + i * kThreads) * 8;
+        float run[8];
+        load_run<8>(p + min(k, V - 1 - first), V - first - k, run);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) x[8 * i + j] = run[j];
     }
+    int owner = -1;  // the row's sequence; a last row has no draft
+    for (int b = threadIdx.x; b < a.B; b += kThreads) {
+        int t0, n;
+        if (usable(a, b, t0, n) && row >= t0 && row < t0 + n - (draft ? 1 : 0)) owner = b;
+    }
+    const uint64_t has = __ballot(owner >= 0);
+    owner = has != 0 ? __shfl(owner, __builtin_ctzll(has)) : -1;
     float top = -INFINITY;
     int at = 0x7fffffff;
     bool nan = false;
 #pragma unroll
     for (int i = 0; i < kEach; ++i) {
         nan |= x[i] != x[i];
-        if (x[i] > top) top = x[i], at = first + threadIdx.x + i * kThreads;
+        if (x[i] > top) top = x[i], at = first + ((int)threadIdx.x + i / 8 * kThreads) * 8 + i % 8;
     }
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) {
-        const float o = __shfl_xor(top, d);
-        const int oa = __shfl_xor(at, d);
-        if (o > top || (o == top && oa < at)) top = o, at = oa;
-    }
-    if ((threadIdx.x & 63) == 0) tops[threadIdx.x >> 6] = top, ats[threadIdx.x >> 6] = at;
+    wave_best(top, at);
+    if ((threadIdx.x & 63) == 0) tops[wave] = top, ats[wave] = at, owners[wave] = owner;
     nan = __syncthreads_or(nan);
-    top = tops[0], at = ats[0];
+    top = tops[0], at = ats[0], owner = max(max(owners[0], owners[1]), max(owners[2], owners[3]));
+    if (owner < 0) return;
 #pragma unroll
     for (int w = 1; w < 4; ++w)
         if (tops[w] > top || (tops[w] == top && ats[w] < at)) top = tops[w], at = ats[w];
+    const float temp = a.temperature[owner];
     double sum = 0.0;
     if (temp > 0.f && top > -INFINITY && top < INFINITY) {
         const double over_t = 1.0 / (double)temp;
 #pragma unroll
-        for (int i = 0; i < kEach; ++i) sum += weight((double)x[i] - (double)top, over_t);
+        for (int i = 0; i < kEach; ++i) sum += weight(((double)x[i] - (double)top) * over_t);
     }
     sum = wave_sum(sum);
-    if ((threadIdx.x & 63) == 0) sums[threadIdx.x >> 6] = sum;
+    if ((threadIdx.x & 63) == 0) sums[wave] = sum;
     __syncthreads();
     if (threadIdx.x == 0)
         (draft ? a.draft_parts + row * a.draft_chunks : a.parts + row * a.chunks)[chunk] = Part{(sums[0] + sums[1]) + (sums[2] + sums[3]), top, nan ? -1 : at};
 }
 
 // A row's largest logit, its place (-1: a NaN) and its sum, by one wave, in all lanes.
-__device__ __forceinline__ void row_stats(const Part *parts, int chunks, double over_t, float &m, int &at, double &z) {
+struct Row {
+    float m;
+    int at;
+    double z;
+};
+// `mine`: the lane's first part, requested before. One copy in the code: a launch of few blocks waits for its instructions more than
+// for its data.
+__device__ __attribute__((noinline)) Row row_stats(const Part *parts, int chunks, Part mine, double over_t) {
     const int lane = threadIdx.x & 63;
-    float top = -INFINITY;
-    at = 0x7fffffff;
+    Row r{-INFINITY, 0x7fffffff, 0.0};
     bool nan = false;
     for (int c = lane; c < chunks; c += 64) {
-        const Part p = parts[c];
-        nan |= p.at < 0;
-        if (p.top > top) top = p.top, at = p.at;
+        const Part x = c < 64 ? mine : parts[c];
+        nan |= x.at < 0;
+        if (x.top > r.m || (x.top == r.m && x.at < r.at)) r.m = x.top, r.at = x.at;
     }
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) {
-        const float o = __shfl_xor(top, d);
-        const int oa = __shfl_xor(at, d);
-        if (o > top || (o == top && oa < at)) top = o, at = oa;
-    }
-    if (__any(nan)) at = -1;
-    m = top;
-    double sum = 0.0;
-    if (top > -INFINITY && top < INFINITY)
+    wave_best(r.m, r.at);
+    if (__any(nan)) r.at = -1;
+    if (fabsf(r.m) < INFINITY)
+#pragma unroll 1
         for (int c = lane; c < chunks; c += 64) {
-            const Part p = parts[c];
-            if (p.top > -INFINITY) sum += p.sum * weight((double)p.top - (double)top, over_t);
+            const Part x = c < 64 ? mine : parts[c];
+            r.z += x.sum * weight(((double)x.top - (double)r.m) * over_t);
         }
-    z = wave_sum(sum);
+    r.z = wave_sum(r.z);
+    return r;
 }
+
+// What a block knows of its sequence's rows.
+struct Rows {
+    double stats[5 * kMaxRows];
+    uint8_t fate[kMaxRows];
+};
 
 // Every thread of the block calls it; the verdict is in `v` (LDS) for all of them.
 template <typename T>
-__device__ __forceinline__ void decide(const Args &a, int b, Verdict &v, uint8_t *fate, double *stats) {
+__device__ __forceinline__ void decide(const Args &a, int b, Verdict &v, Rows &rows) {
     int t0, n;
     const bool ok = usable(a, b, t0, n);
     if (!ok || n == 0) {
-        if (threadIdx.x == 0) v = Verdict{0, 0, 0, 0, 0, ok ? 0 : -1, kNone, 0};
+        if (threadIdx.x == 0) v = Verdict{0, 0, 0, 0, 0, ok ? 0 : -1, kNone, 0, 0, 0, 0};
         __syncthreads();
         return;
     }
@@ -167,56 +255,49 @@ __device__ __forceinline__ void decide(const Args &a, int b, Verdict &v, uint8_t
     const bool greedy = temp <= 0.f;
     const double over_t = greedy ? 0.0 : 1.0 / (double)temp;
     const int wave = threadIdx.x >> 6;
-    for (int i = wave; i < n; i += kThreads / 64) {
+    for (int i = wave; i < n; i += kDrawThreads / 64) {
         const int64_t t = t0 + i;
-        float m, mq = 0.f;
-        int at, atq = 0;
-        double z, zq = 1.0;
-        row_stats(a.parts + t * a.chunks, a.chunks, over_t, m, at, z);
-        bool bad = at < 0 || !(fabsf(m) < INFINITY) || !(fabsf(temp) < INFINITY), stays = false;
-        if (i + 1 < n) {
-            const int d = a.drafts[t];
-            if (d < 0 || d >= a.V) {
-                bad = true;
-            } else if (greedy) {
-                stays = d == at;
-            } else if (!bad) {
+        const bool drafted = i + 1 < n, both = drafted && a.draft_logits != nullptr && !greedy;
+        const int lane = threadIdx.x & 63;
+        const Part p = a.parts[t * a.chunks + min(lane, a.chunks - 1)], pq = both ? a.draft_parts[t * a.draft_chunks + min(lane, a.draft_chunks - 1)] : Part{};
+        const int d = a.drafts[t];
+        const bool inside = d >= 0 && d < a.V;
+        const double u = a.u[2 * t];
+        const float x = load(static_cast<const T *>(a.logits) + t * a.ld + (inside ? d : 0));
+        const float xq = both && inside && d < a.Vd ? load(static_cast<const T *>(a.draft_logits) + t * a.draft_ld + d) : -INFINITY;
+        const Row r = row_stats(a.parts + t * a.chunks, a.chunks, p, over_t);
+        Row rq{0.f, 0, 1.0};
+        bool bad = r.at < 0 || !(fabsf(r.m) < INFINITY) || !(fabsf(temp) < INFINITY) || (drafted && !inside), stays = false;
+        if (drafted && !bad) {
+            if (greedy) {
+                stays = d == r.at;
+            } else {
                 double q = 1.0;
-                if (a.draft_logits != nullptr) {
-                    row_stats(a.draft_parts + t * a.draft_chunks, a.draft_chunks, over_t, mq, atq, zq);
-                    bad = atq < 0 || !(fabsf(mq) < INFINITY);
-                    q = d < a.Vd ? weight((double)load(static_cast<const T *>(a.draft_logits) + t * a.draft_ld + d) - (double)mq, over_t) / zq : 0.0;
+                if (both) {
+                    rq = row_stats(a.draft_parts + t * a.draft_chunks, a.draft_chunks, pq, over_t);
+                    bad = rq.at < 0 || !(fabsf(rq.m) < INFINITY);
+                    q = weight(((double)xq - (double)rq.m) * over_t) / rq.z;
                 }
-                const double p = weight((double)load(static_cast<const T *>(a.logits) + t * a.ld + d) - (double)m, over_t) / z;
-                stays = a.u[2 * t] * q < p;
+                stays = u * q < weight(((double)x - (double)r.m) * over_t) / r.z;
             }
         }
         if ((threadIdx.x & 63) == 0) {
-            fate[i] = bad ? 2 : stays ? 1 : 0;
-            double *s = stats + 5 * i;
-            s[0] = m, s[1] = z, s[2] = mq, s[3] = zq, s[4] = at;
+            rows.fate[i] = bad ? 2 : stays ? 1 : 0;
+            double *s = rows.stats + 5 * i;
+            s[0] = r.m, s[1] = 1.0 / r.z, s[2] = rq.m, s[3] = 1.0 / rq.z, s[4] = r.at;
         }
     }
     __syncthreads();
     if (threadIdx.x == 0) {
         int j = 0;
-        while (fate[j] == 1) ++j;  // the last row has no draft: it is 0 or 2
-        const double *s = stats + 5 * j;
+        while (rows.fate[j] == 1) ++j;  // the last row has no draft: it is 0 or 2
+        const double *s = rows.stats + 5 * j;
         const bool last = j + 1 == n;
-        v = Verdict{s[0], s[1], s[2], s[3], j, fate[j] == 2 ? 1 + j : 0,
-                    fate[j] == 2 ? kNone : greedy ? kGreedy : last ? kTarget : a.draft_logits != nullptr ? kRest : kHole, (int)s[4]};
+        v = Verdict{s[0], s[1], s[2], s[3], j, rows.fate[j] == 2 ? 1 + j : 0,
+                    rows.fate[j] == 2 ? kNone : greedy ? kGreedy : last ? kTarget : a.draft_logits != nullptr ? kRest : kHole, (int)s[4], t0,
+                    a.drafts[t0 + j], a.u[2 * (int64_t)(t0 + j) + 1]};
     }
     __syncthreads();
-}
-
-// Place i's weight in the row a token is drawn from. Only ratios to the row's total count: kTarget and kHole leave z out.
-template <typename T>
-__device__ __forceinline__ double place(const Args &a, const Verdict &v, int64_t row, double over_t, int i, int kind) {
-    const double p = weight((double)load(static_cast<const T *>(a.logits) + row * a.ld + i) - v.m, over_t);
-    if (kind == kTarget) return p;
-    if (kind == kHole) return i == a.drafts[row] ? 0.0 : p;
-    const double q = i < a.Vd ? weight((double)load(static_cast<const T *>(a.draft_logits) + row * a.draft_ld + i) - v.mq, over_t) / v.zq : 0.0;
-    return fmax(p / v.z - q, 0.0);
 }
 
 __device__ __forceinline__ double block_sum(double v, double *part) {
@@ -224,152 +305,164 @@ __device__ __forceinline__ double block_sum(double v, double *part) {
     __syncthreads();  // part may still be read
     if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = v;
     __syncthreads();
-    return (part[0] + part[1]) + (part[2] + part[3]);
+    return ((part[0] + part[1]) + (part[2] + part[3])) + ((part[4] + part[5]) + (part[6] + part[7]));
 }
 
 template <typename T>
-__global__ void __launch_bounds__(kThreads) accept_rest_kernel(const Args a) {
+__global__ void __launch_bounds__(kDrawThreads) accept_decide_kernel(const Args a) {
     __shared__ Verdict v;
-    __shared__ uint8_t fate[kMaxRows];
-    __shared__ double stats[5 * kMaxRows], part[4];
-    const int b = blockIdx.y, chunk = blockIdx.x;
-    decide<T>(a, b, v, fate, stats);
-    if (chunk == 0 && threadIdx.x == 0) a.verdicts[b] = v;
-    if (v.kind != kRest) return;
-    const int64_t row = a.starts[b] + v.kept;
+    __shared__ Rows rows;
+    decide<T>(a, blockIdx.x, v, rows);
+    if (threadIdx.x == 0) a.verdicts[blockIdx.x] = v, a.arrived[blockIdx.x] = 0;
+}
+
+// Grid (1, B) without draft logits; with them (chunks, B) behind accept_decide_kernel: then a block also sums its chunk of
+// max(p - q, 0), and the last block of a sequence to get there draws. (All of them deciding for themselves: 16 sequences of 38 chunks
+// 21.4 us, 5 us more than both launches.)
+template <typename T, bool DRAFT>
+__global__ void __launch_bounds__(kDrawThreads) accept_draw_kernel(const Args a) {
+    __shared__ Verdict v;
+    __shared__ double part[8], ends[8];
+    __shared__ int chosen, last, firsts[8], lasts[8];
+    const int b = blockIdx.y, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const double over_t = 1.0 / (double)a.temperature[b];
-    double sum = 0.0;
-#pragma unroll
-    for (int i = 0; i < kEach; ++i) {
-        const int at = chunk * kChunk + i * kThreads + threadIdx.x;
-        if (at < a.V) sum += place<T>(a, v, row, over_t, at, kRest);
-    }
-    sum = block_sum(sum, part);
-    if (threadIdx.x == 0) a.rest[(int64_t)b * a.chunks + chunk] = sum;
-}
-
-template <typename T>
-__global__ void __launch_bounds__(kThreads) accept_pick_kernel(const Args a) {
-    __shared__ Verdict v;
-    __shared__ uint8_t fate[kMaxRows];
-    __shared__ double stats[5 * kMaxRows], part[4], before[kThreads];
-    __shared__ int chosen;
-    const int b = blockIdx.x;
-    if (a.draft_logits == nullptr) {
-        decide<T>(a, b, v, fate, stats);
-    } else {
+    if constexpr (DRAFT) {
         if (threadIdx.x == 0) v = a.verdicts[b];
         __syncthreads();
+    } else {
+        __shared__ Rows rows;
+        decide<T>(a, b, v, rows);
     }
-    int t0, n;
-    usable(a, b, t0, n);
-    const int64_t row = (int64_t)t0 + v.kept;
-    int token = -1;
-    if (v.kind == kGreedy) token = v.best;
+    const int64_t row = (int64_t)v.t0 + v.kept;
+    const int draft = v.draft;
+    if (DRAFT && v.kind != kRest && blockIdx.x != 0) return;
+    int token = v.kind == kGreedy ? v.best : -1;
     if (v.kind == kTarget || v.kind == kHole || v.kind == kRest) {
-        const double over_t = 1.0 / (double)a.temperature[b];
         int kind = v.kind;
-        // weights of thread t's run of chunks; a row that has nothing left over the draft's is drawn from p
-        const int per = (a.chunks + kThreads - 1) / kThreads, c0 = min((int)threadIdx.x * per, a.chunks), c1 = min(c0 + per, a.chunks);
-        const int hole = kind == kHole ? a.drafts[row] / kChunk : -1;
-        auto of_chunk = [&](int c) {
-            if (kind == kRest) return a.rest[(int64_t)b * a.chunks + c];
-            const Part p = a.parts[row * a.chunks + c];
-            return p.top > -INFINITY ? p.sum * weight((double)p.top - v.m, over_t) : 0.0;
-        };
-        double hole_sum = 0.0, mine = 0.0, total = 0.0;
-        for (int pass = 0; pass < 2; ++pass) {
-            if (kind == kHole) {  // the draft's chunk without it: by taking it off, what is left would be noise
-                double s = 0.0;
-                for (int i = threadIdx.x; i < kChunk; i += kThreads)
-                    if (hole * kChunk + i < a.V) s += place<T>(a, v, row, over_t, hole * kChunk + i, kHole);
-                hole_sum = block_sum(s, part);
+        const int per = (a.chunks + kDrawThreads - 1) / kDrawThreads, c0 = min((int)threadIdx.x * per, a.chunks), c1 = min(c0 + per, a.chunks);
+        const int hole = kind == kHole ? draft / kChunk : -1;
+        double hole_sum = 0.0, upto = 0.0, mine = 0.0, total = 0.0, goal = 0.0, run0 = 0.0;
+        // Running sums of all threads' values: upto ends with this thread's.
+        auto scan = [&]() {
+            upto = mine;
+#pragma unroll
+            for (int d = 1; d < 64; d <<= 1) {
+                const double x = __shfl_up(upto, d);
+                if (lane >= d) upto += x;
             }
+            __syncthreads();  // ends may still be read
+            if (lane == 63) ends[wave] = upto;
+            __syncthreads();
+            double before = 0.0;
+            total = 0.0;
+#pragma unroll
+            for (int w = 0; w < kDrawThreads / 64; ++w) {
+                if (w == wave) before = total;
+                total += ends[w];
+            }
+            upto += before;
+        };
+        // The first thread's candidate (threads hold rising ones); where rounding left none, the last one's fallback.
+        auto first_of = [&](int candidate, int fallback) {
+            const uint64_t c = __ballot(candidate >= 0), f = __ballot(fallback >= 0);
+            candidate = c != 0 ? __shfl(candidate, __builtin_ctzll(c)) : -1;
+            fallback = f != 0 ? __shfl(fallback, 63 - __builtin_clzll(f)) : -1;
+            __syncthreads();  // they may still be read
+            if (lane == 0) firsts[wave] = candidate, lasts[wave] = fallback;
+            __syncthreads();
+            int got = -1;
+#pragma unroll
+            for (int w = 0; w < kDrawThreads / 64; ++w) got = lasts[w] >= 0 ? lasts[w] : got;
+#pragma unroll
+            for (int w = kDrawThreads / 64 - 1; w >= 0; --w) got = firsts[w] >= 0 ? firsts[w] : got;
+            return got;
+        };
+        auto of_chunk = [&](int c) {
+            if (kind == kRest) return __hip_atomic_load(&a.rest[(int64_t)b * a.chunks + c], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+            if (kind == kHole && c == hole) return hole_sum;
+            const Part p = a.parts[row * a.chunks + c];
+            return p.top > -INFINITY ? p.sum * weight(((double)p.top - v.m) * over_t) : 0.0;
+        };
+        // A chunk's places, kDrawEach neighbouring ones a thread: first the chunk of this block's sum (of the hole: by taking the draft
+        // off its chunk's sum, what is left would be noise), then the one that the token is in. The same code for both.
+        int at_chunk = kind == kRest ? (int)blockIdx.x : hole;
+        bool found = false;
+#pragma unroll 1
+        for (;;) {
+            double w[kDrawEach];
             mine = 0.0;
-            for (int c = c0; c < c1; ++c) mine += kind == kHole && c == hole ? hole_sum : of_chunk(c);
-            total = block_sum(mine, part);
-            if (total > 0.0 || kind == kTarget) break;
-            kind = kTarget;
-        }
-        const double goal = a.u[2 * row + 1] * total;
-        if (threadIdx.x == 0) chosen = -1;
-        before[threadIdx.x] = mine;
-        __syncthreads();
-        if (threadIdx.x == 0) {  // the chunk in which the running sum passes the goal (rounding left it out: the last with anything)
-            double run = 0.0;
-            int last = 0;
-            double last_run = 0.0;
-            for (int t = 0; t < kThreads && chosen < 0; ++t) {
-                if (t * per >= a.chunks) break;
-                if (before[t] > 0.0 && run + before[t] > goal) {
-                    for (int c = t * per; c < min((t + 1) * per, a.chunks); ++c) {
-                        const double w = kind == kHole && c == hole ? hole_sum : of_chunk(c);
-                        if (w > 0.0) last = c, last_run = run;
-                        if (run + w > goal) {
-                            chosen = c, part[0] = run;
-                            break;
-                        }
-                        run += w;
-                    }
-                } else {
-                    if (before[t] > 0.0)
-                        for (int c = t * per; c < min((t + 1) * per, a.chunks); ++c) {
-                            const double w = kind == kHole && c == hole ? hole_sum : of_chunk(c);
-                            if (w > 0.0) last = c, last_run = run;
-                            run += w;
-                        }
+            if (at_chunk >= 0) {
+                const int at0 = at_chunk * kChunk + threadIdx.x * kDrawEach;
+                float x[kDrawEach], xq[kDrawEach];
+                load_run<kDrawEach>(static_cast<const T *>(a.logits) + row * a.ld + min(at0, a.V - 1), a.V - at0, x);
+                if (DRAFT && kind == kRest) load_run<kDrawEach>(static_cast<const T *>(a.draft_logits) + row * a.draft_ld + min(at0, a.Vd - 1), a.Vd - at0, xq);
+#pragma unroll
+                for (int i = 0; i < kDrawEach; ++i) {
+                    w[i] = weight(((double)x[i] - v.m) * over_t);
+                    if (DRAFT && kind == kRest) w[i] = fmax(w[i] * v.z - weight(((double)xq[i] - v.mq) * over_t) * v.zq, 0.0);
+                    if (kind == kHole && at0 + i == draft) w[i] = 0.0;
+                    mine += w[i];
                 }
             }
-            if (chosen < 0) chosen = last, part[0] = last_run;
-        }
-        __syncthreads();
-        const int first = chosen * kChunk;
-        const double run0 = part[0];
-        // in the chunk: eight neighbouring places a thread
-        double w[kEach], own = 0.0;
+            if (found) {
+                scan();
+                double run = run0 + (upto - mine);
+                int pass = -1, some = -1;
 #pragma unroll
-        for (int i = 0; i < kEach; ++i) {
-            const int at = first + threadIdx.x * kEach + i;
-            w[i] = at < a.V ? place<T>(a, v, row, over_t, at, kind) : 0.0;
-            own += w[i];
-        }
-        __syncthreads();
-        double run = own;  // of the wave's lanes up to this one
-#pragma unroll
-        for (int d = 1; d < 64; d <<= 1) {
-            const double x = __shfl_up(run, d);
-            if ((threadIdx.x & 63) >= d) run += x;
-        }
-        if ((threadIdx.x & 63) == 63) before[threadIdx.x >> 6] = run;
-        if (threadIdx.x == 0) chosen = 0x7fffffff;
-        __syncthreads();
-        run += run0 - own;
-        for (int w2 = 0; w2 < (int)(threadIdx.x >> 6); ++w2) run += before[w2];
-        int pass = 0x7fffffff, some = -1;
-#pragma unroll
-        for (int i = 0; i < kEach; ++i) {
-            run += w[i];
-            const int at = first + threadIdx.x * kEach + i;
-            if (w[i] > 0.0) {
-                some = at;
-                if (run > goal) pass = min(pass, at);
+                for (int i = 0; i < kDrawEach; ++i) {
+                    run += w[i];
+                    const int at = at_chunk * kChunk + threadIdx.x * kDrawEach + i;
+                    if (w[i] > 0.0) {
+                        some = at;
+                        if (pass < 0 && run > goal) pass = at;
+                    }
+                }
+                token = first_of(pass, some);
+                break;
             }
-        }
-        atomicMin(&chosen, pass);
-        __syncthreads();
-        token = chosen;
-        if (token == 0x7fffffff) {  // rounding between the chunk's sum and its places: the last place with anything
+            if (at_chunk >= 0) hole_sum = block_sum(mine, part);
+            if (DRAFT && kind == kRest) {
+                if (threadIdx.x == 0) {
+                    // written through to where all XCDs see it, and counted once it is there
+                    __hip_atomic_store(&a.rest[(int64_t)b * a.chunks + blockIdx.x], hole_sum, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+                    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+                    last = __hip_atomic_fetch_add(&a.arrived[b], 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == (int)gridDim.x - 1;
+                }
+                __syncthreads();
+                if (!last) return;
+            }
+            // the weights of this thread's run of chunks; a row that has nothing left over the draft's is drawn from p
+            for (;;) {
+                mine = 0.0;
+#pragma unroll 1
+                for (int c = c0; c < c1; ++c) mine += of_chunk(c);
+                scan();
+                if (total > 0.0 || kind == kTarget) break;
+                kind = kTarget;
+            }
+            goal = v.draw * total;
+            const int run_of = first_of(mine > 0.0 && upto > goal ? (int)threadIdx.x : -1, mine > 0.0 ? (int)threadIdx.x : -1);
+            if ((int)threadIdx.x == run_of) {
+                double run = upto - mine, some_run = run;
+                int some = c0;
+                if (per > 1)
+#pragma unroll 1
+                    for (int c = c0; c < c1; ++c) {
+                        const double x = of_chunk(c);
+                        if (x > 0.0) some = c, some_run = run;
+                        if (x > 0.0 && run + x > goal) break;
+                        run += x;
+                    }
+                chosen = some, part[0] = some_run;
+            }
             __syncthreads();
-            if (threadIdx.x == 0) chosen = -1;
-            __syncthreads();
-            atomicMax(&chosen, some);
-            __syncthreads();
-            token = chosen;
+            at_chunk = chosen, run0 = part[0], found = true;
+            __syncthreads();  // both are written again
         }
     }
     const int kept = v.kept;
-    for (int i = threadIdx.x; i < a.max_rows; i += kThreads)
-        a.tokens[(int64_t)b * a.max_rows + i] = i < kept ? a.drafts[t0 + i] : i == kept ? token : -1;
+    for (int i = threadIdx.x; i < a.max_rows; i += kDrawThreads)
+        a.tokens[(int64_t)b * a.max_rows + i] = i < kept ? a.drafts[v.t0 + i] : i == kept ? token : -1;
     if (threadIdx.x == 0) a.count[b] = v.kind == kNone ? kept : kept + 1, a.status[b] = v.status;
 }
 
@@ -381,7 +474,7 @@ Sizes sizes(int64_t T, int64_t B, int64_t V, int64_t Vd) {
     s.chunks = (V + kChunk - 1) / kChunk, s.draft_chunks = (Vd + kChunk - 1) / kChunk;
     s.parts = T * s.chunks * (int64_t)sizeof(Part), s.draft_parts = T * s.draft_chunks * (int64_t)sizeof(Part);
     s.rest = Vd > 0 ? B * s.chunks * 8 : 0;
-    s.bytes = s.parts + s.draft_parts + s.rest + (Vd > 0 ? B * (int64_t)sizeof(Verdict) : 0);
+    s.bytes = s.parts + s.draft_parts + s.rest + (Vd > 0 ? B * ((int64_t)sizeof(Verdict) + 4) : 0);
     return s;
 }
 
@@ -389,8 +482,9 @@ template <typename T>
 void launch(const Args &a, hipStream_t s) {
     const bool drafted = a.draft_logits != nullptr;
     accept_parts_kernel<T><<<dim3((unsigned)std::max(a.chunks, a.draft_chunks), (unsigned)(drafted ? 2 * a.T : a.T)), kThreads, 0, s>>>(a);
-    if (drafted) accept_rest_kernel<T><<<dim3((unsigned)a.chunks, (unsigned)a.B), kThreads, 0, s>>>(a);
-    accept_pick_kernel<T><<<(unsigned)a.B, kThreads, 0, s>>>(a);
+    if (drafted) accept_decide_kernel<T><<<(unsigned)a.B, kDrawThreads, 0, s>>>(a);
+    if (drafted) accept_draw_kernel<T, true><<<dim3((unsigned)a.chunks, (unsigned)a.B), kDrawThreads, 0, s>>>(a);
+    else accept_draw_kernel<T, false><<<dim3(1, (unsigned)a.B), kDrawThreads, 0, s>>>(a);
 }
 
 bool sizes_ok(int64_t T, int64_t B, int64_t V, int64_t Vd) {
@@ -443,6 +537,7 @@ extern "C" int sx_mtp_accept_sampled(const void *logits, int64_t ld, int64_t T, 
     uint8_t *w = static_cast<uint8_t *>(ws);
     const Args a{logits, draft_logits, drafts, starts, u, temperature, tokens, count, status, reinterpret_cast<Part *>(w),
                  reinterpret_cast<Part *>(w + z.parts), reinterpret_cast<double *>(w + z.parts + z.draft_parts),
+                 reinterpret_cast<int32_t *>(w + z.parts + z.draft_parts + z.rest + B * (int64_t)sizeof(Verdict)),
                  reinterpret_cast<Verdict *>(w + z.parts + z.draft_parts + z.rest), ld, draft_ld, (int32_t)T, (int32_t)V, (int32_t)Vd, (int32_t)B,
                  (int32_t)max_rows, (int32_t)z.chunks, (int32_t)z.draft_chunks};
     if (act == SX_ACT_F32) launch<float>(a, stream_of(stream));
