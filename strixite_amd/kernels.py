@@ -5,6 +5,7 @@ torch supplies device memory and the stream (torch.cuda.current_stream() unless 
 a libstrixite_amd.so kernel. Activations are torch.float32 (Act::F32) or torch.bfloat16 (Act::BF16, raw bits).
 """
 import ctypes
+import functools
 import struct
 
 import torch
@@ -466,7 +467,7 @@ def _is_err(err):
 
 def _run(dev, f, *args, stream=None):
     """f(*args, stream) on GPU dev, whichever is current."""
-    if dev != torch.cuda.current_device():
+    if dev != torch._C._cuda_getDevice():
         with torch.cuda.device(dev):
             return _run(dev, f, *args, stream=stream)
     rc = f(*args, torch._C._cuda_getCurrentRawStream(dev) if stream is None else stream.cuda_stream)
@@ -743,29 +744,34 @@ def block_norm_int8(x, post=None, gate=None, residual=None, pre=None, eps=1e-6, 
     stride apart (expanded: one for all), post [K] or [group], pre [K], y (optional): a buffer that receives y itself. codes False: no
     q and scale. Returns (q, scale, residual_out or None); residual_out may be the residual."""
     act, dtype, dev = act_of(x), x.dtype, x.get_device()
-    if x.dim() != 2 or x.stride(1) != 1:
-        _refuse("x must be [M, K] with dense rows and is", tuple(x.shape), x.stride())
-    M, K = shape = x.shape
+    shape, xt = x.shape, x.stride()
+    if len(shape) != 2 or xt[1] != 1:
+        _refuse("x must be [M, K] with dense rows and is", tuple(shape), xt)
+    M, K = shape
     _together(dev, (post, gate, residual, pre, residual_out, y, q, scale))
-    post_len = 0
+    post_len, ldg = 0, 0
     if post is not None:
-        post_len = post.numel()
-        _is("post", post, dtype, (group if group is not None and post_len == group else K,))
-    if gate is not None and (gate.dtype != dtype or gate.shape != shape or gate.stride(1) != 1):
-        _refuse("gate must be", dtype, tuple(shape), "with dense rows and is", gate.dtype, tuple(gate.shape), gate.stride())
+        post_len = post.shape[0]
+        if post.dtype is not dtype or post.dim() != 1 or post_len != K and post_len != group or not post.is_contiguous():
+            _is("post", post, dtype, (K,))
+    if gate is not None:
+        ldg, g1 = gate.stride() if gate.dim() == 2 else (0, 0)
+        if gate.dtype is not dtype or gate.shape != shape or g1 != 1:
+            _refuse("gate must be", dtype, tuple(shape), "with dense rows and is", gate.dtype, tuple(gate.shape), gate.stride())
     if gate_act not in GATES:
         _refuse("gate_act is", repr(gate_act), "and not one of", list(GATES))
-    if pre is not None:
+    if pre is not None and (pre.dtype is not dtype or pre.shape != (K,) or not pre.is_contiguous()):
         _is("pre", pre, dtype, (K,))
     if residual is not None:
-        _is("residual", residual, dtype, shape)
+        if residual.dtype is not dtype or residual.shape != shape or not residual.is_contiguous():
+            _is("residual", residual, dtype, shape)
         if residual_out is None:
             residual_out = _empty_like(residual, stream)
-        else:
+        elif residual_out.dtype is not dtype or residual_out.shape != shape or not residual_out.is_contiguous():
             _is("residual_out", residual_out, dtype, shape)
     elif residual_out is not None:
         _refuse("residual_out without a residual")
-    if y is not None:
+    if y is not None and (y.dtype is not dtype or y.shape != shape or not y.is_contiguous()):
         _is("y", y, dtype, shape)
     if not codes:
         if q is not None or scale is not None:
@@ -780,8 +786,8 @@ def block_norm_int8(x, post=None, gate=None, residual=None, pre=None, eps=1e-6, 
         else:
             _is("scale", scale, torch.float32, (M,))
     a = lambda t: 0 if t is None else t.data_ptr()
-    n = _NORM(x.data_ptr(), a(post), a(gate), a(residual), a(pre), a(residual_out), a(y), a(q), a(scale), x.stride(0) if M > 1 else K,
-              0 if gate is None else gate.stride(0) if M > 1 else K, group or 0, post_len, GATES[gate_act], eps, w_add, residual_scale,
+    n = _NORM(x.data_ptr(), a(post), a(gate), a(residual), a(pre), a(residual_out), a(y), a(q), a(scale), xt[0] if M > 1 else K,
+              ldg if M > 1 else K, group or 0, post_len, GATES[gate_act], eps, w_add, residual_scale,
               branch_scale)
     _run(dev, lib().sx_block_norm_int8, n, M, K, act, stream=stream)
     return q, scale, residual_out
@@ -830,43 +836,64 @@ def linear_int8(x, x_scale, w, out_act=ACT_BF16, y=None, stream=None):
 _DELTA = struct.Struct("@Pqqq Pqqq Pqqq PP qq PPPPP qqqqqqqq iif4x".replace(" ", "")).pack
 
 
-def _rows_of(name, t, heads, dim):
-    """A BF16 tensor [T, heads, dim]'s data pointer and strides (token, head, none) as _DELTA takes them."""
-    if t.dtype != torch.bfloat16 or t.dim() != 3 or t.shape[1:] != (heads, dim) or t.stride(2) != 1:
-        _refuse(name, f"must be BF16 [tokens, {heads}, {dim}] with dense rows and is", t.dtype, tuple(t.shape), t.stride())
-    return t.data_ptr(), t.stride(0), t.stride(1), 0
+_BF16, _F32, _I32 = torch.bfloat16, torch.float32, torch.int32
 
 
-def _delta(q, k, v, a, b, state, starts, slots, A_log, dt_bias, normalize, scale):
-    """The sx_delta of these tensors, and (T, Hk, Hv, Dk, Dv, batch)."""
+def _delta_refuse(q, k, v, a, b, state, starts, slots, A_log, dt_bias):
+    """What of these tensors is not as _delta needs it."""
     if q.dim() != 3 or v.dim() != 3:
         _refuse("q, k and v are [tokens, heads, dim]")
     (T, Hk, Dk), (Hv, Dv) = q.shape, v.shape[1:]
-    if k.shape[0] != T or v.shape[0] != T:
+    if k.shape != q.shape or v.shape[0] != T:
         _refuse("q", tuple(q.shape), "k", tuple(k.shape), "v", tuple(v.shape))
+    for name, t in (("q", q), ("k", k), ("v", v)):
+        if t.dtype != _BF16 or t.stride(2) != 1:
+            _refuse(name, "must be BF16 [tokens, heads, dim] with dense rows and is", t.dtype, tuple(t.shape), t.stride())
     for name, t in (("a", a), ("b", b)):
-        if t.shape != (T, Hv) or t.stride(1) != 1 and Hv > 1 or t.dtype != a.dtype:
+        if t.shape != (T, Hv) or t.stride(1) != 1 or t.dtype != a.dtype:
             _refuse(name, f"must be [{T}, {Hv}] with dense rows, a and b of one type, and is", t.dtype, tuple(t.shape), t.stride())
-    if state.dtype != torch.float32 or state.dim() != 4 or state.shape[1:] != (Hv, Dk, Dv) or state.stride()[1:] != (Dk * Dv, Dv, 1):
+    if state.dtype != _F32 or state.dim() != 4 or state.shape[1:] != (Hv, Dk, Dv) or state.stride()[1:] != (Dk * Dv, Dv, 1):
         _refuse(f"state must be FP32 [states, {Hv}, {Dk}, {Dv}], each dense, and is", state.dtype, tuple(state.shape), state.stride())
     if starts.dim() != 1 or starts.numel() < 2:
         _refuse("starts must be [batch + 1] and is", tuple(starts.shape))
     B = starts.numel() - 1
-    _is("starts", starts, torch.int32, (B + 1,))
+    _is("starts", starts, _I32, (B + 1,))
     if slots is not None:
-        _is("slots", slots, torch.int32, (B,))
+        _is("slots", slots, _I32, (B,))
     if A_log is not None:
-        _is("A_log", A_log, torch.float32, (Hv,))
+        _is("A_log", A_log, _F32, (Hv,))
     if dt_bias is not None:
-        _is("dt_bias", dt_bias, torch.float32, (Hv,))
-    one = Hv * Dk * Dv
-    d = _DELTA(*_rows_of("q", q, Hk, Dk), *_rows_of("k", k, Hk, Dk), *_rows_of("v", v, Hv, Dv), a.data_ptr(), b.data_ptr(),
-               a.stride(0) if T > 1 else Hv, b.stride(0) if T > 1 else Hv, _a(A_log) or 0, _a(dt_bias) or 0, state.data_ptr(),
-               _a(slots) or 0, starts.data_ptr(), T, Hk, Hv, Dk, Dv, state.shape[0],
-               state.stride(0) if state.shape[0] > 1 else one, B, act_of(a), int(normalize), Dk ** -0.5 if scale is None else scale)
+        _is("dt_bias", dt_bias, _F32, (Hv,))
+
+
+def _delta(q, k, v, a, b, state, starts, slots, A_log, dt_bias, normalize, scale):
+    """The sx_delta of these tensors, and (T, Hk, Hv, Dk, Dv, batch). All is looked at in one expression; what is wrong is found out
+    only where something is (half of the host time)."""
+    qs, vs, ss = q.shape, v.shape, state.shape
+    if len(qs) != 3 or len(vs) != 3 or len(ss) != 4 or a.dim() != 2 or b.dim() != 2 or starts.dim() != 1:
+        _delta_refuse(q, k, v, a, b, state, starts, slots, A_log, dt_bias)
+        _refuse("a and b are [tokens, heads]")
+    T, Hk, Dk = qs
+    Tv, Hv, Dv = vs
+    (qt, qh, q1), (kt, kh, k1), (vt, vh, v1) = q.stride(), k.stride(), v.stride()
+    (at, a1), (bt, b1), (st, s1, s2, s3), (n, heads, dk, dv) = a.stride(), b.stride(), state.stride(), ss
+    B, dtype, g = starts.shape[0] - 1, q.dtype, (T, Hv)
+    if (k.shape != qs or Tv != T or dtype is not _BF16 or k.dtype is not dtype or v.dtype is not dtype or q1 * k1 * v1 * a1 * b1 * s3 != 1 or
+            a.shape != g or b.shape != g or b.dtype is not a.dtype or state.dtype is not _F32 or heads != Hv or dk != Dk or dv != Dv or
+            s1 != Dk * Dv or s2 != Dv or B < 1 or starts.dtype is not _I32 or not starts.is_contiguous() or
+            slots is not None and (slots.dtype is not _I32 or slots.shape != (B,) or not slots.is_contiguous()) or
+            A_log is not None and (A_log.dtype is not _F32 or A_log.shape != (Hv,) or not A_log.is_contiguous()) or
+            dt_bias is not None and (dt_bias.dtype is not _F32 or dt_bias.shape != (Hv,) or not dt_bias.is_contiguous())):
+        _delta_refuse(q, k, v, a, b, state, starts, slots, A_log, dt_bias)
+    d = _DELTA(q.data_ptr(), qt, qh, 0, k.data_ptr(), kt, kh, 0, v.data_ptr(), vt, vh, 0, a.data_ptr(), b.data_ptr(),
+               at if T > 1 else Hv, bt if T > 1 else Hv, 0 if A_log is None else A_log.data_ptr(),
+               0 if dt_bias is None else dt_bias.data_ptr(), state.data_ptr(), 0 if slots is None else slots.data_ptr(),
+               starts.data_ptr(), T, Hk, Hv, Dk, Dv, n, st if n > 1 else Hv * Dk * Dv, B, act_of(a), normalize,
+               Dk ** -0.5 if scale is None else scale)
     return d, (T, Hk, Hv, Dk, Dv, B)
 
 
+@functools.lru_cache(256)
 def gated_delta_workspace_bytes(T, B, Hk, Hv, Dk, max_len):
     n = ctypes.c_size_t()
     check(lib().sx_gated_delta_workspace_bytes(T, B, Hk, Hv, Dk, max_len, ctypes.byref(n)))
@@ -893,17 +920,20 @@ def gated_delta(q, k, v, a, b, state, starts, max_len, slots=None, A_log=None, d
     _together(dev, (k, v, a, b, state, starts, slots, A_log, dt_bias, out, ws, err))
     d, (T, Hk, Hv, Dk, Dv, B) = _delta(q, k, v, a, b, state, starts, slots, A_log, dt_bias, normalize, scale)
     if out is None:
-        out = _empty(q, (T, Hv, Dv), torch.bfloat16, stream)
+        out = _empty(q, (T, Hv, Dv), _BF16, stream)
+        o = _ROWS(out.data_ptr(), Hv * Dv, Dv, 0)
     elif out.dim() != 3 or out.shape[0] != T:
         _refuse("out is", tuple(out.shape))
+    else:
+        o = _head_rows("out", out, Hv, Dv)
     if ws is None:
-        n = gated_delta_workspace_bytes(T, B, Hk, Hv, Dk, max_len)
+        n = 0 if max_len <= 16 else gated_delta_workspace_bytes(T, B, Hk, Hv, Dk, max_len)  # steps need none
         ws = _empty(q, ((n + 7) // 8,), torch.int64, stream) if n else None
     elif not ws.is_contiguous():
         _refuse("ws must be contiguous and has strides", ws.stride())
     _is_err(err)
-    _run(dev, lib().sx_gated_delta, d, max_len, _head_rows("out", out, Hv, Dv), _a(ws), 0 if ws is None else ws.numel() * ws.element_size(),
-         _a(err), stream=stream)
+    _run(dev, lib().sx_gated_delta, d, max_len, o, _a(ws), 0 if ws is None else ws.numel() * ws.element_size(), _a(err),
+         stream=stream)
     return out, err
 
 
@@ -918,9 +948,12 @@ def gated_delta_verify(q, k, v, a, b, state, starts, mask, max_new, slots=None, 
     if mask.dtype != torch.int64 or mask.dim() != 2 or mask.shape[0] != T or mask.shape[1] < 1:
         _refuse("mask must be int64 [T, 1] and is", mask.dtype, tuple(mask.shape))
     if out is None:
-        out = _empty(q, (T, Hv, Dv), torch.bfloat16, stream)
+        out = _empty(q, (T, Hv, Dv), _BF16, stream)
+        o = _ROWS(out.data_ptr(), Hv * Dv, Dv, 0)
     elif out.dim() != 3 or out.shape[0] != T:
         _refuse("out is", tuple(out.shape))
+    else:
+        o = _head_rows("out", out, Hv, Dv)
     if u is None:
         u = _empty(q, (T, Hv, Dv), torch.float32, stream)
     else:
@@ -930,7 +963,7 @@ def gated_delta_verify(q, k, v, a, b, state, starts, mask, max_new, slots=None, 
     else:
         _is("decay", decay, torch.float32, (T, Hv))
     _is_err(err)
-    _run(dev, lib().sx_gated_delta_verify, d, max_new, mask.data_ptr(), mask.stride(0) if T > 1 else 1, _head_rows("out", out, Hv, Dv),
+    _run(dev, lib().sx_gated_delta_verify, d, max_new, mask.data_ptr(), mask.stride(0) if T > 1 else 1, o,
          u.data_ptr(), decay.data_ptr(), _a(err), stream=stream)
     return out, u, decay, err
 
@@ -940,44 +973,45 @@ def gated_delta_commit(k, u, decay, state, starts, count, path=None, max_count=N
     of the sequence (int32 [B, at most]; None: i) the i-th of them. k [T, Hk, Dk], u and decay as the verify had and gave them; all
     layers in one launch with k [layers, T, Hk, Dk], u [layers, T, Hv, Dv], decay [layers, T, Hv], state [layers, states, Hv, Dk,
     Dv]. Without a path max_count bounds the counts. Returns err. A sequence that cannot be committed as asked keeps its states."""
-    dev, layered = k.get_device(), k.dim() == 4
+    dev, ks, us, ss = k.get_device(), k.shape, u.shape, state.shape
+    layered = len(ks) == 4
     _together(dev, (u, decay, state, starts, count, path, slots, err))
-    if k.dim() not in (3, 4) or u.dim() != k.dim() or k.dtype != torch.bfloat16 or k.stride(-1) != 1 or u.shape[:-2] != k.shape[:-2]:
-        _refuse("k must be BF16 [tokens, heads, dim] with dense rows, with or without layers as u is:", k.dtype, tuple(k.shape), k.stride(), tuple(u.shape))
-    T, Hk, Dk = k.shape[-3:]
-    Hv, Dv = u.shape[-2:]
-    layers = k.shape[0] if layered else 1
-    _is("u", u, torch.float32, u.shape)
-    _is("decay", decay, torch.float32, u.shape[:-1])
-    if (state.dtype != torch.float32 or state.dim() != 4 + layered or state.shape[-3:] != (Hv, Dk, Dv) or
-            state.stride()[-3:] != (Dk * Dv, Dv, 1) or layered and state.shape[0] != layers):
-        _refuse(f"state must be FP32 [{'layers, ' if layered else ''}states, {Hv}, {Dk}, {Dv}], each dense, and is", state.dtype, tuple(state.shape), state.stride())
-    B = starts.numel() - 1
-    _is("starts", starts, torch.int32, (B + 1,))
-    _is("count", count, torch.int32, (B,))
-    if slots is not None:
-        _is("slots", slots, torch.int32, (B,))
+    if len(ks) not in (3, 4) or len(us) != len(ks) or len(ss) != 4 + layered or starts.dim() != 1:
+        _refuse("k, u and state are", tuple(ks), tuple(us), tuple(ss), "and not of one number of layers")
+    T, Hk, Dk = ks[-3:] if layered else ks
+    Tu, Hv, Dv = us[-3:] if layered else us
+    layers, B, st, kt = ks[0] if layered else 1, starts.shape[0] - 1, state.stride(), k.stride()
+    if (k.dtype is not _BF16 or kt[-1] != 1 or Tu != T or u.dtype is not _F32 or not u.is_contiguous() or layered and (us[0] != layers or ss[0] != layers)):
+        _refuse("k must be BF16 [tokens, heads, dim] with dense rows and u FP32, contiguous, of its layers and tokens:", k.dtype, tuple(ks), kt, u.dtype, tuple(us), u.stride())
+    if decay.dtype is not _F32 or decay.shape != us[:-1] or not decay.is_contiguous():
+        _is("decay", decay, _F32, us[:-1])
+    if state.dtype is not _F32 or ss[-3] != Hv or ss[-2] != Dk or ss[-1] != Dv or st[-3] != Dk * Dv or st[-2] != Dv or st[-1] != 1:
+        _refuse(f"state must be FP32 [{'layers, ' if layered else ''}states, {Hv}, {Dk}, {Dv}], each dense, and is", state.dtype, tuple(ss), st)
+    if (B < 1 or starts.dtype is not _I32 or count.dtype is not _I32 or count.shape != (B,) or not (starts.is_contiguous() and count.is_contiguous()) or
+            slots is not None and (slots.dtype is not _I32 or slots.shape != (B,) or not slots.is_contiguous())):
+        _is("starts", starts, _I32, (B + 1,)), _is("count", count, _I32, (B,)), slots is not None and _is("slots", slots, _I32, (B,))
     ld = 0
     if path is not None:
-        if path.dtype != torch.int32 or path.dim() != 2 or path.shape[0] != B or path.stride(1) != 1:
+        if path.dtype is not _I32 or path.dim() != 2 or path.shape[0] != B or path.stride(1) != 1:
             _refuse("path must be int32 [batch, most tokens kept] with dense rows")
-        max_count = path.shape[1] if max_count is None else max_count
-        ld = path.stride(0) if B > 1 else path.shape[1]
-        if max_count > path.shape[1]:
-            _refuse("max_count =", max_count, "is over the path's", path.shape[1])
+        most = path.shape[1]
+        max_count = most if max_count is None else max_count
+        ld = path.stride(0) if B > 1 else most
+        if max_count > most:
+            _refuse("max_count =", max_count, "is over the path's", most)
     elif max_count is None:
         _refuse("max_count is needed without a path")
     _is_err(err)
-    states, one = state.shape[-4], Hv * Dk * Dv
-    _run(dev, lib().sx_gated_delta_commit, _ROWS(k.data_ptr(), k.stride(-3), k.stride(-2), k.stride(0) if layered else 0), u.data_ptr(),
-         decay.data_ptr(), layers, T, Hk, Hv, Dk, Dv, state.data_ptr(), state.stride(0) if layered else 0,
-         state.stride(-4) if states > 1 else one, states, _a(slots), starts.data_ptr(), B, count.data_ptr(), max_count, _a(path), ld,
+    states, one = ss[-4], Hv * Dk * Dv
+    _run(dev, lib().sx_gated_delta_commit, _ROWS(k.data_ptr(), kt[-3], kt[-2], kt[0] if layered else 0), u.data_ptr(),
+         decay.data_ptr(), layers, T, Hk, Hv, Dk, Dv, state.data_ptr(), st[0] if layered else 0, st[-4] if states > 1 else one, states, _a(slots), starts.data_ptr(), B, count.data_ptr(), max_count, _a(path), ld,
          _a(err), stream=stream)
     return err
 
 
 # ---------------- acceptance by the target's probabilities ----------------
 
+@functools.lru_cache(256)
 def mtp_accept_sampled_workspace_bytes(T, B, n_valid, n_draft):
     n = ctypes.c_size_t()
     check(lib().sx_mtp_accept_sampled_workspace_bytes(T, B, n_valid, n_draft, ctypes.byref(n)))
@@ -993,40 +1027,41 @@ def mtp_accept_sampled(logits, drafts, starts, u, temperature, max_rows, draft_l
     token from max(p - q, 0), and behind the last comes one from p, both by u[t, 1]. u FP64 [T, 2] in [0, 1). temperature 0: the
     largest logits. Returns (tokens int32 [B, max_rows]: what is committed, then -1; count int32 [B], as kv_append and
     gated_delta_commit take it; status int32 [B]: 0, 1 + the row that has no distribution or draft, -1 impossible starts)."""
-    dev, act = logits.get_device(), act_of(logits)
-    if logits.dim() != 2 or logits.stride(1) != 1:
-        _refuse("logits must be [T, vocabulary] with dense rows and are", tuple(logits.shape), logits.stride())
-    T, n_valid, n_draft, dld = logits.shape[0], logits.shape[1] if n_valid is None else n_valid, 0, 0
+    dev, act, shape, lt = logits.get_device(), act_of(logits), logits.shape, logits.stride()
+    if len(shape) != 2 or lt[1] != 1 or starts.dim() != 1:
+        _refuse("logits must be [T, vocabulary] with dense rows and are", tuple(shape), lt, "starts [B + 1]:", tuple(starts.shape))
+    T, width = shape
+    n_valid, n_draft, dld, B = width if n_valid is None else n_valid, 0, 0, starts.shape[0] - 1
     _together(dev, (drafts, starts, u, temperature, draft_logits, tokens, count, status, ws))
-    if n_valid > logits.shape[1]:
-        _refuse("n_valid =", n_valid, "is over the logits'", logits.shape[1])
-    B = starts.numel() - 1
-    _is("drafts", drafts, torch.int32, (T,))
-    _is("starts", starts, torch.int32, (B + 1,))
-    _is("u", u, torch.float64, (T, 2))
-    _is("temperature", temperature, torch.float32, (B,))
+    if n_valid > width:
+        _refuse("n_valid =", n_valid, "is over the logits'", width)
+    if (drafts.dtype is not _I32 or drafts.shape != (T,) or starts.dtype is not _I32 or u.dtype is not torch.float64 or u.shape != (T, 2) or
+            temperature.dtype is not _F32 or temperature.shape != (B,) or
+            not (drafts.is_contiguous() and starts.is_contiguous() and u.is_contiguous() and temperature.is_contiguous())):
+        _is("drafts", drafts, _I32, (T,)), _is("starts", starts, _I32, (B + 1,)), _is("u", u, torch.float64, (T, 2))
+        _is("temperature", temperature, _F32, (B,))
     if draft_logits is not None:
-        if draft_logits.dtype != logits.dtype or draft_logits.dim() != 2 or draft_logits.shape[0] != T or draft_logits.stride(1) != 1:
+        if draft_logits.dtype is not logits.dtype or draft_logits.dim() != 2 or draft_logits.shape[0] != T or draft_logits.stride(1) != 1:
             _refuse("draft_logits must be", logits.dtype, f"[{T}, vocabulary] with dense rows and are", draft_logits.dtype, tuple(draft_logits.shape))
         n_draft = draft_logits.shape[1]
         dld = draft_logits.stride(0) if T > 1 else n_draft
     if tokens is None:
-        tokens = _empty(drafts, (B, max_rows), torch.int32, stream)
+        tokens = _empty(drafts, (B, max_rows), _I32, stream)
     else:
-        _is("tokens", tokens, torch.int32, (B, max_rows))
+        _is("tokens", tokens, _I32, (B, max_rows))
     if count is None:
-        count = _empty(drafts, (B,), torch.int32, stream)
+        count = _empty(drafts, (B,), _I32, stream)
     else:
-        _is("count", count, torch.int32, (B,))
+        _is("count", count, _I32, (B,))
     if status is None:
-        status = _empty(drafts, (B,), torch.int32, stream)
+        status = _empty(drafts, (B,), _I32, stream)
     else:
-        _is("status", status, torch.int32, (B,))
+        _is("status", status, _I32, (B,))
     if ws is None:
         ws = _empty(drafts, ((mtp_accept_sampled_workspace_bytes(T, B, n_valid, n_draft) + 7) // 8,), torch.int64, stream)
     elif not ws.is_contiguous():
         _refuse("ws must be contiguous and has strides", ws.stride())
-    _run(dev, lib().sx_mtp_accept_sampled, logits.data_ptr(), logits.stride(0) if T > 1 else logits.shape[1], T, n_valid,
+    _run(dev, lib().sx_mtp_accept_sampled, logits.data_ptr(), lt[0] if T > 1 else width, T, n_valid,
          _a(draft_logits), dld, n_draft, act, drafts.data_ptr(), starts.data_ptr(), B, max_rows, u.data_ptr(), temperature.data_ptr(),
          tokens.data_ptr(), count.data_ptr(), status.data_ptr(), ws.data_ptr(), ws.numel() * ws.element_size(), stream=stream)
     return tokens, count, status
