@@ -5,9 +5,11 @@
 //   y = r / sqrt(mean(r^2) + eps) * (pre + w_add)       (pre null: y = r)
 // and y as int8 codes with one FP32 scale a row, amax(|y|) / 127: the form sx_linear_int8 takes its activations in.
 //
-// A row is read once into registers (8 features a 16-byte load) and written from there. A code is a whole number, and in FP32 one
-// in some tens of thousands of values lies too near a border to tell its side; so what a code depends on is computed in FP64,
-// which runs at FP32's rate here. The second norm's root cancels in the codes: they come from t = r (pre + w_add) alone.
+// A row is read once into registers (8 features a 16-byte load) and written from there. A code is a whole number that a border
+// decides, so it has to be that of the exact value: all is computed in FP64, which runs at FP32's rate here. The second norm's root
+// cancels in the codes, which come from t = r (pre + w_add) alone. The VALU's work bounds it where there is a gate (2048 rows of 4096, heads
+// of 128: 700 instructions a wave). In FP32 with a bound on what that is off, and FP64 for what the bound leaves open (one code in
+// two thousand, the row's largest value), it was as slow: 820 instructions.
 #include "common.hpp"
 
 #include <cmath>
@@ -16,6 +18,7 @@ namespace sx {
 namespace {
 
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
 
 struct Args {
     const void *x, *post, *gate, *residual, *pre;
@@ -26,6 +29,7 @@ struct Args {
     int32_t K, group, post_wrap;  // group: 0, the row; post_wrap: post has that many values
     int32_t gate_act;
     float eps, w_add, rs, bs;
+    double over_k, over_group;
 };
 
 __device__ __forceinline__ void load8(const float *p, float (&v)[8]) {
@@ -44,22 +48,77 @@ __device__ __forceinline__ void store8(float *p, const float (&v)[8]) {
 __device__ __forceinline__ void store8(uint16_t *p, const float (&v)[8]) {
     u32x4 u;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) u[i] = f32_to_bf16(v[2 * i]) | (f32_to_bf16(v[2 * i + 1]) << 16);
+    for (int i = 0; i < 4; ++i) u[i] = __builtin_bit_cast(uint32_t, bf16x2{(__bf16)v[2 * i], (__bf16)v[2 * i + 1]});
     *reinterpret_cast<u32x4 *>(p) = u;
+}
+
+// 1 / (1 + e^-z) of eight values in FP64: e^-|z| as 2^n times the power series of e^r, |r| <= ln(2) / 2, to the eleventh power (6e-15 is
+// left), the reciprocal by a Newton step (the instruction's
+// is good to 2^-24). The coefficients are held in scalar registers: as literals each took two moves a value.
+__device__ __forceinline__ double held(double c) {
+    asm("" : "+s"(c));
+    return c;
+}
+__device__ __forceinline__ void sigmoid8(const float (&z)[8], double (&s)[8]) {
+    const double c[12] = {1.0, 1.0, 0.5, held(1.0 / 6.0), held(1.0 / 24.0), held(1.0 / 120.0), held(1.0 / 720.0), held(1.0 / 5040.0), held(1.0 / 40320.0),
+                          held(1.0 / 362880.0), held(1.0 / 3628800.0), held(1.0 / 39916800.0)};
+    const double log2e = held(1.4426950408889634), ln2 = held(-0.6931467056274414), rest = held(-4.7493250390316726e-07);  // 21 bits, whose multiples are exact, and the rest
+    const double least = held(-800.0);  // e^-800 is 0
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+        const double y = fmax(-fabs((double)z[k]), least), n = rint(y * log2e), r = fma(n, rest, fma(n, ln2, y));
+        double p = fma(c[11], r, c[10]);
+#pragma unroll
+        for (int i = 9; i >= 0; --i) p = fma(p, r, c[i]);
+        const double e = ldexp(p, (int)n), d = 1.0 + e;
+        double q = __builtin_amdgcn_rcp(d);
+        q = fma(fma(-d, q, 1.0), q, q);
+        s[k] = z[k] < 0.f ? e * q : q;
+    }
+}
+
+// 1 / sqrt(x): the instruction's 2^-24 and two Newton steps (x zero: infinity; no number: none).
+__device__ __forceinline__ double over_root(double x) {
+    double q = __builtin_amdgcn_rsq(x);
+    if (!(q < INFINITY) || q == 0.0) return q;
+    const double half = -0.5 * x;
+    q = fma(fma(half * q, q, 0.5), q, q);
+    return fma(fma(half * q, q, 0.5), q, q);
 }
 
 struct Sum {
     __device__ static double of(double a, double b) { return a + b; }
 };
-struct Top {  // of non-negative values, a NaN the largest
-    __device__ static double of(double a, double b) { return __double_as_longlong(a) > __double_as_longlong(b) ? a : b; }
+struct Top {
+    __device__ static double of(double a, double b) { return a > b ? a : b; }
 };
+
+// A lane's value of the same row of 16: neighbours (0xB1), pairs (0x4E), halves and the row mirrored (0x141, 0x140).
+template <int CTRL>
+__device__ __forceinline__ double across(double v) {
+    const uint64_t u = (uint64_t)__double_as_longlong(v);
+    const uint32_t lo = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)u, CTRL, 0xF, 0xF, false);
+    const uint32_t hi = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)(u >> 32), CTRL, 0xF, 0xF, false);
+    return __longlong_as_double((long long)((uint64_t)hi << 32 | lo));
+}
+
+// Over the group / 8 lanes that hold a run of `group` features.
+__device__ __forceinline__ double group_sum(double v, int group) {
+    if (group > 8) v += across<0xB1>(v);
+    if (group > 16) v += across<0x4E>(v);
+    if (group > 32) v += across<0x141>(v);
+    if (group > 64) v += across<0x140>(v);
+    if (group > 128) v += __shfl_xor(v, 16);
+    if (group > 256) v += __shfl_xor(v, 32);
+    return v;
+}
 
 // Over the TPR threads of a row, in all of them. Every thread of the block calls it.
 template <typename Op, int TPR>
 __device__ __forceinline__ double row_reduce(double v, double *part) {
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) v = Op::of(v, __shfl_xor(v, d));
+    v = Op::of(v, across<0xB1>(v)), v = Op::of(v, across<0x4E>(v));
+    v = Op::of(v, across<0x141>(v)), v = Op::of(v, across<0x140>(v));
+    v = Op::of(v, __shfl_xor(v, 16)), v = Op::of(v, __shfl_xor(v, 32));
     if constexpr (TPR > 64) {
         const int wave = threadIdx.x >> 6, first = wave / (TPR / 64) * (TPR / 64);
         if ((threadIdx.x & 63) == 0) part[wave] = v;
@@ -99,7 +158,7 @@ __global__ void __launch_bounds__(TPR < 256 ? 256 : TPR) block_norm_kernel(const
             for (int j = 0; j < NV; ++j)
 #pragma unroll
                 for (int k = 0; k < 8; ++k) ss = fma(h[j][k], h[j][k], ss);
-            ss = 1.0 / sqrt(row_reduce<Sum, TPR>(ss, part[0]) / (double)a.K + (double)a.eps);
+            ss = over_root(fma(row_reduce<Sum, TPR>(ss, part[0]), a.over_k, (double)a.eps));
         }
 #pragma unroll
         for (int j = 0; j < NV; ++j) {
@@ -109,14 +168,13 @@ __global__ void __launch_bounds__(TPR < 256 ? 256 : TPR) block_norm_kernel(const
                 inv = 0.0;
 #pragma unroll
                 for (int k = 0; k < 8; ++k) inv = fma(h[j][k], h[j][k], inv);
-                for (int d = 1; d < a.group / 8; d <<= 1) inv += __shfl_xor(inv, d);
-                inv = 1.0 / sqrt(inv / (double)a.group + (double)a.eps);
+                inv = over_root(fma(group_sum(inv, a.group), a.over_group, (double)a.eps));
             }
             if (row && i < n8) {
                 float w[8];
-                load8(static_cast<const T *>(a.post) + (i * 8) % a.post_wrap, w);
+                load8(static_cast<const T *>(a.post) + (a.post_wrap == a.K ? i * 8 : i * 8 & (a.post_wrap - 1)), w);
 #pragma unroll
-                for (int k = 0; k < 8; ++k) h[j][k] = h[j][k] * inv * ((double)w[k] + (double)a.w_add);
+                for (int k = 0; k < 8; ++k) h[j][k] = h[j][k] * inv * (a.w_add == 0.f ? (double)w[k] : (double)w[k] + (double)a.w_add);
             }
         }
     }
@@ -128,21 +186,31 @@ __global__ void __launch_bounds__(TPR < 256 ? 256 : TPR) block_norm_kernel(const
                 float z[8];
                 load8(static_cast<const T *>(a.gate) + m * a.ldg + i * 8, z);
 #pragma unroll
-                for (int k = 0; k < 8; ++k) {
-                    const double g = (double)z[k];
-                    if (a.gate_act == SX_GATE_NONE) h[j][k] *= g;
-                    else h[j][k] *= (a.gate_act == SX_GATE_SILU ? g : 1.0) / (1.0 + exp(-g));
+                for (int k = 0; k < 8; ++k)
+                    if (a.gate_act != SX_GATE_SIGMOID) h[j][k] *= (double)z[k];
+                if (a.gate_act != SX_GATE_NONE) {
+                    double g[8];
+                    sigmoid8(z, g);
+#pragma unroll
+                    for (int k = 0; k < 8; ++k) h[j][k] *= g[k];
+                    if (a.gate_act == SX_GATE_SIGMOID) {
+#pragma unroll
+                        for (int k = 0; k < 8; ++k) h[j][k] = z[k] == z[k] ? h[j][k] : (double)z[k];
+                    }
                 }
             }
         }
     }
     double s2 = 0.0, top = 0.0;
+    double odd = 0.0;  // no number where something is none, or too large for one
 #pragma unroll
     for (int j = 0; j < NV; ++j) {
         const int i = tid + j * TPR;
         const bool on = row && i < n8;
+        if (a.bs != 1.f) {
 #pragma unroll
-        for (int k = 0; k < 8; ++k) h[j][k] *= (double)a.bs;
+            for (int k = 0; k < 8; ++k) h[j][k] *= (double)a.bs;
+        }
         if (on && a.residual != nullptr) {
             float v[8];
             load8(static_cast<const T *>(a.residual) + m * a.K + i * 8, v);
@@ -162,11 +230,11 @@ __global__ void __launch_bounds__(TPR < 256 ? 256 : TPR) block_norm_kernel(const
             }
         }
 #pragma unroll
-        for (int k = 0; k < 8; ++k) top = Top::of(top, fabs(h[j][k]));
+        for (int k = 0; k < 8; ++k) top = fmax(top, fabs(h[j][k])), odd = fma(h[j][k], 0.0, odd);
     }
     double inv = 1.0;
-    if (a.pre != nullptr) inv = 1.0 / sqrt(row_reduce<Sum, TPR>(s2, part[1]) / (double)a.K + (double)a.eps);
-    if (a.q != nullptr) top = row_reduce<Top, TPR>(top, part[2]);
+    if (a.pre != nullptr) inv = over_root(fma(row_reduce<Sum, TPR>(s2, part[1]), a.over_k, (double)a.eps));
+    if (a.q != nullptr) top = row_reduce<Top, TPR>(odd == 0.0 ? top : INFINITY, part[2]);
     const bool fine = top < INFINITY;
     const double mul = 127.0 / top;
 #pragma unroll
@@ -176,18 +244,29 @@ __global__ void __launch_bounds__(TPR < 256 ? 256 : TPR) block_norm_kernel(const
         if (a.y != nullptr) {
             float v[8];
 #pragma unroll
-            for (int k = 0; k < 8; ++k) v[k] = (float)(h[j][k] * inv);
+            for (int k = 0; k < 8; ++k) v[k] = (float)(a.pre != nullptr ? h[j][k] * inv : h[j][k]);
             store8(static_cast<T *>(a.y) + m * a.K + i * 8, v);
         }
         if (a.q == nullptr) continue;
         uint32_t o[2] = {0u, 0u};
         if (fine && top > 0.0) {
+            double n[8];
+            double far = 0.0;
 #pragma unroll
             for (int k = 0; k < 8; ++k) {
-                double c = h[j][k] * mul;
-                // beside a border the quotient itself says which side, and a tie that it is one
-                if (fabs(fabs(c - rint(c)) - 0.5) < 1e-9) c = h[j][k] * 127.0 / top;
-                o[k / 4] |= ((uint32_t)(int)rint(c) & 0xFFu) << (8 * (k & 3));
+                const double c = h[j][k] * mul;
+                n[k] = rint(c);
+                far = fmax(far, fabs(c - n[k]));
+            }
+            if (far > 0.5 - 1e-9) {  // beside a border the quotient itself says which side, and a tie that it is one
+#pragma unroll
+                for (int k = 0; k < 8; ++k) n[k] = rint(h[j][k] * 127.0 / top);
+            }
+#pragma unroll
+            for (int k = 0; k < 8; k += 4) {
+                const uint32_t lo = __builtin_amdgcn_perm((uint32_t)(int)n[k + 1], (uint32_t)(int)n[k], 0x0C0C0400);
+                const uint32_t hi = __builtin_amdgcn_perm((uint32_t)(int)n[k + 3], (uint32_t)(int)n[k + 2], 0x04000C0C);
+                o[k / 4] = lo | hi;
             }
         }
         *reinterpret_cast<uint2 *>(a.q + m * a.K + i * 8) = uint2{o[0], o[1]};
@@ -254,7 +333,8 @@ extern "C" int sx_block_norm_int8(const sx_block_norm *p, int64_t M, int64_t K, 
         for (int k = 0; k < o; ++k) SX_CHECK(outs[k].p == nullptr || apart(outs[k].p, outs[k].n, outs[o].p, outs[o].n), "outputs ", k, " and ", o, " overlap");
     }
     const Args a{n.x, n.post, n.gate, n.residual, n.pre, n.residual_out, n.y, n.q, n.scale, M, n.ldx, n.ld_gate, (int32_t)K, (int32_t)(g == K ? 0 : g),
-                 (int32_t)(n.post_len != 0 ? n.post_len : K), n.gate_act, n.eps, n.w_add, n.residual_scale, n.branch_scale};
+                 (int32_t)(n.post_len != 0 ? n.post_len : K), n.gate_act, n.eps, n.w_add, n.residual_scale, n.branch_scale,
+                 1.0 / (double)K, g == 0 ? 0.0 : 1.0 / (double)g};
     if (act == SX_ACT_F32) launch<float>(a, stream_of(stream));
     else launch<uint16_t>(a, stream_of(stream));
     SX_LAUNCHED("block_norm_int8 M=", M, " K=", K);
