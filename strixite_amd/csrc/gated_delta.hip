@@ -110,6 +110,16 @@ __global__ void __launch_bounds__(256) delta_step_kernel(const Args a) {
 
 // ---------------- verify ----------------
 
+// Over the C neighbouring lanes (8 or 16) that hold a row.
+template <int C>
+__device__ __forceinline__ float sum_chunks(float x) {
+    x += __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(x), 0xB1, 0xF, 0xF, false));
+    x += __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(x), 0x4E, 0xF, 0xF, false));
+    x += __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(x), 0x141, 0xF, 0xF, false));
+    if constexpr (C == 16) x += __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(x), 0x140, 0xF, 0xF, false));
+    return x;
+}
+
 constexpr int kMaxNew = 64;
 
 struct VerifyArgs {
@@ -119,13 +129,14 @@ struct VerifyArgs {
     float *u, *decay;
 };
 
-// NT tiles of 16 tokens, W waves of 16 columns each that share the products of keys and queries through LDS. All operand
-// orders are natural: a lane (n16, g) of a 32-deep product has values 8 g .. 8 g + 7 of row n16, of a result column n16 and
-// rows 4 g .. 4 g + 3.
+// NT tiles of 16 tokens, W waves of 16 columns each, which share the tokens' keys and queries and their products in LDS. All operand
+// orders are natural: a lane (n16, g4) of a 32-deep product has values 8 g4 .. 8 g4 + 7 of row n16, of a result column n16 and rows
+// 4 g4 .. 4 g4 + 3. A row's 16-byte chunk c lies at c ^ row, so that 16 rows' reads spread over all banks.
 template <int DK, int NT, int W>
 __global__ void __launch_bounds__(64 * W) delta_verify_kernel(const VerifyArgs va) {
-    constexpr int N = 16 * NT, KS = DK / 32, kPitch = N + 4;
+    constexpr int N = 16 * NT, KS = DK / 32, kPitch = N + 4, kRow = DK / 8;  // chunks a row
     const Args &a = va.d;
+    __shared__ u32x4 keys[N * kRow], queries[N * kRow];
     __shared__ __attribute__((aligned(16))) float At[N * kPitch];  // [j][i]: of token j in row i's system
     __shared__ __attribute__((aligned(16))) float P[N * kPitch];   // [i][j]
     __shared__ double path[N];                                     // G
@@ -148,6 +159,21 @@ __global__ void __launch_bounds__(64 * W) delta_verify_kernel(const VerifyArgs v
         return;
     }
     // everything from memory is requested before anything is used
+    constexpr int kPieces = (N * kRow + 64 * W - 1) / (64 * W);
+    u32x4 kp[kPieces], qp[kPieces];
+#pragma unroll
+    for (int i = 0; i < kPieces; ++i) {
+        const int id = threadIdx.x + i * 64 * W;
+        const int64_t at = s.t0 + min(id / kRow, s.n - 1);
+        kp[i] = *reinterpret_cast<const u32x4 *>(a.k + at * a.k_t + hk * a.k_h + id % kRow * 8);
+        qp[i] = *reinterpret_cast<const u32x4 *>(a.q + at * a.q_t + hk * a.q_h + id % kRow * 8);
+    }
+    float g = 0.f, be = 0.f;
+    uint64_t word = 0;
+    if (wave == 0 && lane < s.n) {
+        gates(a, s.t0 + lane, h, g, be);
+        word = (va.mask[(s.t0 + lane) * va.mask_ld] & ((1ull << lane) - 1)) | 1ull << lane;
+    }
     float st[KS][8];
     if (on) {
         const float *state = a.state + s.slot * a.s_slot + (int64_t)h * DK * a.Dv + col;
@@ -156,59 +182,44 @@ __global__ void __launch_bounds__(64 * W) delta_verify_kernel(const VerifyArgs v
 #pragma unroll
             for (int j = 0; j < 8; ++j) st[ks][j] = state[(int64_t)(ks * 32 + g4 * 8 + j) * a.Dv];
     }
-    bf16x8 K[NT][KS], Q[NT][KS];
-#pragma unroll
-    for (int t = 0; t < NT; ++t) {
-        const int i = t * 16 + n16;
-        const int64_t at = s.t0 + min(i, s.n - 1);
-        const u32x4 none = {0u, 0u, 0u, 0u};
-#pragma unroll
-        for (int ks = 0; ks < KS; ++ks) {
-            const u32x4 kw = *reinterpret_cast<const u32x4 *>(a.k + at * a.k_t + hk * a.k_h + ks * 32 + g4 * 8);
-            const u32x4 qw = *reinterpret_cast<const u32x4 *>(a.q + at * a.q_t + hk * a.q_h + ks * 32 + g4 * 8);
-            K[t][ks] = __builtin_bit_cast(bf16x8, i < s.n ? kw : none);
-            Q[t][ks] = __builtin_bit_cast(bf16x8, i < s.n ? qw : none);
-        }
-    }
     uint16_t v[NT][4];
 #pragma unroll
     for (int t = 0; t < NT; ++t)
 #pragma unroll
         for (int r = 0; r < 4; ++r) v[t][r] = a.v[(s.t0 + min(t * 16 + g4 * 4 + r, s.n - 1)) * a.v_t + h * a.v_h + (on ? col : 0)];
-    if (wave == 0) {
-        // token `lane`: gates, its path's sum in 64 bits (differences of long paths lose bits in 32), lengths
-        float g = 0.f, be = 0.f;
-        uint64_t word = 0;
-        if (lane < s.n) {
-            gates(a, s.t0 + lane, h, g, be);
-            word = va.mask[(s.t0 + lane) * va.mask_ld] & ((1ull << lane) - 1) | 1ull << lane;
-            if (blockIdx.x == 0) va.decay[(int64_t)(s.t0 + lane) * a.Hv + h] = g;
-        }
-        double G = 0.0;
-        for (int j = 0; j < s.n; ++j) {
-            const float gj = __shfl(g, j);
-            if (word >> j & 1) G += (double)gj;
-        }
-        if (lane < N) path[lane] = G, sees[lane] = word, beta[lane] = be, grow[lane] = expf((float)G);
 #pragma unroll
-        for (int t = 0; t < NT; ++t) {
-            float kk = 0.f, qq = 0.f;
+    for (int i = 0; i < kPieces; ++i) {
+        if (threadIdx.x + i * 64 * W >= N * kRow) break;
+        const int id = threadIdx.x + i * 64 * W, row = id / kRow, c = (id % kRow) ^ (row & (kRow - 1));
+        const u32x4 none = {0u, 0u, 0u, 0u};
+        if (row >= s.n) kp[i] = none, qp[i] = none;
+        keys[row * kRow + c] = kp[i], queries[row * kRow + c] = qp[i];
+        float x[8], y[8], kk = 0.f, qq = 0.f;
+        unpack8(kp[i], x);
+        unpack8(qp[i], y);
 #pragma unroll
-            for (int ks = 0; ks < KS; ++ks) {
-                float x[8], y[8];
-                unpack8(__builtin_bit_cast(u32x4, K[t][ks]), x);
-                unpack8(__builtin_bit_cast(u32x4, Q[t][ks]), y);
-#pragma unroll
-                for (int j = 0; j < 8; ++j) kk = fmaf(x[j], x[j], kk), qq = fmaf(y[j], y[j], qq);
-            }
-            kk = sum_rows(kk), qq = sum_rows(qq);
-            if (g4 == 0) {
-                rk[t * 16 + n16] = a.normalize ? 1.f / sqrtf(kk + kNormEps) : 1.f;
-                rq[t * 16 + n16] = (a.normalize ? 1.f / sqrtf(qq + kNormEps) : 1.f) * a.scale;
-            }
+        for (int j = 0; j < 8; ++j) kk = fmaf(x[j], x[j], kk), qq = fmaf(y[j], y[j], qq);
+        kk = sum_chunks<kRow>(kk), qq = sum_chunks<kRow>(qq);
+        if (id % kRow == 0) {
+            rk[row] = a.normalize ? 1.f / sqrtf(kk + kNormEps) : 1.f;
+            rq[row] = (a.normalize ? 1.f / sqrtf(qq + kNormEps) : 1.f) * a.scale;
         }
     }
+    if (wave == 0) {
+        // token `lane`'s path, its sum in 64 bits: differences of long paths lose bits in 32
+        double G = 0.0;
+        for (int j = 0; j < s.n; ++j) {
+            const float gj = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(g), j));
+            G += word >> j & 1 ? (double)gj : 0.0;
+        }
+        if (lane < N) path[lane] = G, sees[lane] = word, beta[lane] = be, grow[lane] = expf((float)G);
+        if (blockIdx.x == 0 && lane < s.n) va.decay[(int64_t)(s.t0 + lane) * a.Hv + h] = g;
+    }
     __syncthreads();
+    auto operand = [&](const u32x4 *rows, int t, int ks) __attribute__((always_inline)) {
+        const int row = t * 16 + n16;
+        return __builtin_bit_cast(bf16x8, rows[row * kRow + ((ks * 4 + g4) ^ (row & (kRow - 1)))]);
+    };
     // Products of tokens. An unseen pair is -0.0, which no seen one is: what it would meet is left out, NaN too.
 #pragma unroll
     for (int ti = 0; ti < NT; ++ti)
@@ -218,7 +229,10 @@ __global__ void __launch_bounds__(64 * W) delta_verify_kernel(const VerifyArgs v
             f32x4 kk = {0.f, 0.f, 0.f, 0.f}, qk = kk;
             if (tj <= ti) {
 #pragma unroll
-                for (int ks = 0; ks < KS; ++ks) kk = mfma(K[ti][ks], K[tj][ks], kk), qk = mfma(Q[ti][ks], K[tj][ks], qk);
+                for (int ks = 0; ks < KS; ++ks) {
+                    const bf16x8 other = operand(keys, tj, ks);
+                    kk = mfma(operand(keys, ti, ks), other, kk), qk = mfma(operand(queries, ti, ks), other, qk);
+                }
             }
             const int j = tj * 16 + n16, i0 = ti * 16 + g4 * 4;
             const float rj = rk[j];
@@ -241,12 +255,17 @@ __global__ void __launch_bounds__(64 * W) delta_verify_kernel(const VerifyArgs v
     for (int t = 0; t < NT; ++t) X[t] = Y[t] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int ks = 0; ks < KS; ++ks) {
-        bf16x8 o[3];
+        bf16x8 o[3], K[NT], Q[NT];
+#pragma unroll
+        for (int t = 0; t < NT; ++t) K[t] = operand(keys, t, ks), Q[t] = operand(queries, t, ks);
         split(st[ks], o);
 #pragma unroll
         for (int p = 2; p >= 0; --p)
 #pragma unroll
-            for (int t = 0; t < NT; ++t) X[t] = mfma(K[t][ks], o[p], X[t]), Y[t] = mfma(Q[t][ks], o[p], Y[t]);
+            for (int t = 0; t < NT; ++t) {
+                X[t] = mfma(K[t], o[p], X[t]);
+                if (p < 2) Y[t] = mfma(Q[t], o[p], Y[t]);
+            }
     }
 #pragma unroll
     for (int t = 0; t < NT; ++t)
@@ -340,7 +359,7 @@ __global__ void __launch_bounds__(64 * W) delta_verify_kernel(const VerifyArgs v
         for (int r = 0; r < 4; ++r) {
             const int i = t * 16 + g4 * 4 + r;
             if (i >= s.n) continue;
-            a.out[(s.t0 + i) * a.o_t + h * a.o_h + col] = (uint16_t)f32_to_bf16(O[t][r]);
+            a.out[(s.t0 + i) * a.o_t + h * a.o_h + col] = __builtin_bit_cast(uint16_t, (__bf16)O[t][r]);
             va.u[((int64_t)(s.t0 + i) * a.Hv + h) * a.Dv + col] = rk[i] * U[t][r];
         }
 }
@@ -494,12 +513,8 @@ template <int DK, int NT>
 void launch_verify(const VerifyArgs &v, hipStream_t s) {
     const Args &a = v.d;
     const int64_t waves = (int64_t)a.Dv / 16 * a.Hv * a.B;
-    bool apiece = NT == 1;
-    if constexpr (NT > 1) {
-        apiece = waves <= 2 * device_cus();
-        if (!apiece) delta_verify_kernel<DK, NT, 4><<<dim3((unsigned)((a.Dv + 63) / 64), (unsigned)a.Hv, (unsigned)a.B), 256, 0, s>>>(v);
-    }
-    if (apiece) delta_verify_kernel<DK, NT, 1><<<dim3((unsigned)(a.Dv / 16), (unsigned)a.Hv, (unsigned)a.B), 64, 0, s>>>(v);
+    if (waves > 2 * device_cus()) delta_verify_kernel<DK, NT, 4><<<dim3((unsigned)((a.Dv + 63) / 64), (unsigned)a.Hv, (unsigned)a.B), 256, 0, s>>>(v);
+    else delta_verify_kernel<DK, NT, 1><<<dim3((unsigned)(a.Dv / 16), (unsigned)a.Hv, (unsigned)a.B), 64, 0, s>>>(v);
 }
 
 template <int DK>
