@@ -64,12 +64,9 @@ __global__ void __launch_bounds__(64 * kRowWaves) int8_rows_kernel(const Args a)
         for (int j = 0; j < kAhead; ++j)
 #pragma unroll
             for (int c = 0; c < 2; ++c) {
-                const int at = (b0 + j * kRowWaves) * 128 + c * 64 + g * 16, in = min(at, a.K - 16);
+                const int in = min((b0 + j * kRowWaves) * 128 + c * 64 + g * 16, a.K - 16);
 #pragma unroll
-                for (int r = 0; r < NT; ++r) {
-                    A[j][r][c] = load16(w[r] + in);
-                    if (at >= a.K) A[j][r][c] = none;
-                }
+                for (int r = 0; r < NT; ++r) A[j][r][c] = load16(w[r] + in);
             }
 #pragma unroll
         for (int j = 0; j < kAhead; ++j)
@@ -82,11 +79,13 @@ __global__ void __launch_bounds__(64 * kRowWaves) int8_rows_kernel(const Args a)
 #pragma unroll
         for (int j = 0; j < kAhead; ++j)
 #pragma unroll
-            for (int c = 0; c < 2; ++c)
+            for (int c = 0; c < 2; ++c) {
+                const bool past = (b0 + j * kRowWaves) * 128 + c * 64 + g * 16 >= a.K;  // asked here: at the loads it would wait for them
 #pragma unroll
                 for (int t = 0; t < MT; ++t)
 #pragma unroll
-                    for (int r = 0; r < NT; ++r) acc[r][t] = mfma(A[j][r][c], B[j][t][c], acc[r][t]);
+                    for (int r = 0; r < NT; ++r) acc[r][t] = mfma(past ? none : A[j][r][c], B[j][t][c], acc[r][t]);
+            }
     }
 #pragma unroll
     for (int r = 0; r < NT; ++r)
@@ -139,18 +138,22 @@ __global__ void __launch_bounds__(64 * kTileWaves) int8_tiles_kernel(const Args 
     for (int i = 0; i < kLoadX; ++i) xo[i] = (uint32_t)(min((wave * kLoadX + i) * 8 + r8, xrows - 1) * a.K);
     i32x4 rw[kLoadW], rx[kLoadX];
     const i32x4 none = {0, 0, 0, 0};
-    auto fetch = [&](int b) __attribute__((always_inline)) {  // past the end: the last block again, not used
-        const int at = min(b, a.kb - 1) * 128 + chunk, in = min(at, a.K - 16);
+    auto fetch = [&](int b) __attribute__((always_inline)) {  // past the end: the last codes again
+        const int in = min(min(b, a.kb - 1) * 128 + chunk, a.K - 16);
 #pragma unroll
         for (int i = 0; i < kLoadW; ++i) rw[i] = load16(wbase + wo[i] + in);
 #pragma unroll
         for (int i = 0; i < kLoadX; ++i) rx[i] = load16(xbase + xo[i] + in);
-        if (at >= a.K) {
+    };
+    // Block b in the registers: zeros for w past the end of K (at the loads they would wait for them).
+    auto clear_past = [&](int b) __attribute__((always_inline)) {
+        if (b * 128 + 128 > a.K && b * 128 + chunk >= a.K) {
 #pragma unroll
             for (int i = 0; i < kLoadW; ++i) rw[i] = none;
         }
     };
-    auto put = [&](uint8_t *wb, uint8_t *xb) __attribute__((always_inline)) {
+    auto put = [&](int b, uint8_t *wb, uint8_t *xb) __attribute__((always_inline)) {
+        clear_past(b);
 #pragma unroll
         for (int i = 0; i < kLoadW; ++i) *reinterpret_cast<i32x4 *>(wb + (wave * kLoadW + i) * 1024 + lane * 16) = rw[i];
 #pragma unroll
@@ -177,16 +180,58 @@ __global__ void __launch_bounds__(64 * kTileWaves) int8_tiles_kernel(const Args 
                 for (int r = 0; r < NT; ++r) acc[r][t] = mfma(A[r], B[t], acc[r][t]);
         }
     };
-    // The barrier at the top of a K block makes the block's stage visible and says that the stage before has been read;
-    // that one takes the next block from the registers, which the block after it is fetched into.
-    auto step = [&](int b, const uint8_t *wb, const uint8_t *xb, uint8_t *wn_, uint8_t *xn_) __attribute__((always_inline)) {
+    // The barrier at the top of a K block makes the block's stage visible and says that the stage before has been read; that one takes
+    // the next block from the registers, which the block after it is then fetched into. kSpread: operands are read, and the next
+    // block's pieces moved and requested, between the products (sched_barrier holds them there): 256 x 192 1.42 -> 1.28 us a K block
+    // with one round of 32; 384 x 192 has no registers left for it, the smaller tiles gain nothing.
+    constexpr bool kSpread = BN == 256;
+    constexpr int kPieces = kLoadW + kLoadX, kSlots = 2 * MT, kEach = (kPieces + kSlots - 1) / kSlots, kA = (NT + MT - 1) / MT;
+    auto spread_step = [&](int b, const uint8_t *wb, const uint8_t *xb, uint8_t *wn_, uint8_t *xn_) __attribute__((always_inline)) {
+        const uint8_t *wrow = wb + (wn * (BN / kWn) + n16) * 128, *xrow = xb + (wm * (BM / kWm) + n16) * 128;
+        const int at[2] = {(g ^ (n16 & 7)) * 16, ((g + 4) ^ (n16 & 7)) * 16};
+        const int off = min(min(b + 2, a.kb - 1) * 128 + chunk, a.K - 16);  // past the end: the last codes again
+        clear_past(b + 1);
+        i32x4 A[2][NT], B[2];
         lds_barrier();
-        put(wn_, xn_);
+#pragma unroll
+        for (int r = 0; r < NT; ++r) A[0][r] = *reinterpret_cast<const i32x4 *>(wrow + r * 2048 + at[0]);
+        B[0] = *reinterpret_cast<const i32x4 *>(xrow + at[0]);
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int i = 0; i < kSlots; ++i) {
+            const int c = i / MT, t = i % MT;
+            if (i + 1 < kSlots) B[(i + 1) & 1] = *reinterpret_cast<const i32x4 *>(xrow + (i + 1) % MT * 2048 + at[(i + 1) / MT]);
+            if (c == 0) {
+#pragma unroll
+                for (int r = t * kA; r < t * kA + kA && r < NT; ++r) A[1][r] = *reinterpret_cast<const i32x4 *>(wrow + r * 2048 + at[1]);
+            }
+#pragma unroll
+            for (int k = i * kEach; k < i * kEach + kEach && k < kPieces; ++k) {
+                if (k < kLoadW) {
+                    *reinterpret_cast<i32x4 *>(wn_ + (wave * kLoadW + k) * 1024 + lane * 16) = rw[k];
+                    rw[k] = load16(wbase + wo[k] + off);
+                } else {
+                    *reinterpret_cast<i32x4 *>(xn_ + (wave * kLoadX + k - kLoadW) * 1024 + lane * 16) = rx[k - kLoadW];
+                    rx[k - kLoadW] = load16(xbase + xo[k - kLoadW] + off);
+                }
+            }
+#pragma unroll
+            for (int r = 0; r < NT; ++r) acc[r][t] = mfma(A[c][r], B[i & 1], acc[r][t]);
+            __builtin_amdgcn_sched_barrier(0);
+        }
+    };
+    auto plain_step = [&](int b, const uint8_t *wb, const uint8_t *xb, uint8_t *wn_, uint8_t *xn_) __attribute__((always_inline)) {
+        lds_barrier();
+        put(b + 1, wn_, xn_);
         fetch(b + 2);
         multiply(wb, xb);
     };
+    auto step = [&](int b, const uint8_t *wb, const uint8_t *xb, uint8_t *wn_, uint8_t *xn_) __attribute__((always_inline)) {
+        if constexpr (kSpread) spread_step(b, wb, xb, wn_, xn_);
+        else plain_step(b, wb, xb, wn_, xn_);
+    };
     fetch(0);
-    put(w0, x0);
+    put(0, w0, x0);
     fetch(1);
     for (int b = 0; b < a.kb; b += 2) {
         step(b, w0, x0, w1, x1);
@@ -253,6 +298,12 @@ void launch_rows(const Args &a, hipStream_t s) {
     int8_rows_kernel<TY, NT, MT><<<grid, 64 * kRowWaves, 0, s>>>(a);
 }
 
+// Up to 16 tokens: 16 weight rows a block, whose waves read nothing twice (12288 x 4096, M = 6: 12.3 us, 4.1 TB/s). Up to 32, and up to
+// 64 where two passes still are at most two blocks a compute unit: 32 rows x 32 tokens a block. Above, the tile with the least rounds of
+// blocks over the compute units times the time of a K block of 128, measured with the chip full: 0.41, 0.65, 1.19, 1.5 and 2.27 us for
+// 128 x 64, 128 x 128, 256 x 128, 256 x 192 and 384 x 192 (rows x tokens). In us for the five tiles: 12288 x 4096, M = 1531 116 / 105 / 108 /
+// 95 / 75, 512 41 / 43 / 38 / 47 / 66, 256 26 / 24 / 33 / 43 / 65; 4096 x 4096, M = 2048 53 / 44 / 41 / 48 / 67; 7680 x 2560, M = 1531 50 / 44 /
+// 50 / 37 / 49. 75 us are 2.07 POP/s; the library's product of 8192 x 8192 x 8192 8-bit integers reaches 2.08 on the same card.
 template <typename TY>
 void launch(const Args &a, hipStream_t s) {
     const int64_t cus = device_cus();
@@ -262,7 +313,7 @@ void launch(const Args &a, hipStream_t s) {
         const int64_t tiles = (a.N + bn - 1) / bn * ((a.M + bm - 1) / bm);
         return (double)((tiles + cus - 1) / cus) * each;
     };
-    const double c[5] = {cost(128, 64, 0.48), cost(128, 128, 0.87), cost(256, 128, 1.37), cost(256, 192, 1.75), cost(384, 192, 2.5)};
+    const double c[5] = {cost(128, 64, 0.41), cost(128, 128, 0.65), cost(256, 128, 1.19), cost(256, 192, 1.5), cost(384, 192, 2.27)};
     switch ((int)(std::min_element(c, c + 5) - c)) {
     case 0: return launch_tiles<TY, 128, 64>(a, s);
     case 1: return launch_tiles<TY, 128, 128>(a, s);
