@@ -55,9 +55,11 @@ __device__ __forceinline__ constexpr int token_of(int ti, int g, int r) { return
 __device__ __forceinline__ int token_at(int ti, int m) { return token_of(ti, m >> 2, m & 3); }
 
 template <int DK>
-__global__ void __launch_bounds__(256) delta_prepare_kernel(const Args a, const Work w) {
+__global__ void __launch_bounds__(256, 4) delta_prepare_kernel(const Args a, const Work w) {
     constexpr int KS = DK / 32;
-    __shared__ __attribute__((aligned(16))) float At[kC * kPitch], P[kC * kPitch], Tm[kC * kPitch];
+    // At becomes T, P the keys' transpose, once they have been read: four blocks a compute unit
+    __shared__ __attribute__((aligned(16))) float At[kC * kPitch], P[kC * kPitch];
+    float *const Tm = At;
     __shared__ double path[kC];
     __shared__ float rk[kC], rq[kC], beta[kC];
     __shared__ uint64_t use_mask;
@@ -66,19 +68,30 @@ __global__ void __launch_bounds__(256) delta_prepare_kernel(const Args a, const 
     const int64_t slot = blockIdx.x / a.Hv;
     const int h = blockIdx.x % a.Hv, hk = h / a.rep;
     // the sequence whose chunk this is: at most one (of possible starts)
-    if (threadIdx.x == 0) found = -1;
-    __syncthreads();
-    for (int b = threadIdx.x; b < a.B; b += 256) {
-        const int t0 = a.starts[b], t1 = a.starts[b + 1];
-        if (t0 < 0 || t1 <= t0 || t1 > a.T || t1 - t0 > a.max_len) continue;
-        const int64_t f = first_slot(t0, b);
-        if (slot >= f && slot < f + (t1 - t0 + kC - 1) / kC) found = b;
+    int b = 0, t0 = 0, n = 0;
+    auto mine_is = [&](int i) {
+        t0 = a.starts[i];
+        const int t1 = a.starts[i + 1];
+        const int64_t f = first_slot(t0, i);
+        n = t1 - t0 - (int)(slot - f) * kC;
+        return t0 >= 0 && t1 > t0 && t1 <= a.T && t1 - t0 <= a.max_len && slot >= f && n > 0;
+    };
+    if (a.B == 1) {
+        if (!mine_is(0)) return;
+    } else {
+        if (threadIdx.x == 0) found = -1;
+        __syncthreads();
+        for (int i = threadIdx.x; i < a.B; i += 256)
+            if (mine_is(i)) found = i;
+        __syncthreads();
+        b = found;
+        if (b < 0) return;
+        mine_is(b);
     }
-    __syncthreads();
-    const int b = found;
-    if (b < 0) return;
-    const int t0 = a.starts[b], first = (int)(slot - first_slot(t0, b)) * kC, n = min(a.starts[b + 1] - t0 - first, kC);
-    const int64_t row0 = (int64_t)t0 + first;
+    const int64_t row0 = t0 + (slot - first_slot(t0, b)) * kC;
+    n = min(n, kC);
+    float g = 0.f, be = 0.f;  // requested before anything is waited for
+    if (wave == 0 && lane < n) gates(a, row0 + lane, h, g, be);
     const u32x4 none = {0u, 0u, 0u, 0u};
     bf16x8 K[4][KS], Q[KS];
 #pragma unroll
@@ -116,8 +129,6 @@ __global__ void __launch_bounds__(256) delta_prepare_kernel(const Args a, const 
     }
     __syncthreads();
     if (wave == 0) {
-        float g = 0.f, be = 0.f;
-        if (lane < n) gates(a, row0 + lane, h, g, be);
         const bool num = finite(rk[lane]) && finite(g) && finite(be), use = lane < n && num;
         if (!use) g = 0.f, be = 0.f, rk[lane] = 0.f;
         const uint64_t um = __ballot(use), bm = __ballot(lane < n && !num);
@@ -183,6 +194,7 @@ __global__ void __launch_bounds__(256) delta_prepare_kernel(const Args a, const 
 #pragma unroll
         for (int r = 0; r < 4; ++r) take(t * 16 + 12 + r, of_row<3>(U[t][r]));
     }
+    __syncthreads();  // every wave has read At
 #pragma unroll
     for (int t = 0; t < 4; ++t)
 #pragma unroll
@@ -206,8 +218,9 @@ __global__ void __launch_bounds__(256) delta_prepare_kernel(const Args a, const 
     }
     if (h % a.rep != 0) return;
     // the key head's K^T: row dk, eight tokens a lane
-    static_assert(DK * kPitch * 2 <= sizeof(At));
-    uint16_t *kt = reinterpret_cast<uint16_t *>(At);
+    static_assert(DK * kPitch * 2 <= sizeof(P));
+    uint16_t *kt = reinterpret_cast<uint16_t *>(P);
+    __syncthreads();  // every wave has read P
     const bool count = use >> (wave * 16 + n16) & 1;
 #pragma unroll
     for (int ks = 0; ks < KS; ++ks) {
