@@ -164,6 +164,76 @@ class VerifyAttention:
         return self.y[:T], x if residual is None else res
 
 
+class VerifyDelta:
+    """The recurrent half of a verify layer (a layer whose memory is a state): post norm of the block before, residual and norm in one
+    launch with 8-bit codes -> int8 projection -> the gated delta rule -> a norm of each head with its gate, as 8-bit codes -> int8
+    output projection. norm_w BF16 [d], post_w BF16 [d] or None; proj an Int8Weight [N, d] whose rows are queries and keys (Hk Dk
+    each), values and gates (Hv Dv each), then the decays' and the corrections' inputs (Hv each; N may be more, to a multiple of
+    8); A_log, dt_bias FP32 [Hv]; head_w BF16 [Dv], Dv a power of two up to 512; out_w an Int8Weight [d, Hv Dv]. mix (optional): called
+    with the BF16 views q, k [T, Hk, Dk] and v [T, Hv, Dv] after the projection (a short convolution), forward's stream being the
+    current one. Drafted tokens (a mask) leave the states as they are until commit takes the accepted path of the last forward;
+    without a mask (prompts, decoding) forward updates them. Buffers are kept for every stream that forward is called on; k, u and
+    decay, residual and y are the last forward's."""
+
+    def __init__(self, norm_w, proj, A_log, dt_bias, head_w, out_w, Hk, Hv, Dk, Dv, max_tokens, post_w=None, eps=1e-6, residual_scale=1.0,
+                 mix=None):
+        rows = 2 * Hk * Dk + 2 * Hv * Dv + 2 * Hv
+        assert proj.N >= rows and proj.N % 8 == 0 and out_w.K == Hv * Dv and out_w.N == proj.K == norm_w.numel() and head_w.numel() == Dv
+        self.norm_w, self.proj, self.A_log, self.dt_bias, self.head_w, self.out_w, self.post_w = norm_w, proj, A_log, dt_bias, head_w, out_w, post_w
+        self.Hk, self.Hv, self.Dk, self.Dv, self.M, self.eps, self.residual_scale, self.mix = Hk, Hv, Dk, Dv, max_tokens, eps, residual_scale, mix
+        self._dev = norm_w.device
+        self.err = torch.zeros(4, dtype=torch.int32, device=self._dev)
+        self.k = None
+        self._buffers = {}
+
+    def _buffers_for(self, stream):
+        """The stream's buffers become the layer's."""
+        key = (stream or torch.cuda.current_stream(self._dev)).cuda_stream
+        if key not in self._buffers:
+            M, d, Hv, Dv = self.M, self.proj.K, self.Hv, self.Dv
+            with torch.cuda.device(self._dev), torch.cuda.stream(stream):  # from the stream's pool (None: the current one's)
+                e = lambda dtype, *shape: torch.empty(shape, dtype=dtype, device=self._dev)
+                bf, f32, i8 = torch.bfloat16, torch.float32, torch.int8
+                self._buffers[key] = dict(residual=e(bf, M, d), q8=e(i8, M, d), scale=e(f32, M), rows=e(bf, M, self.proj.N), out=e(bf, M, Hv, Dv),
+                                          u=e(f32, M, Hv, Dv), decay=e(f32, M, Hv), o8=e(i8, M, Hv * Dv), o_scale=e(f32, M), y=e(bf, M, d))
+        vars(self).update(self._buffers[key])
+
+    def forward(self, x, residual, state, starts, max_len, mask=None, slots=None, stream=None):
+        """x, residual (None in the first layer) BF16 [T, d]; state, starts, slots and, for drafted tokens, mask as gated_delta_verify
+        takes them, at most max_len tokens a sequence. Returns (y [T, d], the residual stream). Runs on the layer's device, whichever is
+        current."""
+        if self.norm_w.is_cuda and self._dev.index != torch.cuda.current_device():
+            with torch.cuda.device(self._dev):
+                return self.forward(x, residual, state, starts, max_len, mask, slots, stream)
+        T, Hk, Hv, Dk, Dv = x.shape[0], self.Hk, self.Hv, self.Dk, self.Dv
+        assert T <= self.M
+        self._buffers_for(stream)
+        res = None if residual is None else self.residual[:T]
+        kx.block_norm_int8(x, post=self.post_w, residual=residual, pre=self.norm_w, eps=self.eps, residual_scale=self.residual_scale,
+                           residual_out=res, q=self.q8[:T], scale=self.scale[:T], stream=stream)
+        rows = kx.linear_int8(self.q8[:T], self.scale[:T], self.proj, y=self.rows[:T], stream=stream)
+        q, k, v, z, a, b = rows[:, :2 * Hk * Dk + 2 * Hv * Dv + 2 * Hv].split([Hk * Dk, Hk * Dk, Hv * Dv, Hv * Dv, Hv, Hv], dim=1)
+        q, self.k, v = q.unflatten(1, (Hk, Dk)), k.unflatten(1, (Hk, Dk)), v.unflatten(1, (Hv, Dv))
+        if self.mix is not None:
+            with torch.cuda.stream(stream):  # the projection runs there (None: the current one)
+                self.mix(q, self.k, v)
+        args, kw = (q, self.k, v, a, b, state, starts), dict(slots=slots, A_log=self.A_log, dt_bias=self.dt_bias, out=self.out[:T], err=self.err, stream=stream)
+        if mask is None:
+            kx.gated_delta(*args, max_len, **kw)
+        else:
+            kx.gated_delta_verify(*args, mask, max_len, u=self.u[:T], decay=self.decay[:T], **kw)
+        kx.block_norm_int8(self.out[:T].view(T, Hv * Dv), post=self.head_w, gate=z, group=Dv, gate_act="silu", eps=self.eps, q=self.o8[:T],
+                           scale=self.o_scale[:T], stream=stream)
+        kx.linear_int8(self.o8[:T], self.o_scale[:T], self.out_w, y=self.y[:T], stream=stream)
+        return self.y[:T], x if residual is None else res
+
+    def commit(self, state, starts, count, path=None, max_count=None, slots=None, stream=None):
+        """The accepted path of the last forward's drafted tokens (of its stream's) into the states, as gated_delta_commit."""
+        T = self.k.shape[0]
+        kx.gated_delta_commit(self.k, self.u[:T], self.decay[:T], state, starts, count, path=path, max_count=max_count, slots=slots, err=self.err,
+                              stream=stream)
+
+
 class VerifyTail:
     """The verify head: q8 LM head [V, d] -> FP32 logits [M, V] -> logits_topk (k candidates) -> device acceptance."""
 
@@ -195,3 +265,11 @@ class VerifyTail:
                        stream=stream)
         return kx.mtp_accept(self.cands[:M], self.nan[:M], drafts, u, temperature, top_k, top_p, self.n_valid,
                              out=out, stream=stream)
+
+    def accept_sampled(self, h, drafts, starts, u, temperature, max_rows, draft_logits=None, stream=None):
+        """The head's rows of a batch (sequence b's are starts[b] .. starts[b + 1] - 1) and acceptance by their probabilities, as
+        mtp_accept_sampled: (tokens, count, status). draft_logits in FP32, as the head's are."""
+        M = h.shape[0]
+        kx.linear(h, self.w, out_act=0, y=self.logits[:M], stream=stream)
+        return kx.mtp_accept_sampled(self.logits[:M], drafts, starts, u, temperature, max_rows, draft_logits=draft_logits, n_valid=self.n_valid,
+                                     stream=stream)
