@@ -464,9 +464,11 @@ std::string delta_error(const sx_delta &d) {
     if (!aligned(d.starts, 4) || !aligned(d.slot, 4) || !aligned(d.A_log, 4) || !aligned(d.dt_bias, 4) ||
         !aligned(d.a, act_bytes(d.gate_act)) || !aligned(d.b, act_bytes(d.gate_act)))
         return "starts, slot and the gates must be aligned to their elements";
-    const int64_t s[6] = {d.q.token, d.q.head, d.k.token, d.k.head, d.v.token, d.v.head};
-    for (int64_t x : s)
-        if (x < 0 || x > (int64_t)1 << 24 || x % 8 != 0) return cat("strides of q, k and v must be multiples of 8 up to 2^24 (", x, ")");
+    // a chunk's rows are addressed by 32-bit offsets, heads by 64-bit ones
+    const int64_t t[3] = {d.q.token, d.k.token, d.v.token}, h[3] = {d.q.head, d.k.head, d.v.head};
+    for (int i = 0; i < 3; ++i)
+        if (t[i] < 0 || t[i] > (int64_t)1 << 24 || t[i] % 8 != 0 || h[i] < 0 || h[i] > (int64_t)1 << 40 || h[i] % 8 != 0)
+            return cat("strides of q, k and v must be multiples of 8, of tokens up to 2^24 (", t[i], ", ", h[i], ")");
     if (d.a_token < 0 || d.b_token < 0 || d.a_token > (int64_t)1 << 32 || d.b_token > (int64_t)1 << 32) return cat("gate strides ", d.a_token, ", ", d.b_token);
     if (!std::isfinite(d.scale)) return cat("scale = ", d.scale);
     return "";
@@ -490,8 +492,8 @@ std::string output_error(const sx_delta &d, const void *o, int64_t n) {
 
 std::string out_error(const sx_delta &d, const sx_head_rows &o) {
     if (o.p == nullptr) return "null pointer";
-    if (!aligned(o.p, 8) || o.token < 0 || o.head < 0 || o.token % 4 != 0 || o.head % 4 != 0 || o.token > (int64_t)1 << 24 || o.head > (int64_t)1 << 24)
-        return cat("must be 8-byte aligned with strides that are multiples of 4, up to 2^24 (", o.token, ", ", o.head, ")");
+    if (!aligned(o.p, 8) || o.token < 0 || o.head < 0 || o.token % 4 != 0 || o.head % 4 != 0 || o.token > (int64_t)1 << 24 || o.head > (int64_t)1 << 40)
+        return cat("must be 8-byte aligned with strides that are multiples of 4, of tokens up to 2^24 (", o.token, ", ", o.head, ")");
     if (!rows_apart(d.dim, {{d.T, o.token}, {d.heads, o.head}})) return "has heads that overlap";
     const std::string e = output_error(d, o.p, span(o, d.T, d.heads, d.dim));
     if (!e.empty()) return e;
@@ -501,7 +503,7 @@ std::string out_error(const sx_delta &d, const sx_head_rows &o) {
 delta::Args args_of(const sx_delta &d, const sx_head_rows *out, int64_t max_len, uint32_t *err) {
     const auto h = [](const sx_head_rows &r) { return static_cast<const uint16_t *>(r.p); };
     return {h(d.q), h(d.k), h(d.v), d.a, d.b, d.A_log, d.dt_bias, d.state, d.slot, d.starts, static_cast<uint16_t *>(out->p), err,
-            d.q.token, d.q.head, d.k.token, d.k.head, d.v.token, d.v.head, d.a_token, d.b_token, out->token, out->head, d.state_slot,
+            d.q.token, d.q.head, d.k.token, d.k.head, d.v.token, d.v.head, d.a_token, d.b_token, d.T > 1 ? out->token : d.dim, out->head, d.state_slot,
             (int32_t)d.T, (int32_t)d.key_heads, (int32_t)d.heads, (int32_t)(d.heads / d.key_heads), (int32_t)d.dim, (int32_t)d.batch,
             (int32_t)d.slots, (int32_t)max_len, d.scale, d.gate_act == SX_ACT_F32, d.normalize != 0};
 }

@@ -522,7 +522,7 @@ __global__ void __launch_bounds__(512) delta_scan_kernel(const Args a, const Wor
             uint8_t *oc = reinterpret_cast<uint8_t *>(op + (int64_t)c * kC * a.o_t);
             // Always four stores, of rows past the sequence's end too, which the buffer's size leaves out: stores that a branch skips
             // would make the next chunk's Q wait for all that is in flight.
-            const auto rows = __builtin_amdgcn_make_buffer_rsrc(oc, 0, min(left, kC) * (int)ostep, 0x00020000);
+            const auto rows = __builtin_amdgcn_make_buffer_rsrc(oc, 0, (int)((uint32_t)min(left, kC) * ostep), 0x00020000);
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
                 const float o = mine + r >= from ? qnan() : O[r] + O2[r];

@@ -4,7 +4,7 @@ preallocated device buffers so a forward allocates nothing.
 """
 import torch
 
-from . import MOE_F32, SxError
+from . import MOE_F32, SX_EINVAL, SxError
 from . import kernels as kx
 
 
@@ -183,7 +183,7 @@ class VerifyDelta:
         self.Hk, self.Hv, self.Dk, self.Dv, self.M, self.eps, self.residual_scale, self.mix = Hk, Hv, Dk, Dv, max_tokens, eps, residual_scale, mix
         self._dev = norm_w.device
         self.err = torch.zeros(4, dtype=torch.int32, device=self._dev)
-        self.k = None
+        self.k, self.drafted = None, False
         self._buffers = {}
 
     def _buffers_for(self, stream):
@@ -218,6 +218,7 @@ class VerifyDelta:
             with torch.cuda.stream(stream):  # the projection runs there (None: the current one)
                 self.mix(q, self.k, v)
         args, kw = (q, self.k, v, a, b, state, starts), dict(slots=slots, A_log=self.A_log, dt_bias=self.dt_bias, out=self.out[:T], err=self.err, stream=stream)
+        self.drafted = mask is not None
         if mask is None:
             kx.gated_delta(*args, max_len, **kw)
         else:
@@ -228,7 +229,9 @@ class VerifyDelta:
         return self.y[:T], x if residual is None else res
 
     def commit(self, state, starts, count, path=None, max_count=None, slots=None, stream=None):
-        """The accepted path of the last forward's drafted tokens (of its stream's) into the states, as gated_delta_commit."""
+        """The accepted path of the last forward's drafted tokens into the states, as gated_delta_commit."""
+        if not self.drafted:
+            raise SxError(SX_EINVAL, "the last forward had no drafted tokens: its states are up to date")
         T = self.k.shape[0]
         kx.gated_delta_commit(self.k, self.u[:T], self.decay[:T], state, starts, count, path=path, max_count=max_count, slots=slots, err=self.err,
                               stream=stream)

@@ -167,6 +167,25 @@ def test_a_prompt_in_two_calls(cut):
     close(got[x.slot(0)], state[x.slot(0)], stol[x.slot(0)], 40 * U32)
 
 
+def test_heads_ahead_of_tokens_and_a_single_row_of_stride_zero():
+    """[heads, tokens, dim] in memory on every side, and an output of one token whose stride says nothing."""
+    x = Tokens([70, 20], Hk=2, Hv=4, seed=12)
+    s = x.state.clone()
+    ref, _ = x.run(s)
+    turn = lambda t: t.transpose(0, 1).contiguous().transpose(0, 1)
+    x.q, x.k, x.v = turn(x.q), turn(x.k), turn(x.v)
+    got, out = x.state.clone(), torch.empty(x.Hv, x.T, x.Dv, dtype=BF, device="cuda").transpose(0, 1)
+    x.run(got, out=out)
+    assert torch.equal(out, ref) and torch.equal(got, s)
+    x = Tokens([1], seed=13)
+    for limit in (1, 64):
+        a, b = x.state.clone(), x.state.clone()
+        ref, _ = x.run(a, max_len=limit)
+        out = torch.zeros(1, x.Hv, x.Dv, dtype=BF, device="cuda").as_strided((1, x.Hv, x.Dv), (0, x.Dv, 1))
+        x.run(b, max_len=limit, out=out)
+        assert torch.equal(out, ref) and torch.equal(a, b)
+
+
 def test_new_sequences_long_decays_and_full_resets():
     x = Tokens([40, 90, 6], raw=True, f32=True, seed=5)
     x.state.zero_()

@@ -7,6 +7,7 @@ kernel's codes where it makes them, and the projections, the rule and the norms 
 import pytest
 import torch
 
+from strixite_amd import SxError
 from strixite_amd import kernels as kx
 from strixite_amd import synthetic as syn
 from strixite_amd.verify import VerifyDelta, VerifyTail
@@ -125,6 +126,14 @@ def test_verifies_go_where_decoding_goes():
             on = [i for i in range(B) if t < count[i]]
             one.forward(torch.cat([x[i * n + t:i * n + t + 1] for i in on]), None, b, i32(list(range(len(on) + 1))), 1, slots=i32(on))
         near(a, b, 200 * 2.0 ** -24)
+
+
+def test_there_is_nothing_to_commit_behind_a_prompt():
+    L = layer(2)
+    x, state = torch.randn(8, d, device="cuda").to(BF), torch.zeros(1, Hv, Dk, Dv, device="cuda")
+    L.forward(x, None, state, i32([0, 8]), 8)
+    with pytest.raises(SxError, match="no drafted tokens"):
+        L.commit(state, i32([0, 8]), i32([1]), max_count=8)
 
 
 def test_what_is_accepted_is_committed():

@@ -69,7 +69,7 @@ BAD_DELTA = [
     (dict(dim=0), "dim = 0"), (dict(slots=0), "slots"), (dict(slot=None, slots=1), "slots = 1"), (dict(state_slot=16380), "state_slot"),
     (dict(state_slot=16386), "state_slot"), (dict(state=BASE + 65540), "16-byte"), (dict(q=sx.HeadRows(BASE + 2, 512, 64, 0)), "16-byte"),
     (dict(k=sx.HeadRows(BASE, 508, 64, 0)), "multiples of 8"), (dict(v=sx.HeadRows(BASE, -512, 64, 0)), "multiples of 8"), (dict(a=BASE + 8193), "aligned"),
-    (dict(b_token=-1), "gate strides"), (dict(scale=float("nan")), "scale"), (dict(scale=float("inf")), "scale"),
+    (dict(b_token=-1), "gate strides"), (dict(q=sx.HeadRows(BASE, 1 << 25, 64, 0)), "up to 2^24"), (dict(out=(16384, 1 << 25, 64)), "up to 2^24"), (dict(scale=float("nan")), "scale"), (dict(scale=float("inf")), "scale"),
     (dict(out=(16384, 250, 64)), "multiples of 4"), (dict(out=(16388, 256, 64)), "8-byte aligned"), (dict(out=(16384, 256, 32)), "heads that overlap"),
     (dict(out=(512, 512, 64)), "overlaps q, k or v"), (dict(out=(8192, 256, 64)), "overlaps the gates"), (dict(out=(65536, 256, 64)), "overlaps the states"),
 ]
