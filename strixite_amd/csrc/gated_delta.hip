@@ -19,6 +19,7 @@
 
 #include <algorithm>
 #include <cmath>
+#include <type_traits>
 
 namespace sx {
 namespace {
@@ -274,46 +275,62 @@ __global__ void __launch_bounds__(64 * W) delta_verify_kernel(const VerifyArgs v
             const int i = t * 16 + g4 * 4 + r;
             U[t][r] = i < s.n ? beta[i] * (bf16_to_f32(v[t][r]) - grow[i] * rk[i] * X[t][r]) : 0.f;
         }
-    // Forward substitution: token i's u is ready once those before it have been taken off its row, and then taken off all
-    // rows behind it.
+    // Forward substitution: token i's u is ready once those before it have been taken off its row, and then taken off all rows behind
+    // it. GUARD leaves unseen pairs out; without it they are zeros, which is as good while all is finite.
+    auto solve = [&](auto guard) __attribute__((always_inline)) {
+        constexpr bool GUARD = decltype(guard)::value;
 #pragma unroll
-    for (int t = 0; t < NT; ++t) {
-        auto take = [&](int i, float u) __attribute__((always_inline)) {
+        for (int t = 0; t < NT; ++t) {
+            auto take = [&](int i, float u) __attribute__((always_inline)) {
 #pragma unroll
-            for (int x = t; x < NT; ++x) {
-                const f32x4 c = *reinterpret_cast<const f32x4 *>(&At[i * kPitch + x * 16 + g4 * 4]);
+                for (int x = t; x < NT; ++x) {
+                    const f32x4 c = *reinterpret_cast<const f32x4 *>(&At[i * kPitch + x * 16 + g4 * 4]);
 #pragma unroll
-                for (int r = 0; r < 4; ++r) U[x][r] = __float_as_uint(c[r]) == 0x80000000u ? U[x][r] : fmaf(-c[r], u, U[x][r]);
+                    for (int r = 0; r < 4; ++r) U[x][r] = GUARD && __float_as_uint(c[r]) == 0x80000000u ? U[x][r] : fmaf(-c[r], u, U[x][r]);
+                }
+            };
+            if (t * 16 < s.n) {
+#pragma unroll
+                for (int r = 0; r < 4; ++r) take(t * 16 + r, of_row<0>(U[t][r]));
             }
-        };
-        if (t * 16 < s.n) {
+            if (t * 16 + 4 < s.n) {
 #pragma unroll
-            for (int r = 0; r < 4; ++r) take(t * 16 + r, of_row<0>(U[t][r]));
-        }
-        if (t * 16 + 4 < s.n) {
+                for (int r = 0; r < 4; ++r) take(t * 16 + 4 + r, of_row<1>(U[t][r]));
+            }
+            if (t * 16 + 8 < s.n) {
 #pragma unroll
-            for (int r = 0; r < 4; ++r) take(t * 16 + 4 + r, of_row<1>(U[t][r]));
-        }
-        if (t * 16 + 8 < s.n) {
+                for (int r = 0; r < 4; ++r) take(t * 16 + 8 + r, of_row<2>(U[t][r]));
+            }
+            if (t * 16 + 12 < s.n) {
 #pragma unroll
-            for (int r = 0; r < 4; ++r) take(t * 16 + 8 + r, of_row<2>(U[t][r]));
+                for (int r = 0; r < 4; ++r) take(t * 16 + 12 + r, of_row<3>(U[t][r]));
+            }
         }
-        if (t * 16 + 12 < s.n) {
+    };
+    f32x4 before[NT];
 #pragma unroll
-            for (int r = 0; r < 4; ++r) take(t * 16 + 12 + r, of_row<3>(U[t][r]));
-        }
+    for (int t = 0; t < NT; ++t) before[t] = U[t];
+    solve(std::false_type{});
+    bool fine = true;
+#pragma unroll
+    for (int t = 0; t < NT; ++t)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) fine &= finite(U[t][r]);
+    const bool all_fine = !__any(!fine);
+    if (!all_fine) {
+#pragma unroll
+        for (int t = 0; t < NT; ++t) U[t] = before[t];
+        solve(std::true_type{});
     }
     f32x4 O[NT];
-    bool fine = true;
 #pragma unroll
     for (int t = 0; t < NT; ++t)
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
             const int i = t * 16 + g4 * 4 + r;
             O[t][r] = grow[i] * rq[i] * Y[t][r];
-            fine &= finite(U[t][r]);
         }
-    if (!__any(!fine)) {
+    if (all_fine) {
         // P U with both in two BF16 terms (2^-16), one product of 32 tokens a pair of tiles
 #pragma unroll
         for (int p = 0; p < (NT + 1) / 2; ++p) {
