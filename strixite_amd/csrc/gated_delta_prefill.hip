@@ -44,8 +44,10 @@ static_assert(sizeof(Words) <= 1024);
 
 struct Work {
     uint8_t *heads;  // [chunk slots][Hv] kHeadBytes: T, P, Words
-    uint8_t *keys;   // [chunk slots][Hk] K^T as operands: [Dk / 16][2][64 lanes][8]
+    uint8_t *keys;   // [chunk slots][Hk] 3 Dk 128: K^T, K and Q as operands: K^T [Dk / 16][2][64 lanes][8], K and Q [4 tiles][4][64 lanes][Dk / 16]
 };
+template <int DK>
+constexpr int kKeyBytes = DK * kC * 2;  // of one of the three
 
 // A sequence's chunks take slots starts[b] / 64 + b on: enough for a last chunk that is not full.
 __device__ __forceinline__ int64_t first_slot(int t0, int b) { return t0 / kC + b; }
@@ -62,7 +64,7 @@ __global__ void __launch_bounds__(256, 4) delta_prepare_kernel(const Args a, con
     float *const Tm = At;
     __shared__ double path[kC];
     __shared__ float rk[kC], rq[kC], beta[kC];
-    __shared__ uint64_t use_mask;
+    __shared__ uint64_t use_mask, key_mask;  // tokens that count; those whose key does, whatever this head's gates are
     __shared__ int found;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), n16 = lane & 15, g4 = lane >> 4;
     const int64_t slot = blockIdx.x / a.Hv;
@@ -129,6 +131,8 @@ __global__ void __launch_bounds__(256, 4) delta_prepare_kernel(const Args a, con
     }
     __syncthreads();
     if (wave == 0) {
+        const uint64_t km = __ballot(lane < n && finite(rk[lane]));
+        if (lane == 0) key_mask = km;
         const bool num = finite(rk[lane]) && finite(g) && finite(be), use = lane < n && num;
         if (!use) g = 0.f, be = 0.f, rk[lane] = 0.f;
         const uint64_t um = __ballot(use), bm = __ballot(lane < n && !num);
@@ -217,11 +221,33 @@ __global__ void __launch_bounds__(256, 4) delta_prepare_kernel(const Args a, con
         for (int s = 0; s < 2; ++s) *reinterpret_cast<bf16x8 *>(head + kTBytes + (blk * 2 + s) * 1024 + lane * 16) = ps[s];
     }
     if (h % a.rep != 0) return;
-    // the key head's K^T: row dk, eight tokens a lane
+    // The key head's K and Q, their rows in the order of the tiles, and K^T: row dk, eight tokens a lane. (Read from the caller's rows,
+    // half a line of each, they cost the scan 45 us of a prompt of 8192 tokens.)
+    uint8_t *keys = w.keys + (slot * a.Hk + hk) * (3 * kKeyBytes<DK>);
+    {
+        const int i = wave * 16 + n16, at = 2 * (i >> 5) + (i >> 2 & 1), m = 4 * (i >> 3 & 3) + (i & 3);  // tile and row of token i
+        const bool in = key_mask >> i & 1;
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks) {
+            const u32x4 kx = in ? __builtin_bit_cast(u32x4, mine[ks]) : none, qx = __builtin_bit_cast(u32x4, Q[ks]);
+            if constexpr (DK == 128) {
+                const int to = ((at * 4 + ks) * 64 + m + 16 * g4) * 16;
+                *reinterpret_cast<u32x4 *>(keys + kKeyBytes<DK> + to) = kx;
+                *reinterpret_cast<u32x4 *>(keys + 2 * kKeyBytes<DK> + to) = qx;
+            } else {
+#pragma unroll
+                for (int half = 0; half < 2; ++half) {
+                    const int to = ((at * 4 + 2 * ks + (g4 >> 1)) * 64 + m + 16 * ((g4 & 1) * 2 + half)) * 8;
+                    *reinterpret_cast<u32x2 *>(keys + kKeyBytes<DK> + to) = u32x2{kx[2 * half], kx[2 * half + 1]};
+                    *reinterpret_cast<u32x2 *>(keys + 2 * kKeyBytes<DK> + to) = u32x2{qx[2 * half], qx[2 * half + 1]};
+                }
+            }
+        }
+    }
     static_assert(DK * kPitch * 2 <= sizeof(P));
     uint16_t *kt = reinterpret_cast<uint16_t *>(P);
     __syncthreads();  // every wave has read P
-    const bool count = use >> (wave * 16 + n16) & 1;
+    const bool count = key_mask >> (wave * 16 + n16) & 1;
 #pragma unroll
     for (int ks = 0; ks < KS; ++ks) {
         const u32x4 x = __builtin_bit_cast(u32x4, mine[ks]);
@@ -230,7 +256,6 @@ __global__ void __launch_bounds__(256, 4) delta_prepare_kernel(const Args a, con
             kt[(ks * 32 + g4 * 8 + j) * kPitch + wave * 16 + n16] = count ? (uint16_t)(x[j / 2] >> (16 * (j & 1))) : (uint16_t)0;
     }
     __syncthreads();
-    uint8_t *keys = w.keys + (slot * a.Hk + hk) * (DK / 16 * 2048);
     constexpr int TS = DK / 64;
 #pragma unroll
     for (int s = 0; s < TS; ++s)
@@ -303,8 +328,8 @@ __global__ void __launch_bounds__(512) delta_scan_kernel(const Args a, const Wor
     if (threadIdx.x < 16) poison[threadIdx.x] = 0x7fffffff;
     const int chunks = (s.n + kC - 1) / kC;
     const int64_t slot0 = first_slot(s.t0, b);
-    const uint8_t *const heads = w.heads + (slot0 * a.Hv + h) * kHeadBytes, *const keys = w.keys + (slot0 * a.Hk + hk) * (DK / 16 * 2048);
-    const uint16_t *const kp = a.k + s.t0 * a.k_t + hk * a.k_h, *const qp = a.q + s.t0 * a.q_t + hk * a.q_h, *const vp = a.v + s.t0 * a.v_t + h * a.v_h;
+    const uint8_t *const heads = w.heads + (slot0 * a.Hv + h) * kHeadBytes, *const keys = w.keys + (slot0 * a.Hk + hk) * (3 * kKeyBytes<DK>);
+    const uint16_t *const vp = a.v + s.t0 * a.v_t + h * a.v_h;
     const f32x4 zero = {0.f, 0.f, 0.f, 0.f};
     const uint32_t at16 = lane * 16;
     const int mine = token_of(wt, g4, 0);  // the first of this lane's four tokens
@@ -321,24 +346,18 @@ __global__ void __launch_bounds__(512) delta_scan_kernel(const Args a, const Wor
         for (int t = 0; t < TS; ++t)
 #pragma unroll
             for (int r = 0; r < 4; ++r) S[t][r] = state[(int64_t)(4 * t + r) * a.Dv];
-        // byte offsets of a whole chunk's rows from its first
-        const uint32_t kstep = (uint32_t)a.k_t * 2, vstep = (uint32_t)a.v_t * 2, kcol = (16 * TS * wave + 4 * TS * g4) * 2, vcol = col * 2;
-        uint32_t ko[4], vo[4];
+        // byte offsets of a whole chunk's values from its first
+        const uint32_t vstep = (uint32_t)a.v_t * 2, vcol = col * 2;
+        uint32_t vo[4];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) ko[i] = token_at(i, n16) * kstep + kcol, vo[i] = (mine + i) * vstep + vcol;
+        for (int i = 0; i < 4; ++i) vo[i] = (mine + i) * vstep + vcol;
         StateChunk<TS> now;
         // past the last chunk: the last one again, not used
         auto fetch_k = [&](int c, StateChunk<TS> &o) __attribute__((always_inline)) {
             c = min(c, chunks - 1);
-            const uint16_t *kc = kp + (int64_t)c * kC * a.k_t;
-            const int left = s.n - 1 - c * kC;
-            if (left >= kC - 1) {
+            const uint8_t *key = keys + (int64_t)c * a.Hk * (3 * kKeyBytes<DK>) + kKeyBytes<DK> + wave * (512 * TS);
 #pragma unroll
-                for (int i = 0; i < 4; ++i) o.K[i] = load_piece<TS>(kc, ko[i]);
-            } else {
-#pragma unroll
-                for (int i = 0; i < 4; ++i) o.K[i] = load_piece<TS>(kc, min(token_at(i, n16), left) * kstep + kcol);
-            }
+            for (int i = 0; i < 4; ++i) o.K[i] = load_piece<TS>(key + i * (2048 * TS), lane * (8 * TS));
         };
         auto fetch_v = [&](int c, StateChunk<TS> &o) __attribute__((always_inline)) {
             c = min(c, chunks - 1);
@@ -367,7 +386,7 @@ __global__ void __launch_bounds__(512) delta_scan_kernel(const Args a, const Wor
         };
         auto fetch_kt = [&](int c, StateChunk<TS> &o) __attribute__((always_inline)) {
             c = min(c, chunks - 1);
-            const uint8_t *key = keys + (int64_t)c * a.Hk * (DK / 16 * 2048) + wave * TS * 2048;
+            const uint8_t *key = keys + (int64_t)c * a.Hk * (3 * kKeyBytes<DK>) + wave * TS * 2048;
 #pragma unroll
             for (int t = 0; t < TS; ++t)
 #pragma unroll
@@ -385,12 +404,6 @@ __global__ void __launch_bounds__(512) delta_scan_kernel(const Args a, const Wor
             bf16x8 so[3];
             split(s8, so);
             ss[wave][0][lane] = __builtin_bit_cast(u32x4, so[0]), ss[wave][1][lane] = __builtin_bit_cast(u32x4, so[1]);
-            if (now.use != ~0ull) {
-                const u32x4 none = {0u, 0u, 0u, 0u};
-#pragma unroll
-                for (int t = 0; t < 4; ++t)
-                    if (!(now.use >> token_at(t, n16) & 1)) now.K[t] = __builtin_bit_cast(bf16x8, none);
-            }
             f32x4 X[4];
 #pragma unroll
             for (int t = 0; t < 4; ++t) X[t] = mfma(now.K[t], so[2], zero);
@@ -472,19 +485,16 @@ __global__ void __launch_bounds__(512) delta_scan_kernel(const Args a, const Wor
     };
     auto output = [&](auto count) __attribute__((always_inline)) {
         constexpr int PAIRS = decltype(count)::value;
-        const uint32_t qstep = (uint32_t)a.q_t * 2, ostep = (uint32_t)a.o_t * 2, qcol = 4 * TS * g4 * 2;
-        const uint32_t qo = token_at(wt, n16) * qstep + qcol;
+        const uint32_t ostep = (uint32_t)a.o_t * 2;
         uint32_t oo[4];
 #pragma unroll
         for (int r = 0; r < 4; ++r) oo[r] = (mine + r) * ostep + col * 2;
         OutChunk now;
         auto fetch_q = [&](int c, OutChunk &o) __attribute__((always_inline)) {
             c = min(c, chunks - 1);
-            const uint16_t *qc = qp + (int64_t)c * kC * a.q_t;
-            const int left = s.n - 1 - c * kC;
-            const uint32_t off = left >= kC - 1 ? qo : min(token_at(wt, n16), left) * qstep + qcol;
+            const uint8_t *key = keys + (int64_t)c * a.Hk * (3 * kKeyBytes<DK>) + 2 * kKeyBytes<DK> + wt * (2048 * TS);
 #pragma unroll
-            for (int i = 0; i < 4; ++i) o.Q[i] = load_piece<TS>(qc, off + 32 * TS * i);
+            for (int i = 0; i < 4; ++i) o.Q[i] = load_piece<TS>(key + i * (512 * TS), lane * (8 * TS));
             o.out = __builtin_bit_cast(f32x4, load16(reinterpret_cast<const Words *>(heads + (int64_t)c * a.Hv * kHeadBytes + kTBytes + kPBytes)->out, mine * 4));
         };
         auto fetch_p = [&](int c, OutChunk &o) __attribute__((always_inline)) {
@@ -541,7 +551,7 @@ __global__ void __launch_bounds__(512) delta_scan_kernel(const Args a, const Wor
 }  // namespace
 
 size_t prefill_bytes(int64_t T, int64_t B, int64_t Hk, int64_t Hv, int64_t Dk) {
-    return (size_t)((T / kC + B) * (Hv * kHeadBytes + Hk * (Dk / 16 * 2048)));
+    return (size_t)((T / kC + B) * (Hv * kHeadBytes + Hk * (3 * Dk * kC * 2)));
 }
 
 void prefill(const Args &a, int Dk, void *ws, hipStream_t s) {

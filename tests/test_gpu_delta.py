@@ -308,6 +308,7 @@ def test_a_token_that_is_no_number(n, at, what):
     heads = {"k": 2, "q": 2, "v": 1, "a": 1}[what]
     o, _ = x.run(clean)
     assert torch.equal(o[:at], ref[:at]) and torch.equal(o[n:], ref[n:]) and torch.equal(o[:, heads:], ref[:, heads:])
+    assert torch.equal(clean[:, heads:], cs[:, heads:])  # value heads that share the key head, too
     if what == "q":
         assert o[at, :heads].isnan().all() and torch.equal(o[at + 1:], ref[at + 1:]) and torch.equal(clean, cs)
     elif what == "v":
