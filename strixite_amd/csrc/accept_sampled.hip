@@ -8,7 +8,8 @@
 // place and its sum of exponentials. Then a wave combines a row's chunks, the rows of a sequence at once, which tells the last row that
 // counts; that one's chunks of max(p - q, 0) are summed where there are draft logits, and one block a sequence finds the chunk,
 // and in it the token, at which the running sum passes u times the total (second launch). Sums are taken in one order, whatever
-// the schedule.
+// the schedule. 16 sequences of up to 6 rows of 151,936 logits with draft logits: 24 + 5.7 + 17 us, the first the VALU's (an FP64
+// exponential a logit, 0.65 of its cycles); one sequence without: 5.4 + 8.7, latencies.
 #include "common.hpp"
 
 #include <cmath>
@@ -317,8 +318,8 @@ __global__ void __launch_bounds__(kDrawThreads) accept_decide_kernel(const Args 
 }
 
 // Grid (1, B) without draft logits; with them (chunks, B) behind accept_decide_kernel: then a block also sums its chunk of
-// max(p - q, 0), and the last block of a sequence to get there draws. (All of them deciding for themselves: 16 sequences of 38 chunks
-// 21.4 us, 5 us more than both launches.)
+// max(p - q, 0), and the last block of a sequence to get there draws. (All of them deciding for themselves took
+// 21.4 us for 16 sequences of 38 chunks, both launches take 5.7 + 17; but that grows with rows times chunks.)
 template <typename T, bool DRAFT>
 __global__ void __launch_bounds__(kDrawThreads) accept_draw_kernel(const Args a) {
     __shared__ Verdict v;

@@ -8,7 +8,8 @@
 // 32 heads of 128) and its four waves share a chunk: wave w holds a quarter of the state's rows in registers, multiplies K
 // and Q with them for all 64 tokens, and has a quarter of the tokens after that. What passes between the waves (sums of K S
 // and Q S, V - e^G K S, U) goes through LDS, three barriers a chunk. The latency of that chain is what bounds one
-// sequence.
+// sequence: 8192 tokens, 32 heads of 128: 94 + 240 us, 1.9 us a chunk (the matrix unit busy 0.15 of it; 1.2 us without any loads,
+// which are 100 KB a chunk and compute unit).
 //
 // Operands: a result of the matrix unit has four consecutive rows a lane, an operand eight consecutive values of a row. The
 // rows of two result tiles are dealt out so that a lane's four of the one and four of the other are eight consecutive
