@@ -380,7 +380,7 @@ __global__ void __launch_bounds__(512) delta_scan_kernel(const Args a, const Wor
             c = min(c, chunks - 1);
 #pragma unroll
             for (int p = 0; p < PAIRS; ++p) {
-                const uint8_t *blk = heads + (int64_t)c * a.Hv * kHeadBytes + block_of(wave, p) * 3072;
+                const uint8_t *blk = heads + (int64_t)c * a.Hv * kHeadBytes + block_of(wave, p) * (3 * 1024);
 #pragma unroll
                 for (int i = 0; i < 3; ++i) o.T[p][i] = __builtin_bit_cast(bf16x8, load16(blk, at16 + i * 1024));
             }
