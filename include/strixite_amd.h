@@ -388,8 +388,9 @@ int sx_mtp_accept_sampled(const void *logits, int64_t ld, int64_t T, int64_t n_v
  *   r = residual_scale * residual + branch_scale * h    rounded to act and stored to residual_out; residual null: branch_scale * h
  *   y = r / sqrt(mean(r^2) + eps) * (pre + w_add)       pre null: y = r
  * Outputs: residual_out (with a residual), y (nullable) [M, K] in act, q (nullable) [M, K] int8 codes of y with scale [M] FP32 =
- * amax(|y|) / 127, the activations sx_linear_int8 takes. A code is the nearest one, ties to even, of the exact y / scale (FP64: off
- * where they lie 1e-13 from a border). A row of zeros has scale 0 and codes 0, one that holds NaN or an infinity scale NaN and
+ * amax(|y|) / 127, the activations sx_linear_int8 takes. A code is the nearest one, ties to even, of y / scale as the formulas give it
+ * in FP64, in their order (a mean is the sum times the rounded
+ * 1 / K; only the order in which squares are added is open). A row of zeros has scale 0 and codes 0, one that holds NaN or an infinity scale NaN and
  * codes 0. post has post_len values: K (0 says so too) or the group's. K a multiple of 8, up to 16384. residual_out and y may be x,
  * the residual or the gate, row for row. No reference counterpart. */
 enum sx_gate_act { SX_GATE_NONE = 0, SX_GATE_SILU = 1, SX_GATE_SIGMOID = 2 };
@@ -400,7 +401,7 @@ typedef struct sx_block_norm {
     float *scale;
     int64_t ldx, ld_gate, group, post_len;
     int32_t gate_act;
-    float eps, w_add, residual_scale, branch_scale;
+    double eps, w_add, residual_scale, branch_scale;
 } sx_block_norm;
 int sx_block_norm_int8(const sx_block_norm *p, int64_t M, int64_t K, int act, sx_stream stream);
 

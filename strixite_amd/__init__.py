@@ -57,7 +57,7 @@ class BlockNormC(ctypes.Structure):
     """sx_block_norm: the norms around a block."""
     _fields_ = [(n, ctypes.c_void_p) for n in ("x", "post", "gate", "residual", "pre", "residual_out", "y", "q", "scale")] + [
         (n, ctypes.c_int64) for n in ("ldx", "ld_gate", "group", "post_len")] + [("gate_act", ctypes.c_int32)] + [
-        (n, ctypes.c_float) for n in ("eps", "w_add", "residual_scale", "branch_scale")]
+        (n, ctypes.c_double) for n in ("eps", "w_add", "residual_scale", "branch_scale")]
 
 
 class HeadRows(ctypes.Structure):

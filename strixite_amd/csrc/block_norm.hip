@@ -6,10 +6,13 @@
 // and y as int8 codes with one FP32 scale a row, amax(|y|) / 127: the form sx_linear_int8 takes its activations in.
 //
 // A row is read once into registers (8 features a 16-byte load) and written from there. A code is a whole number that a border
-// decides, so it has to be that of the exact value: all is computed in FP64, which runs at FP32's rate here. The second norm's root
-// cancels in the codes, which come from t = r (pre + w_add) alone. The VALU's work bounds it where there is a gate (2048 rows of 4096, heads
-// of 128: 700 instructions a wave). In FP32 with a bound on what that is off, and FP64 for what the bound leaves open (one code in
-// two thousand, the row's largest value), it was as slow: 820 instructions.
+// decides, so it has to be that of the exact value: all is computed in FP64, which runs at FP32's rate here. Where a product of BF16
+// values lies on the border itself, the rounding of x / root decides, so mean, root and quotient are FP64's nearest and the code is
+// the formula's in 64 bits (40 instructions of 744 a wave; with a reciprocal root three calls in a hundred, without a residual, had a
+// code on the border's other side). The second norm's root cancels in the codes, which come from t = r (pre + w_add) alone. The VALU's
+// work bounds it where there is a gate (2048 rows of 4096, heads of 128: 24.9 us a call, 0.74 of the VALU's cycles). In FP32 with a
+// bound on what that is off, and FP64 for what the bound leaves open (one code in two thousand, the row's largest value), it was as
+// slow: 820 instructions.
 #include "common.hpp"
 
 #include <cmath>
@@ -28,8 +31,7 @@ struct Args {
     int64_t M, ldx, ldg;
     int32_t K, group, post_wrap;  // group: 0, the row; post_wrap: post has that many values
     int32_t gate_act;
-    float eps, w_add, rs, bs;
-    double over_k, over_group;
+    double eps, w_add, rs, bs, over_k, over_group;
 };
 
 __device__ __forceinline__ void load8(const float *p, float (&v)[8]) {
@@ -84,6 +86,21 @@ __device__ __forceinline__ double over_root(double x) {
     const double half = -0.5 * x;
     q = fma(fma(half * q, q, 0.5), q, q);
     return fma(fma(half * q, q, 0.5), q, q);
+}
+
+// sqrt(mean + eps), its reciprocal and, for the quotients' correction, its negative (0 where it is infinite: x / infinity is 0).
+struct Root {
+    double inv, neg;
+};
+__device__ __forceinline__ Root root_of(double sum, double over, double eps) {
+#pragma clang fp contract(off)
+    const double mean = sum * over, root = sqrt(mean + eps);  // two roundings, as the formula has them
+    return {1.0 / root, root < INFINITY ? -root : 0.0};
+}
+// x / root: the product's error, computed exactly, put right in one step.
+__device__ __forceinline__ double divided(double x, Root r) {
+    const double q = x * r.inv;
+    return fma(fma(q, r.neg, x), r.inv, q);
 }
 
 struct Sum {
@@ -153,28 +170,29 @@ __global__ void __launch_bounds__(TPR < 256 ? 256 : TPR) block_norm_kernel(const
         }
     }
     if (a.post != nullptr) {
+        Root whole{};
         if (a.group == 0) {
 #pragma unroll
             for (int j = 0; j < NV; ++j)
 #pragma unroll
                 for (int k = 0; k < 8; ++k) ss = fma(h[j][k], h[j][k], ss);
-            ss = over_root(fma(row_reduce<Sum, TPR>(ss, part[0]), a.over_k, (double)a.eps));
+            whole = root_of(row_reduce<Sum, TPR>(ss, part[0]), a.over_k, a.eps);
         }
 #pragma unroll
         for (int j = 0; j < NV; ++j) {
             const int i = tid + j * TPR;
-            double inv = ss;
+            Root root = whole;
             if (a.group != 0) {
-                inv = 0.0;
+                double sum = 0.0;
 #pragma unroll
-                for (int k = 0; k < 8; ++k) inv = fma(h[j][k], h[j][k], inv);
-                inv = over_root(fma(group_sum(inv, a.group), a.over_group, (double)a.eps));
+                for (int k = 0; k < 8; ++k) sum = fma(h[j][k], h[j][k], sum);
+                root = root_of(group_sum(sum, a.group), a.over_group, a.eps);
             }
             if (row && i < n8) {
                 float w[8];
                 load8(static_cast<const T *>(a.post) + (a.post_wrap == a.K ? i * 8 : i * 8 & (a.post_wrap - 1)), w);
 #pragma unroll
-                for (int k = 0; k < 8; ++k) h[j][k] = h[j][k] * inv * (a.w_add == 0.f ? (double)w[k] : (double)w[k] + (double)a.w_add);
+                for (int k = 0; k < 8; ++k) h[j][k] = divided(h[j][k], root) * (a.w_add == 0.0 ? (double)w[k] : (double)w[k] + a.w_add);
             }
         }
     }
@@ -207,15 +225,15 @@ __global__ void __launch_bounds__(TPR < 256 ? 256 : TPR) block_norm_kernel(const
     for (int j = 0; j < NV; ++j) {
         const int i = tid + j * TPR;
         const bool on = row && i < n8;
-        if (a.bs != 1.f) {
+        if (a.bs != 1.0) {
 #pragma unroll
-            for (int k = 0; k < 8; ++k) h[j][k] *= (double)a.bs;
+            for (int k = 0; k < 8; ++k) h[j][k] *= a.bs;
         }
         if (on && a.residual != nullptr) {
             float v[8];
             load8(static_cast<const T *>(a.residual) + m * a.K + i * 8, v);
 #pragma unroll
-            for (int k = 0; k < 8; ++k) v[k] = as_stored((float)fma((double)a.rs, (double)v[k], h[j][k]), (const T *)nullptr);
+            for (int k = 0; k < 8; ++k) v[k] = as_stored((float)fma(a.rs, (double)v[k], h[j][k]), (const T *)nullptr);
             store8(static_cast<T *>(a.residual_out) + m * a.K + i * 8, v);
 #pragma unroll
             for (int k = 0; k < 8; ++k) h[j][k] = (double)v[k];
@@ -226,14 +244,14 @@ __global__ void __launch_bounds__(TPR < 256 ? 256 : TPR) block_norm_kernel(const
 #pragma unroll
             for (int k = 0; k < 8; ++k) {
                 s2 = fma(h[j][k], h[j][k], s2);
-                h[j][k] *= (double)w[k] + (double)a.w_add;
+                h[j][k] *= (double)w[k] + a.w_add;
             }
         }
 #pragma unroll
         for (int k = 0; k < 8; ++k) top = fmax(top, fabs(h[j][k])), odd = fma(h[j][k], 0.0, odd);
     }
     double inv = 1.0;
-    if (a.pre != nullptr) inv = over_root(fma(row_reduce<Sum, TPR>(s2, part[1]), a.over_k, (double)a.eps));
+    if (a.pre != nullptr) inv = over_root(fma(row_reduce<Sum, TPR>(s2, part[1]), a.over_k, a.eps));
     if (a.q != nullptr) top = row_reduce<Top, TPR>(odd == 0.0 ? top : INFINITY, part[2]);
     const bool fine = top < INFINITY;
     const double mul = 127.0 / top;
@@ -312,7 +330,7 @@ extern "C" int sx_block_norm_int8(const sx_block_norm *p, int64_t M, int64_t K, 
     const int64_t g = n.group;
     SX_CHECK(g == 0 || g == K || (g >= 8 && g <= 512 && (g & (g - 1)) == 0 && K % g == 0), "group = ", g, ", expected 0, K or a power of two, 8..512, that divides K = ", K);
     SX_CHECK(n.post_len == 0 || n.post_len == K || n.post_len == g, "post_len = ", n.post_len, ", expected K or the group");
-    SX_CHECK(std::isfinite(n.eps) && n.eps >= 0.f && std::isfinite(n.w_add) && std::isfinite(n.residual_scale) && std::isfinite(n.branch_scale),
+    SX_CHECK(std::isfinite(n.eps) && n.eps >= 0.0 && std::isfinite(n.w_add) && std::isfinite(n.residual_scale) && std::isfinite(n.branch_scale),
              "eps = ", n.eps, ", w_add = ", n.w_add, ", residual_scale = ", n.residual_scale, ", branch_scale = ", n.branch_scale);
     SX_CHECK(aligned(n.x, 16) && aligned(n.post, 16) && aligned(n.gate, 16) && aligned(n.residual, 16) && aligned(n.pre, 16) && aligned(n.residual_out, 16) &&
                  aligned(n.y, 16) && aligned(n.q, 8) && aligned(n.scale, 4),

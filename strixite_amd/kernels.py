@@ -732,7 +732,7 @@ def moe_router_scored(logits, E, k, score="sigmoid", bias=None, groups=1, top_gr
 # ---------------- 8-bit integer activations and linear ----------------
 
 GATES = {"none": GATE_NONE, "silu": GATE_SILU, "sigmoid": GATE_SIGMOID}
-_NORM = struct.Struct("@9P4qi4f4x").pack  # sx_block_norm as bytes
+_NORM = struct.Struct("@9P4qi4d").pack  # sx_block_norm as bytes
 
 
 def block_norm_int8(x, post=None, gate=None, residual=None, pre=None, eps=1e-6, w_add=0.0, group=None, gate_act="none",

@@ -183,6 +183,28 @@ def test_block_norm_ties_and_rows_without_a_scale():
     assert y[1].isnan().all() and torch.isfinite(y[0]).all() and (y[3] == 0).all()
 
 
+def test_block_norm_ties_are_those_of_the_formula_in_64_bits():
+    """Few distinct values and no residual between the norm and the codes, so that products stand on a border between two codes:
+    the rounding of x / root says which. The squares' sum is exact in 64 bits, so every order of adding gives the same root (the mean is
+    the sum times the rounded 1 / K)."""
+    for M, K, group, gated, pre, seed in [(512, 4096, 0, False, False, 1), (512, 1024, 0, False, True, 2), (256, 1024, 0, True, False, 3),
+                                          (256, 2048, 64, False, False, 4), (256, 512, 512, True, True, 5), (512, 2560, 0, False, False, 6)]:
+        g = gen(seed)
+        draw = lambda *shape: (torch.randint(-12, 13, shape, generator=g, device="cuda").float() / 8).bfloat16()
+        x, post = draw(M, K), draw(K) + 2
+        gate, w = draw(M, K) if gated else None, draw(K) + 2 if pre else None
+        q, _, _ = kx.block_norm_int8(x, post, gate, None, w, eps=1e-6, group=group or None, gate_act="none")
+        h = x.double().cpu().view(M, -1, group or K)
+        mean = h.square().sum(2, keepdim=True) * (1.0 / (group or K)) + 1e-6
+        root = torch.tensor([math.sqrt(v) for v in mean.flatten().tolist()], dtype=torch.float64).view(mean.shape)  # the nearest; torch's here is not always
+        h = (h / root).flatten(1) * post.double().cpu()
+        h = h * gate.double().cpu() if gated else h
+        h = h * w.double().cpu() if pre else h
+        n = h * 127.0 / h.abs().amax(1, keepdim=True)
+        assert ((n - n.floor() - 0.5).abs() < 1e-12).any(), "no product near a border"
+        assert torch.equal(q.cpu(), torch.round(n).to(torch.int8)), (M, K, group, gated, pre)
+
+
 def test_block_norm_streams_and_graphs():
     g = gen(4)
     x, w = torch.randn(40, 2560, device="cuda", generator=g).to(BF), torch.randn(2560, device="cuda", generator=g).to(BF)
