@@ -8,13 +8,14 @@
 // 32 heads of 128) and its four waves share a chunk: wave w holds a quarter of the state's rows in registers, multiplies K
 // and Q with them for all 64 tokens, and has a quarter of the tokens after that. What passes between the waves (sums of K S
 // and Q S, V - e^G K S, U) goes through LDS, three barriers a chunk. The latency of that chain is what bounds one
-// sequence: 8192 tokens, 32 heads of 128: 94 + 240 us, 1.9 us a chunk (the matrix unit busy 0.15 of it; 1.2 us without any loads,
+// sequence: 8192 tokens, 32 heads of 128: 96 + 254 us, 2.0 us a chunk (the matrix unit busy 0.16 of it; 1.2 us without any loads,
 // which are 100 KB a chunk and compute unit).
 //
 // Operands: a result of the matrix unit has four consecutive rows a lane, an operand eight consecutive values of a row. The
 // rows of two result tiles are dealt out so that a lane's four of the one and four of the other are eight consecutive
 // ones: row 4 g + r of tile s stands for 8 g + 4 s + r. So the state, V - e^G K S and U become operands where they are.
-// FP32 values enter as three BF16 terms, which together are the value (P U, which only the BF16 output sees: two).
+// FP32 values enter as three BF16 terms, which together are the value; of a product of two such values the six largest of the nine
+// products are taken (what is left is under 2^-22 of it).
 //
 // Tokens that are no numbers: a triangular product would carry them to the tokens before them in the chunk. They are taken
 // out and everything from them on (a value's: in its column) is NaN, as the rule has it.
@@ -28,7 +29,7 @@ namespace {
 
 constexpr int kC = 64, kPitch = kC + 4;
 constexpr int kBlocksT = 6;  // (row tile, pair of column tiles) with anything in it: 1, 1, 2, 2
-constexpr int64_t kTBytes = kBlocksT * 3 * 1024, kPBytes = kBlocksT * 2 * 1024, kHeadBytes = kTBytes + kPBytes + 1024;
+constexpr int64_t kTBytes = kBlocksT * 3 * 1024 /* BF16 terms */, kPBytes = kBlocksT * 2 * 1024, kHeadBytes = kTBytes + kPBytes + 1024;
 
 __host__ __device__ constexpr int block_of(int ti, int p) { return ti < 2 ? ti : 2 * (ti - 1) + p; }
 
@@ -213,13 +214,13 @@ __global__ void __launch_bounds__(256, 4) delta_prepare_kernel(const Args a, con
         float t8[8], p8[8];
 #pragma unroll
         for (int j = 0; j < 8; ++j) t8[j] = Tm[at + j], p8[j] = P[at + j];
-        bf16x8 ts[3], ps[2];
+        bf16x8 ts[3];
         split(t8, ts);
-        split(p8, ps);
 #pragma unroll
         for (int s = 0; s < 3; ++s) *reinterpret_cast<bf16x8 *>(head + (blk * 3 + s) * 1024 + lane * 16) = ts[s];
 #pragma unroll
-        for (int s = 0; s < 2; ++s) *reinterpret_cast<bf16x8 *>(head + kTBytes + (blk * 2 + s) * 1024 + lane * 16) = ps[s];
+        for (int s = 0; s < 2; ++s)
+            *reinterpret_cast<f32x4 *>(head + kTBytes + (blk * 2 + s) * 1024 + lane * 16) = f32x4{p8[4 * s], p8[4 * s + 1], p8[4 * s + 2], p8[4 * s + 3]};
     }
     if (h % a.rep != 0) return;
     // The key head's K and Q, their rows in the order of the tiles, and K^T: row dk, eight tokens a lane. (Read from the caller's rows,
@@ -283,7 +284,8 @@ struct StateChunk {
 };
 // And an output wave.
 struct OutChunk {
-    bf16x8 Q[4], P[2][2];
+    bf16x8 Q[4];
+    f32x4 P[2][2];  // FP32: as three terms they are half as many bytes again, and the scan of 8192 tokens took 274 us for 255
     f32x4 out;
 };
 
@@ -311,8 +313,8 @@ template <int DK>
 __global__ void __launch_bounds__(512) delta_scan_kernel(const Args a, const Work w, int pairs8) {
     constexpr int TS = DK / 64;  // tiles of the state's rows a state wave has
     __shared__ __attribute__((aligned(16))) f32x4 xs[4][4][64];  // [wave][tile]: K S over the wave's rows
-    __shared__ __attribute__((aligned(16))) u32x4 ss[4][2][64];  // the state's rows of each wave as operands
-    __shared__ __attribute__((aligned(16))) u32x2 rs[3][4][64], us[2][4][64], ks[3][4][64];
+    __shared__ __attribute__((aligned(16))) u32x4 ss[4][3][64];  // the state's rows of each wave as operands
+    __shared__ __attribute__((aligned(16))) u32x2 rs[3][4][64], us[3][4][64], ks[3][4][64];
     __shared__ int poison[16];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wt = wave & 3, n16 = lane & 15, g4 = lane >> 4;
     const int pair = blockIdx.x % pairs8, b = pair / a.Hv, h = pair % a.Hv, hk = h / a.rep;
@@ -404,7 +406,8 @@ __global__ void __launch_bounds__(512) delta_scan_kernel(const Args a, const Wor
             for (int j = 0; j < 4; ++j) s8[j] = S[0][j], s8[4 + j] = TS == 2 ? S[TS - 1][j] : 0.f;
             bf16x8 so[3];
             split(s8, so);
-            ss[wave][0][lane] = __builtin_bit_cast(u32x4, so[0]), ss[wave][1][lane] = __builtin_bit_cast(u32x4, so[1]);
+#pragma unroll
+            for (int i = 0; i < 3; ++i) ss[wave][i][lane] = __builtin_bit_cast(u32x4, so[i]);
             f32x4 X[4];
 #pragma unroll
             for (int t = 0; t < 4; ++t) X[t] = mfma(now.K[t], so[2], zero);
@@ -459,7 +462,7 @@ __global__ void __launch_bounds__(512) delta_scan_kernel(const Args a, const Wor
 #pragma unroll
             for (int i = 0; i < 3; ++i) put(ks, i, uk);
 #pragma unroll
-            for (int i = 0; i < 2; ++i) put(us, i, uu);
+            for (int i = 0; i < 3; ++i) put(us, i, uu);
             lds_barrier();
 #pragma unroll
             for (int t = 0; t < TS; ++t)
@@ -504,7 +507,7 @@ __global__ void __launch_bounds__(512) delta_scan_kernel(const Args a, const Wor
             for (int p = 0; p < PAIRS; ++p) {
                 const uint8_t *blk = heads + (int64_t)c * a.Hv * kHeadBytes + kTBytes + block_of(wt, p) * 2048;
 #pragma unroll
-                for (int i = 0; i < 2; ++i) o.P[p][i] = __builtin_bit_cast(bf16x8, load16(blk, at16 + i * 1024));
+                for (int i = 0; i < 2; ++i) o.P[p][i] = __builtin_bit_cast(f32x4, load16(blk, at16 + i * 1024));
             }
         };
         auto chunk = [&](int c, OutChunk &now) __attribute__((always_inline)) {
@@ -512,6 +515,7 @@ __global__ void __launch_bounds__(512) delta_scan_kernel(const Args a, const Wor
             f32x4 Y = zero, Y2 = zero;
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
+                Y2 = mfma(now.Q[i], __builtin_bit_cast(bf16x8, ss[i][2][lane]), Y2);
                 Y2 = mfma(now.Q[i], __builtin_bit_cast(bf16x8, ss[i][1][lane]), Y2);
                 Y = mfma(now.Q[i], __builtin_bit_cast(bf16x8, ss[i][0][lane]), Y);
             }
@@ -520,14 +524,22 @@ __global__ void __launch_bounds__(512) delta_scan_kernel(const Args a, const Wor
 #pragma unroll
             for (int r = 0; r < 4; ++r) O[r] = now.out[r] * (Y[r] + Y2[r]);
             fetch_q(c + 1, now);
+            bf16x8 P[PAIRS][3];
+#pragma unroll
+            for (int p = 0; p < PAIRS; ++p) {
+                float p8[8];
+#pragma unroll
+                for (int j = 0; j < 4; ++j) p8[j] = now.P[p][0][j], p8[4 + j] = now.P[p][1][j];
+                split(p8, P[p]);
+            }
             lds_barrier();
             const int from = poison[n16] - c * kC, left = s.n - c * kC;
 #pragma unroll
             for (int p = 0; p < PAIRS; ++p) {
-                const bf16x8 u0 = pair_of(us[0], p), u1 = pair_of(us[1], p);
-                O2 = mfma(now.P[p][1], u0, O2);
-                O = mfma(now.P[p][0], u0, O);
-                O2 = mfma(now.P[p][0], u1, O2);
+                const bf16x8 u0 = pair_of(us[0], p), u1 = pair_of(us[1], p), u2 = pair_of(us[2], p);
+                O2 = mfma(P[p][2], u0, O2), O = mfma(P[p][1], u0, O);
+                O2 = mfma(P[p][1], u1, O2), O = mfma(P[p][0], u1, O);
+                O2 = mfma(P[p][0], u2, O2), O = mfma(P[p][0], u0, O);
             }
             fetch_p(c + 1, now);
             uint8_t *oc = reinterpret_cast<uint8_t *>(op + (int64_t)c * kC * a.o_t);
