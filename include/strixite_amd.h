@@ -427,7 +427,8 @@ int sx_linear_int8(const int8_t *x, const float *x_scale, const sx_int8_view *w,
  * sigmoid(b); without (both null) g = a (0 or less; -1e4 and less all say: forget everything) and beta = b.
  * Sequence b's tokens are rows starts[b] .. starts[b + 1] - 1 (device int32 [batch + 1]); its state is number slot[b] (null: b)
  * of `slots` states, state_slot floats apart, each [heads, key_dim, dim] dense. key_dim 64 or 128, dim a multiple of 16 up to
- * 1024, batch up to 1024. States, sums and norms are FP32; products of states and corrections are exact in BF16 thirds. A sequence
+ * 1024, batch up to 1024. States, sums and norms are FP32. A state enters all its products whole, as three BF16 terms; of a
+ * product of two FP32 values (corrections, products of tokens) the six largest of nine products of such terms are taken. A sequence
  * whose run of tokens is impossible (negative, over the call's limit, outside T) is left alone; one with tokens whose slot is none
  * of the states, or (where states are written) is another such sequence's too, keeps its state and its rows come out NaN. err
  * (nullable) is then {1, the first row or the slot, the sequence}. Sequences of no tokens need no slot. Rows behind

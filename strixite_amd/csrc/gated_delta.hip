@@ -268,7 +268,7 @@ __global__ void __launch_bounds__(64 * W) delta_verify_kernel(const VerifyArgs v
 #pragma unroll
             for (int t = 0; t < NT; ++t) {
                 X[t] = mfma(K[t], o[p], X[t]);
-                if (p < 2) Y[t] = mfma(Q[t], o[p], Y[t]);
+                Y[t] = mfma(Q[t], o[p], Y[t]);
             }
     }
 #pragma unroll
@@ -334,13 +334,14 @@ __global__ void __launch_bounds__(64 * W) delta_verify_kernel(const VerifyArgs v
             O[t][r] = grow[i] * rq[i] * Y[t][r];
         }
     if (all_fine) {
-        // P U with both in two BF16 terms (2^-16), one product of 32 tokens a pair of tiles
+        // P U with both in three BF16 terms, of whose products the six largest are taken (what is left is under 2^-22), one of 32
+        // tokens a pair of tiles
 #pragma unroll
         for (int p = 0; p < (NT + 1) / 2; ++p) {
             float u8[8];
 #pragma unroll
             for (int j = 0; j < 4; ++j) u8[j] = U[2 * p][j], u8[4 + j] = 2 * p + 1 < NT ? U[(2 * p + 1) % NT][j] : 0.f;
-            bf16x8 ub[2];
+            bf16x8 ub[3];
             split(u8, ub);
 #pragma unroll
             for (int t = 2 * p; t < NT; ++t) {
@@ -349,8 +350,11 @@ __global__ void __launch_bounds__(64 * W) delta_verify_kernel(const VerifyArgs v
                 f32x4 hi = {0.f, 0.f, 0.f, 0.f};
                 if (2 * p + 1 < NT) hi = *reinterpret_cast<const f32x4 *>(prow + 16);
                 const float p8[8] = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
-                bf16x8 pb[2];
+                bf16x8 pb[3];
                 split(p8, pb);
+                O[t] = mfma(pb[2], ub[0], O[t]);
+                O[t] = mfma(pb[1], ub[1], O[t]);
+                O[t] = mfma(pb[0], ub[2], O[t]);
                 O[t] = mfma(pb[1], ub[0], O[t]);
                 O[t] = mfma(pb[0], ub[1], O[t]);
                 O[t] = mfma(pb[0], ub[0], O[t]);

@@ -96,7 +96,8 @@ __device__ __forceinline__ uint32_t tops(uint32_t lo, uint32_t hi) { return __bu
 
 // Eight FP32 values as N BF16 operands: each takes the next eight leading bits, so three of them are the value itself
 // (24 bits; what is left after each is exact). Products of such operands with BF16 values are exact, their sums FP32:
-// a state meets the matrix unit without being rounded.
+// a state meets the matrix unit without being rounded, for corrections and outputs alike. Of a product of two FP32 values the six
+// largest of nine products are taken.
 template <int N>
 __device__ __forceinline__ void split(const float (&x)[8], bf16x8 (&o)[N]) {
     float r[8];

@@ -27,7 +27,8 @@ def through(x, form):
 
 # ---------------- sums that cancel ----------------
 
-@pytest.mark.parametrize("Dk,Dv,n,form", [(128, 128, 16, "steps"), (128, 128, 40, "prompt"), (128, 64, 150, "prompt"), (64, 64, 64, "prompt")])
+@pytest.mark.parametrize("Dk,Dv,n,form", [(128, 128, 16, "steps"), (128, 128, 40, "prompt"), (128, 64, 150, "prompt"), (64, 64, 64, "prompt"),
+                                          (128, 128, 6, "verify"), (128, 64, 24, "verify"), (64, 128, 64, "verify")])
 def test_an_overwritten_value_leaves_nothing_of_itself(Dk, Dv, n, form):
     """The state holds one key's value of 2^12; the first token writes zero there (beta 1, no decay), the others' keys and values are
     small change, and every query is that key. An output is the state's large share less the first token's, both FP32: each is a
