@@ -429,10 +429,10 @@ int sx_linear_int8(const int8_t *x, const float *x_scale, const sx_int8_view *w,
  * of `slots` states, state_slot floats apart, each [heads, key_dim, dim] dense. key_dim 64 or 128, dim a multiple of 16 up to
  * 1024, batch up to 1024. States, sums and norms are FP32. A state enters all its products whole, as three BF16 terms; of a
  * product of two FP32 values (corrections, products of tokens) the six largest of nine products of such terms are taken. A sequence
- * whose run of tokens is impossible (negative, over the call's limit, outside T) is left alone; one with tokens whose slot is none
- * of the states, or (where states are written) is another such sequence's too, keeps its state and its rows come out NaN. err
- * (nullable) is then {1, the first row or the slot, the sequence}. Sequences of no tokens need no slot. Rows behind
- * starts[batch] are left as they are. */
+ * whose run of tokens is impossible (negative, over the call's limit, outside T, or behind a start that is below the one before it) is
+ * left alone; one with tokens whose slot is none of the states, or (where states are written) is another such sequence's too, keeps
+ * its state and its rows come out NaN. err (nullable) is then {1, the first row or the slot, the sequence}. Sequences of no tokens
+ * need no slot. Rows behind starts[batch] are left as they are. */
 typedef struct sx_delta {
     sx_head_rows q, k, v;
     const void *a, *b;

@@ -29,7 +29,9 @@ struct Args {
 };
 
 // A sequence's rows t0 .. t0 + n - 1 and its state. run false: its words are impossible, nothing of it is touched. ok
-// false: its rows are NaN and its state stays as it is.
+// false: its rows are NaN and its state stays as it is. Starts that fall make every sequence from the falling one on impossible: what
+// lies behind could be another's rows, and two blocks that write one row, or two sequences' chunks in one place of a prompt's
+// workspace, would race.
 struct Seq {
     int t0, n, slot;
     bool run, ok;
@@ -40,14 +42,17 @@ struct Seq {
 __device__ __forceinline__ Seq sequence(const int32_t *starts, const int32_t *slots, int b, int B, int T, int max_len, int states, bool alone) {
     const int t0 = starts[b], t1 = starts[b + 1];
     const int slot = slots != nullptr ? slots[b] : b;
-    Seq s{t0, t1 - t0, slot, t0 >= 0 && t1 >= t0 && t1 <= T && t1 - t0 <= max_len, slot >= 0 && slot < states};
-    if (!s.run) s.n = 0;
-    if (alone && slots != nullptr && s.ok) {
-        bool twice = false;
-        for (int j = threadIdx.x & 63; j < B; j += 64)
-            if (j != b && slots[j] == slot && starts[j + 1] > starts[j]) twice = true;
-        if (__any(twice)) s.ok = false;
+    Seq s{t0, (int)((uint32_t)t1 - (uint32_t)t0), slot, t0 >= 0 && t1 >= t0 && t1 <= T && t1 - t0 <= max_len, slot >= 0 && slot < states};
+    const bool others = alone && slots != nullptr;
+    bool twice = false, falls = false;
+    for (int j = threadIdx.x & 63; j < (others ? B : b); j += 64) {
+        const int at = starts[j], next = starts[j + 1];
+        if (j < b && next < at) falls = true;
+        if (others && j != b && slots[j] == slot && next > at) twice = true;
     }
+    if (__any(falls)) s.run = false;
+    if (__any(twice)) s.ok = false;
+    if (!s.run) s.n = 0;
     return s;
 }
 

@@ -51,7 +51,7 @@ struct Work {
 template <int DK>
 constexpr int kKeyBytes = DK * kC * 2;  // of one of the three
 
-// A sequence's chunks take slots starts[b] / 64 + b on: enough for a last chunk that is not full.
+// A sequence's chunks take slots starts[b] / 64 + b on: enough for a last chunk that is not full, where starts rise.
 __device__ __forceinline__ int64_t first_slot(int t0, int b) { return t0 / kC + b; }
 
 // The token that result row 4 g + r of tile ti stands for, and that of operand row m.
@@ -67,29 +67,33 @@ __global__ void __launch_bounds__(256, 4) delta_prepare_kernel(const Args a, con
     __shared__ double path[kC];
     __shared__ float rk[kC], rq[kC], beta[kC];
     __shared__ uint64_t use_mask, key_mask;  // tokens that count; those whose key does, whatever this head's gates are
-    __shared__ int found;
+    __shared__ int found, falls;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), n16 = lane & 15, g4 = lane >> 4;
     const int64_t slot = blockIdx.x / a.Hv;
     const int h = blockIdx.x % a.Hv, hk = h / a.rep;
-    // the sequence whose chunk this is: at most one (of possible starts)
+    // the sequence whose chunk this is: the lowest whose words say so, if starts have not fallen before it. Up to there they only
+    // rise, so it is the only one; sequences behind a falling start are impossible (sequence())
     int b = 0, t0 = 0, n = 0;
     auto mine_is = [&](int i) {
         t0 = a.starts[i];
         const int t1 = a.starts[i + 1];
         const int64_t f = first_slot(t0, i);
+        if (t0 < 0 || t1 <= t0 || t1 > a.T || t1 - t0 > a.max_len || slot < f) return false;
         n = t1 - t0 - (int)(slot - f) * kC;
-        return t0 >= 0 && t1 > t0 && t1 <= a.T && t1 - t0 <= a.max_len && slot >= f && n > 0;
+        return n > 0;
     };
     if (a.B == 1) {
         if (!mine_is(0)) return;
     } else {
-        if (threadIdx.x == 0) found = -1;
+        if (threadIdx.x == 0) found = falls = a.B;
         __syncthreads();
-        for (int i = threadIdx.x; i < a.B; i += 256)
-            if (mine_is(i)) found = i;
+        for (int i = threadIdx.x; i < a.B; i += 256) {
+            if (a.starts[i + 1] < a.starts[i]) atomicMin(&falls, i);
+            if (mine_is(i)) atomicMin(&found, i);
+        }
         __syncthreads();
         b = found;
-        if (b < 0) return;
+        if (b >= falls) return;
         mine_is(b);
     }
     const int64_t row0 = t0 + (slot - first_slot(t0, b)) * kC;

@@ -49,3 +49,59 @@ def test_an_overwritten_value_leaves_nothing_of_itself(Dk, Dv, n, form):
     d = (out.double() - ref).norm(dim=2)
     print(form, "worst / u32 of the value:", float(((d - U16 * ref.norm(dim=2)).clamp(min=0) / big).max() / U32))
     assert (d <= U16 * ref.norm(dim=2) + 32 * U32 * big).all()
+
+
+# ---------------- starts that fall ----------------
+
+def possible(starts, T, most):
+    """The sequences that the contract serves: possible words, and no start before them that falls."""
+    ok, rises = [], True
+    for t0, t1 in zip(starts, starts[1:]):
+        rises = rises and t1 >= t0
+        ok.append(rises and t0 >= 0 and t1 <= T and t1 - t0 <= most)
+    return ok
+
+
+@pytest.mark.parametrize("form", ["steps", "prompt", "verify"])
+@pytest.mark.parametrize("starts", [[200, 400, 0, 200], [0, 300, 50, 350], [0, 60, 40, 100], [0, 5, 3, 8], [10, 0, 16], [0, 64, 64, 63, 127, 140], [50, 60, 20, 80, 90],
+                                    [-7, 9, 20, 15, 30], [0, 9, 2 ** 31 - 1, 20, 40], [0, 12, -2 ** 31, 12, 25]])
+def test_sequences_from_a_falling_start_on_are_left_alone(starts, form):
+    B, T = len(starts) - 1, 400
+    limit = {"steps": 16, "prompt": 400, "verify": 64}[form]
+    x = Tokens([T] + [0] * (B - 1), Hk=1, Hv=2, Dk=64, Dv=64, seed=B)
+    ok, at = possible(starts, T, limit), i32(starts)
+    mask = (2 ** 63 - 1) * torch.ones(T, 1, dtype=torch.int64, device="cuda")  # every token before its own: a chain
+
+    def call(starts, state, out, err):
+        if form != "verify":
+            return kx.gated_delta(x.q, x.k, x.v, x.a, x.b, state, starts, limit, **x.kw(out=out, err=err))
+        _, u, decay, _ = kx.gated_delta_verify(x.q, x.k, x.v, x.a, x.b, state, starts, mask, limit, **x.kw(out=out, err=err))
+        n = starts[1:] - starts[:-1]
+        kx.gated_delta_commit(x.k, u, decay, state, starts, torch.where((n > 0) & (n <= limit), n, 0).to(torch.int32), max_count=limit, slots=x.slots)
+    for again in range(3):
+        state, out, err = x.state.clone(), torch.full((T, 2, 64), 7.0, dtype=BF, device="cuda"), torch.zeros(4, dtype=torch.int32, device="cuda")
+        call(at, state, out, err)
+        want, want_out = x.state.clone(), torch.full_like(out, 7.0)
+        for b in range(B):
+            if ok[b]:  # alone, its words where they were
+                lone = [starts[b]] * (b + 1) + [starts[b + 1]] * (B - b)
+                call(i32(lone), want, want_out, None)
+        assert torch.equal(out, want_out) and torch.equal(state, want)
+        word = err.tolist()
+        assert word[0] == (not all(ok)) and (all(ok) or (not ok[word[2]] and word[1] == starts[word[2]]))
+
+
+def test_many_sequences_with_one_falling_start():
+    B, n = 1000, 20
+    x = Tokens([n] * B, Hk=1, Hv=1, Dk=64, Dv=16, seed=1)
+    clean = x.state.clone()
+    ref, _ = x.run(clean)
+    for at in (1, 255, 256, 700, 999):
+        starts = x.starts.clone()
+        starts[at] = starts[at - 1] - 1
+        state, out = x.state.clone(), torch.full_like(ref, 7.0)
+        kx.gated_delta(x.q, x.k, x.v, x.a, x.b, state, starts, n + 1, **x.kw(out=out))
+        assert torch.equal(out[:(at - 1) * n], ref[:(at - 1) * n]) and (out[(at - 1) * n:] == 7).all()
+        served = [x.slot(b) for b in range(at - 1)]
+        rest = [i for i in range(state.shape[0]) if i not in set(served)]
+        assert torch.equal(state[served], clean[served]) and torch.equal(state[rest], x.state[rest])
