@@ -373,8 +373,9 @@ int sx_moe_router_scored(const void *logits, int64_t ld, int64_t M, int64_t E, i
  * stays if it is the row's largest logit (ties: the lowest place), which is the token otherwise. Probabilities and sums are FP64.
  * tokens [batch, max_rows]: the drafts that stay, the token, then -1; count: how many; status 0. A row that counts and holds NaN or
  * no finite largest logit, a draft outside the vocabulary or a temperature that is not finite: status 1 + the row, count and tokens
- * the drafts before it. Impossible starts: status -1, count 0. ws: sx_mtp_accept_sampled_workspace_bytes, 16-byte aligned, never read
- * before it is written; one per stream. T up to 32767, batch up to 1024. */
+ * the drafts before it. Impossible starts (negative, over max_rows, outside T, or behind a start that is below the one before it):
+ * status -1, count 0. ws: sx_mtp_accept_sampled_workspace_bytes, 16-byte aligned, never read before it is written; one per
+ * stream. T up to 32767, batch up to 1024. */
 int sx_mtp_accept_sampled_workspace_bytes(int64_t T, int64_t batch, int64_t n_valid, int64_t n_draft, size_t *bytes);
 int sx_mtp_accept_sampled(const void *logits, int64_t ld, int64_t T, int64_t n_valid, const void *draft_logits, int64_t draft_ld,
                           int64_t n_draft, int act, const int32_t *drafts, const int32_t *starts, int64_t batch, int64_t max_rows,

@@ -86,9 +86,11 @@ __device__ __forceinline__ void load_run(const uint16_t *p, int left, float (&x)
     }
 }
 
+// Sequence b's own words. Where starts fall, that sequence and all behind it are impossible too: their rows could be another's,
+// whose temperature a row's sums are taken at.
 __device__ __forceinline__ bool usable(const Args &a, int b, int &t0, int &n) {
     t0 = a.starts[b];
-    n = a.starts[b + 1] - t0;
+    n = (int)((uint32_t)a.starts[b + 1] - (uint32_t)t0);
     return t0 >= 0 && n >= 0 && (int64_t)t0 + n <= a.T && n <= a.max_rows;
 }
 
@@ -153,7 +155,7 @@ __device__ __forceinline__ double weight(double y) {
 template <typename T>
 __global__ void __launch_bounds__(kThreads) accept_parts_kernel(const Args a) {
     __shared__ float tops[4];
-    __shared__ int ats[4], owners[4];
+    __shared__ int ats[4], owners[4], fallen[4];
     __shared__ double sums[4];
     const int chunk = blockIdx.x, wave = threadIdx.x >> 6;
     const int64_t row = blockIdx.y % a.T;
@@ -170,13 +172,20 @@ __global__ void __launch_bounds__(kThreads) accept_parts_kernel(const Args a) {
 #pragma unroll
         for (int j = 0; j < 8; ++j) x[8 * i + j] = run[j];
     }
-    int owner = -1;  // the row's sequence; a last row has no draft
-    for (int b = threadIdx.x; b < a.B; b += kThreads) {
-        int t0, n;
-        if (usable(a, b, t0, n) && row >= t0 && row < t0 + n - (draft ? 1 : 0)) owner = b;
+    // the row's sequence (a last row has no draft): the lowest whose words say so, if starts have not fallen before it
+    int owner = a.B, falls = a.B;
+    for (int b0 = threadIdx.x & ~63; b0 < a.B; b0 += kThreads) {
+        const int b = b0 + (threadIdx.x & 63);
+        bool has = false, down = false;
+        if (b < a.B) {
+            int t0, n;
+            has = usable(a, b, t0, n) && row >= t0 && row < t0 + n - (draft ? 1 : 0);
+            down = a.starts[b + 1] < t0;
+        }
+        const uint64_t h = __ballot(has), d = __ballot(down);
+        if (h != 0 && owner == a.B) owner = b0 + __builtin_ctzll(h);
+        if (d != 0 && falls == a.B) falls = b0 + __builtin_ctzll(d);
     }
-    const uint64_t has = __ballot(owner >= 0);
-    owner = has != 0 ? __shfl(owner, __builtin_ctzll(has)) : -1;
     float top = -INFINITY;
     int at = 0x7fffffff;
     bool nan = false;
@@ -186,10 +195,10 @@ __global__ void __launch_bounds__(kThreads) accept_parts_kernel(const Args a) {
         if (x[i] > top) top = x[i], at = first + ((int)threadIdx.x + i / 8 * kThreads) * 8 + i % 8;
     }
     wave_best(top, at);
-    if ((threadIdx.x & 63) == 0) tops[wave] = top, ats[wave] = at, owners[wave] = owner;
+    if ((threadIdx.x & 63) == 0) tops[wave] = top, ats[wave] = at, owners[wave] = owner, fallen[wave] = falls;
     nan = __syncthreads_or(nan);
-    top = tops[0], at = ats[0], owner = max(max(owners[0], owners[1]), max(owners[2], owners[3]));
-    if (owner < 0) return;
+    top = tops[0], at = ats[0], owner = min(min(owners[0], owners[1]), min(owners[2], owners[3]));
+    if (owner >= min(min(fallen[0], fallen[1]), min(fallen[2], fallen[3]))) return;
 #pragma unroll
     for (int w = 1; w < 4; ++w)
         if (tops[w] > top || (tops[w] == top && ats[w] < at)) top = tops[w], at = ats[w];
@@ -246,7 +255,10 @@ struct Rows {
 template <typename T>
 __device__ __forceinline__ void decide(const Args &a, int b, Verdict &v, Rows &rows) {
     int t0, n;
-    const bool ok = usable(a, b, t0, n);
+    bool falls = false;
+    for (int j = threadIdx.x; j < b; j += kDrawThreads) falls |= a.starts[j + 1] < a.starts[j];
+    falls = b > 0 && __syncthreads_or(falls);
+    const bool ok = usable(a, b, t0, n) && !falls;
     if (!ok || n == 0) {
         if (threadIdx.x == 0) v = Verdict{0, 0, 0, 0, 0, ok ? 0 : -1, kNone, 0, 0, 0, 0};
         __syncthreads();
