@@ -425,7 +425,7 @@ int sx_linear_int8(const int8_t *x, const float *x_scale, const sx_int8_view *w,
  * q, k [T, key_heads, key_dim], v [T, heads, dim] BF16; value head h goes with key head h / (heads / key_heads). normalize: k
  * and q are divided by sqrt(sum of squares + 1e-6) first; q is then multiplied by scale. Gates a, b [T, heads] in gate_act, rows
  * a_token and b_token elements apart: with A_log and dt_bias (FP32 [heads]) g = -exp(A_log) softplus(a + dt_bias) and beta =
- * sigmoid(b); without (both null) g = a (0 or less; -1e4 and less all say: forget everything) and beta = b.
+ * sigmoid(b); without (both null) g = a (0 or less) and beta = b. A g of -1e4 or less, -inf too, says: forget everything.
  * Sequence b's tokens are rows starts[b] .. starts[b + 1] - 1 (device int32 [batch + 1]); its state is number slot[b] (null: b)
  * of `slots` states, state_slot floats apart, each [heads, key_dim, dim] dense. key_dim 64 or 128, dim a multiple of 16 up to
  * 1024, batch up to 1024. States, sums and norms are FP32. A state enters all its products whole, as three BF16 terms; of a

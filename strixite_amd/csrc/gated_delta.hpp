@@ -62,16 +62,18 @@ __device__ __forceinline__ void tell(const Seq &s, int b, uint32_t *err) {
     else if (s.n > 0 && !s.ok) report(err, (uint32_t)s.slot, (uint32_t)b);
 }
 
-// The logarithm of token t's decay for head h, and the share of its correction that is written.
+// The logarithm of token t's decay for head h, and the share of its correction that is written. A decay of -1e4 and less, -inf too,
+// is a full reset: e to it is 0, and sums and differences of it stay numbers.
 __device__ __forceinline__ void gates(const Args &a, int64_t t, int h, float &g, float &beta) {
     const float x = a.f32_gates ? static_cast<const float *>(a.a)[t * a.a_t + h] : bf16_to_f32(static_cast<const uint16_t *>(a.a)[t * a.a_t + h]);
     const float y = a.f32_gates ? static_cast<const float *>(a.b)[t * a.b_t + h] : bf16_to_f32(static_cast<const uint16_t *>(a.b)[t * a.b_t + h]);
-    g = x < -1e4f ? -1e4f : x, beta = y;  // a full reset too: sums of it stay numbers
+    g = x, beta = y;
     if (a.A_log != nullptr) {
         const float z = x + a.dt_bias[h];
         g = -expf(a.A_log[h]) * (z > 20.f ? z : log1pf(expf(z)));
         beta = 1.f / (1.f + expf(-y));
     }
+    g = g < -1e4f ? -1e4f : g;
 }
 
 __device__ __forceinline__ void unpack8(u32x4 u, float (&v)[8]) {

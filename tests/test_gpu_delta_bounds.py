@@ -1,11 +1,14 @@
-"""The gated delta rule on cuda:0 where its sums cancel, in its three forms: steps, prompts in chunks, drafted trees with their commit.
+"""The gated delta rule on cuda:0 where its sums cancel, where starts fall and where a gate forgets everything: the three forms (steps,
+prompts in chunks, drafted trees with their commit) give one answer.
 
 Tolerances as in test_gpu_delta.py (u16 = 2^-8, u32 = 2^-24; c roundings a step)."""
+import math
+
 import pytest
 import torch
 
 from strixite_amd import kernels as kx
-from tests.test_gpu_delta import BF, U16, U32, Tokens, gen, i32
+from tests.test_gpu_delta import BF, U16, U32, Tokens, close, gen, i32
 
 pytestmark = pytest.mark.gpu
 
@@ -105,3 +108,51 @@ def test_many_sequences_with_one_falling_start():
         served = [x.slot(b) for b in range(at - 1)]
         rest = [i for i in range(state.shape[0]) if i not in set(served)]
         assert torch.equal(state[served], clean[served]) and torch.equal(state[rest], x.state[rest])
+
+
+# ---------------- gates that forget everything ----------------
+
+class Resets(Tokens):
+    def gates(self):
+        g, beta = super().gates()
+        return g.clamp(min=-100.0), beta  # e^-100 of a state is nothing beside u32 |v|, and the tolerance stays a number
+
+
+@pytest.mark.parametrize("form,lens", [("steps", [16, 9]), ("prompt", [40, 90, 6]), ("prompt", [16, 9]), ("verify", [24, 9]), ("verify", [64, 6])])
+@pytest.mark.parametrize("how", ["-inf", "-1e4", "-3e38", "a = inf", "overflow"])
+def test_full_resets(form, lens, how):
+    x = Resets(lens, Hk=2, Hv=4, raw=how[0] == "-", f32=how != "a = inf", seed=len(lens) + lens[0])
+    at = [0, 3, 7, lens[0] - 1, lens[0] + 5]
+    if how == "overflow":  # exp(A_log) softplus is past FP32's largest
+        x.A_log[1] = 88.0
+        x.dt_bias[:] = 0.0
+        x.a[:, 1] = 0.5 * x.a[:, 1].abs()  # every token of this head
+        for t in at:
+            x.a[t, 1] = 1000.0
+    else:
+        for t in at:
+            x.a[t, 1:3] = math.inf if how == "a = inf" else float(how)
+    ref, states, _, _, tol, stol = x.rule(parents=chains(lens) if form == "verify" else None, chunked=form != "steps")
+    out, got = through(x, form)
+    close(out, ref, tol, U16, "out")
+    for b, n in enumerate(lens):
+        want, e = x.nodes[b][-1]
+        mine = got[x.slot(b)]
+        assert torch.isfinite(mine).all() and (mine.double() - want).norm() <= 40 * U32 * want.norm(), b
+
+
+@pytest.mark.parametrize("Dk", [64, 128])
+def test_a_reset_is_the_same_token_in_every_form(Dk):
+    """A token that forgets everything and one behind it: the three forms' outputs and states, against each other."""
+    x = Tokens([12, 3], Hk=1, Hv=2, Dk=Dk, Dv=64, seed=Dk)
+    x.a[5, 0] = math.inf
+    x.a[13] = math.inf
+    (o1, s1), (o2, s2), (o3, s3) = (through(x, f) for f in ("steps", "prompt", "verify"))
+    for o, s in ((o2, s2), (o3, s3)):
+        assert torch.isfinite(o).all() and torch.isfinite(s).all()
+        assert (o.double() - o1.double()).norm() <= 2 * U16 * o1.double().norm() and (s.double() - s1.double()).norm() <= 40 * U32 * s1.double().norm()
+    # what came before the reset is gone: a state of other numbers ends as this one does
+    y = x.state.clone()
+    x.state = torch.where(torch.arange(x.state.shape[0], device="cuda")[:, None, None, None] == x.slot(1), -3 * y, y)
+    for f, s in zip(("steps", "prompt", "verify"), (s1, s2, s3)):
+        assert torch.equal(through(x, f)[1][x.slot(1)], s[x.slot(1)]), f
