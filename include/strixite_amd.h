@@ -423,7 +423,8 @@ int sx_linear_int8(const int8_t *x, const float *x_scale, const sx_int8_view *w,
  * kernels/gdn.hpp runs chains of tokens). A state S [key_dim, dim] FP32 for each of `heads` value heads; for each token
  *   S <- e^g S;  u = beta (v - S^T k);  S <- S + k u^T;  o = S^T q.
  * q, k [T, key_heads, key_dim], v [T, heads, dim] BF16; value head h goes with key head h / (heads / key_heads). normalize: k
- * and q are divided by sqrt(sum of squares + 1e-6) first; q is then multiplied by scale. Gates a, b [T, heads] in gate_act, rows
+ * and q are divided by sqrt(sum of squares + 1e-6) first; q is then multiplied by scale. A key whose FP32 sum of squares is not
+ * finite is no number, normalized or not, and so is such a query where it is normalized. Gates a, b [T, heads] in gate_act, rows
  * a_token and b_token elements apart: with A_log and dt_bias (FP32 [heads]) g = -exp(A_log) softplus(a + dt_bias) and beta =
  * sigmoid(b); without (both null) g = a (0 or less) and beta = b. A g of -1e4 or less, -inf too, says: forget everything.
  * Sequence b's tokens are rows starts[b] .. starts[b + 1] - 1 (device int32 [batch + 1]); its state is number slot[b] (null: b)

@@ -92,7 +92,7 @@ __global__ void __launch_bounds__(256) delta_step_kernel(const Args a) {
 #pragma unroll
             for (int c = 0; c < 4; ++c) sk[c] = fmaf(S[r][c], k[r], sk[c]), sq[c] = fmaf(S[r][c], q[r], sq[c]);
         kk = sum_slices(kk), qq = sum_slices(qq), kq = sum_slices(kq);
-        const float rk = a.normalize ? 1.f / sqrtf(kk + kNormEps) : 1.f, rq = (a.normalize ? 1.f / sqrtf(qq + kNormEps) : 1.f) * a.scale;
+        const float rk = key_scale(a, kk), rq = query_scale(a, qq);
         const float fade = expf(g);
         float o[4];
         f32x4 u;
@@ -205,8 +205,7 @@ __global__ void __launch_bounds__(64 * W) delta_verify_kernel(const VerifyArgs v
         for (int j = 0; j < 8; ++j) kk = fmaf(x[j], x[j], kk), qq = fmaf(y[j], y[j], qq);
         kk = sum_chunks<kRow>(kk), qq = sum_chunks<kRow>(qq);
         if (id % kRow == 0) {
-            rk[row] = a.normalize ? 1.f / sqrtf(kk + kNormEps) : 1.f;
-            rq[row] = (a.normalize ? 1.f / sqrtf(qq + kNormEps) : 1.f) * a.scale;
+            rk[row] = key_scale(a, kk), rq[row] = query_scale(a, qq);
         }
     }
     if (wave == 0) {

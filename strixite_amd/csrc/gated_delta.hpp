@@ -76,6 +76,15 @@ __device__ __forceinline__ void gates(const Args &a, int64_t t, int h, float &g,
     g = g < -1e4f ? -1e4f : g;
 }
 
+__device__ __forceinline__ bool finite(float x) { return (__float_as_uint(x) & 0x7f800000u) != 0x7f800000u; }
+
+// The factors that scale a key and a query, from their sums of squares. A key whose squares overflow has no length in FP32 and its
+// products with others none either: it is no number, in every form. So is a query that is to be divided by its length.
+__device__ __forceinline__ float key_scale(const Args &a, float kk) { return !finite(kk) ? qnan() : a.normalize ? 1.f / sqrtf(kk + kNormEps) : 1.f; }
+__device__ __forceinline__ float query_scale(const Args &a, float qq) {
+    return (!a.normalize ? 1.f : finite(qq) ? 1.f / sqrtf(qq + kNormEps) : qnan()) * a.scale;
+}
+
 __device__ __forceinline__ void unpack8(u32x4 u, float (&v)[8]) {
 #pragma unroll
     for (int i = 0; i < 4; ++i) v[2 * i] = __uint_as_float(u[i] << 16), v[2 * i + 1] = __uint_as_float(u[i] & 0xFFFF0000u);
@@ -124,8 +133,6 @@ __device__ __forceinline__ void split(const float (&x)[8], bf16x8 (&o)[N]) {
 }
 
 __device__ __forceinline__ f32x4 mfma(bf16x8 a, bf16x8 b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
-
-__device__ __forceinline__ bool finite(float x) { return (__float_as_uint(x) & 0x7f800000u) != 0x7f800000u; }
 
 // Host: what prefill needs (gated_delta_prefill.hip).
 size_t prefill_bytes(int64_t T, int64_t B, int64_t Hk, int64_t Hv, int64_t Dk);

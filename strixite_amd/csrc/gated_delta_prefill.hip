@@ -131,9 +131,8 @@ __global__ void __launch_bounds__(256, 4) delta_prepare_kernel(const Args a, con
     }
     kk = sum_rows(kk), qq = sum_rows(qq);
     if (g4 == 0) {
-        // a key that is no number has no length
-        rk[wave * 16 + n16] = !finite(kk) ? qnan() : a.normalize ? 1.f / sqrtf(kk + kNormEps) : 1.f;
-        rq[wave * 16 + n16] = (a.normalize ? 1.f / sqrtf(qq + kNormEps) : 1.f) * a.scale;
+        rk[wave * 16 + n16] = key_scale(a, kk);
+        rq[wave * 16 + n16] = query_scale(a, qq);
     }
     __syncthreads();
     if (wave == 0) {

@@ -1,5 +1,5 @@
-"""The gated delta rule on cuda:0 where its sums cancel, where starts fall and where a gate forgets everything: the three forms (steps,
-prompts in chunks, drafted trees with their commit) give one answer.
+"""The gated delta rule on cuda:0 where its sums cancel, where starts fall, where a gate forgets everything and where a key has no
+length: the three forms (steps, prompts in chunks, drafted trees with their commit) give one answer.
 
 Tolerances as in test_gpu_delta.py (u16 = 2^-8, u32 = 2^-24; c roundings a step)."""
 import math
@@ -156,3 +156,29 @@ def test_a_reset_is_the_same_token_in_every_form(Dk):
     x.state = torch.where(torch.arange(x.state.shape[0], device="cuda")[:, None, None, None] == x.slot(1), -3 * y, y)
     for f, s in zip(("steps", "prompt", "verify"), (s1, s2, s3)):
         assert torch.equal(through(x, f)[1][x.slot(1)], s[x.slot(1)]), f
+
+
+# ---------------- keys and queries without a length ----------------
+
+@pytest.mark.parametrize("normalize", [True, False])
+@pytest.mark.parametrize("form,n,at", [("steps", 9, 4), ("prompt", 9, 4), ("prompt", 100, 70), ("verify", 9, 4), ("verify", 40, 33)])
+def test_a_key_whose_squares_overflow_is_no_number(form, n, at, normalize):
+    x = Tokens([n, 2], Hk=2, Hv=4, seed=n + at, normalize=normalize, raw=not normalize)
+    ref, refs = through(x, form)
+    x.k[at, 0, 3] = 2.0 ** 65
+    out, got = through(x, form)
+    assert torch.equal(out[n:], ref[n:]) and torch.equal(out[:, 2:], ref[:, 2:]) and torch.equal(got[:, 2:], refs[:, 2:])
+    assert out[at:n, :2].isnan().all() and got[x.slot(0), :2].isnan().all() and torch.equal(got[x.slot(1)], refs[x.slot(1)])
+    before, was = out[:at].double(), ref[:at].double()  # (verify: products of tokens in FP32 where one is no number)
+    assert torch.equal(before, was) if form != "verify" else (before - was).norm() <= 2 * U16 * was.norm()
+
+
+@pytest.mark.parametrize("form,n,at", [("steps", 9, 4), ("prompt", 100, 70), ("verify", 40, 33)])
+def test_a_query_whose_squares_overflow_is_its_own_rows_loss(form, n, at):
+    x = Tokens([n, 2], Hk=2, Hv=4, seed=n + at)
+    ref, refs = through(x, form)
+    x.q[at, 0, 3] = 2.0 ** 65
+    out, got = through(x, form)
+    assert out[at, :2].isnan().all() and torch.equal(got, refs) and torch.equal(out[at, 2:], ref[at, 2:])
+    rest = [i for i in range(n + 2) if i != at]
+    assert torch.equal(out[rest], ref[rest])
