@@ -172,8 +172,9 @@ class VerifyDelta:
     8); A_log, dt_bias FP32 [Hv]; head_w BF16 [Dv], Dv a power of two up to 512; out_w an Int8Weight [d, Hv Dv]. mix (optional): called
     with the BF16 views q, k [T, Hk, Dk] and v [T, Hv, Dv] after the projection (a short convolution), forward's stream being the
     current one. Drafted tokens (a mask) leave the states as they are until commit takes the accepted path of the last forward;
-    without a mask (prompts, decoding) forward updates them. Buffers are kept for every stream that forward is called on; k, u and
-    decay, residual and y are the last forward's."""
+    without a mask (prompts, decoding) forward updates them. A forward is committed once; one in a captured graph once behind every replay,
+    which is the caller's to see to. Buffers are kept for every stream that forward is called on; k, u and decay, residual and y are
+    the last forward's."""
 
     def __init__(self, norm_w, proj, A_log, dt_bias, head_w, out_w, Hk, Hv, Dk, Dv, max_tokens, post_w=None, eps=1e-6, residual_scale=1.0,
                  mix=None):
@@ -183,7 +184,7 @@ class VerifyDelta:
         self.Hk, self.Hv, self.Dk, self.Dv, self.M, self.eps, self.residual_scale, self.mix = Hk, Hv, Dk, Dv, max_tokens, eps, residual_scale, mix
         self._dev = norm_w.device
         self.err = torch.zeros(4, dtype=torch.int32, device=self._dev)
-        self.k, self.drafted = None, False
+        self.k, self.drafted, self._replayed = None, False, False
         self._buffers = {}
 
     def _buffers_for(self, stream):
@@ -207,6 +208,7 @@ class VerifyDelta:
                 return self.forward(x, residual, state, starts, max_len, mask, slots, stream)
         T, Hk, Hv, Dk, Dv = x.shape[0], self.Hk, self.Hv, self.Dk, self.Dv
         assert T <= self.M
+        self.drafted = False  # until all of it has been taken
         self._buffers_for(stream)
         res = None if residual is None else self.residual[:T]
         kx.block_norm_int8(x, post=self.post_w, residual=residual, pre=self.norm_w, eps=self.eps, residual_scale=self.residual_scale,
@@ -218,7 +220,6 @@ class VerifyDelta:
             with torch.cuda.stream(stream):  # the projection runs there (None: the current one)
                 self.mix(q, self.k, v)
         args, kw = (q, self.k, v, a, b, state, starts), dict(slots=slots, A_log=self.A_log, dt_bias=self.dt_bias, out=self.out[:T], err=self.err, stream=stream)
-        self.drafted = mask is not None
         if mask is None:
             kx.gated_delta(*args, max_len, **kw)
         else:
@@ -226,15 +227,18 @@ class VerifyDelta:
         kx.block_norm_int8(self.out[:T].view(T, Hv * Dv), post=self.head_w, gate=z, group=Dv, gate_act="silu", eps=self.eps, q=self.o8[:T],
                            scale=self.o_scale[:T], stream=stream)
         kx.linear_int8(self.o8[:T], self.o_scale[:T], self.out_w, y=self.y[:T], stream=stream)
+        self.drafted, self._replayed = mask is not None, torch.cuda.is_current_stream_capturing()
         return self.y[:T], x if residual is None else res
 
     def commit(self, state, starts, count, path=None, max_count=None, slots=None, stream=None):
         """The accepted path of the last forward's drafted tokens into the states, as gated_delta_commit."""
         if not self.drafted:
-            raise SxError(SX_EINVAL, "the last forward had no drafted tokens: its states are up to date")
+            raise SxError(SX_EINVAL, "no drafted tokens to commit: the last forward had none, was refused, or is committed")
         T = self.k.shape[0]
         kx.gated_delta_commit(self.k, self.u[:T], self.decay[:T], state, starts, count, path=path, max_count=max_count, slots=slots, err=self.err,
                               stream=stream)
+        if not self._replayed and not torch.cuda.is_current_stream_capturing():  # captured, it has not run yet, or runs again
+            self.drafted = False
 
 
 class VerifyTail:

@@ -1,0 +1,81 @@
+"""What VerifyDelta keeps from call to call on cuda:0: a forward's drafted tokens are committed once, a forward that was refused
+leaves nothing to commit."""
+import pytest
+import torch
+
+from strixite_amd import SxError
+from strixite_amd import kernels as kx
+from tests.test_gpu_recurrent_layer import BF, Dk, Dv, Hv, d, gen, i32, layer
+
+pytestmark = pytest.mark.gpu
+
+
+def drafted(L, n=6, seed=0):
+    """A forward of drafted tokens and the arguments of its commit."""
+    x, state = torch.randn(n, d, device="cuda", generator=gen(seed)).to(BF), 0.3 * torch.randn(2, Hv, Dk, Dv, device="cuda", generator=gen(seed + 1))
+    starts, mask = i32([0, n]), kx.tree_mask([list(range(-1, n - 1))]).cuda()
+    run = lambda **kw: L.forward(x, None, state, starts, n, **{**dict(mask=mask), **kw})
+    run()
+    return state, starts, run
+
+
+def test_a_forward_is_committed_once():
+    L = layer(2)
+    state, starts, run = drafted(L)
+    L.commit(state, starts, i32([3]), max_count=6)
+    once = state.clone()
+    with pytest.raises(SxError, match="no drafted tokens"):
+        L.commit(state, starts, i32([3]), max_count=6)
+    assert torch.equal(state, once)
+    run()
+    L.commit(state, starts, i32([2]), max_count=6)
+    assert not torch.equal(state, once)
+
+
+def test_a_refused_commit_may_be_asked_again():
+    L = layer(2)
+    state, starts, _ = drafted(L)
+    with pytest.raises(SxError, match="max_count"):
+        L.commit(state, starts, i32([3]))
+    L.commit(state, starts, i32([3]), max_count=6)
+
+
+def test_a_captured_forward_is_committed_behind_every_replay():
+    L = layer(2)
+    state, starts, run = drafted(L)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        run()
+    ref = state.clone()
+    for i in range(4):
+        graph.replay()
+        torch.cuda.synchronize()
+        L.commit(state, starts, i32([1 + i]), max_count=6)
+        M = layer(2)
+        M.forward(torch.randn(6, d, device="cuda", generator=gen(0)).to(BF), None, ref, starts, 6, mask=kx.tree_mask([list(range(-1, 5))]).cuda())
+        M.commit(ref, starts, i32([1 + i]), max_count=6)
+        assert torch.equal(state, ref)
+
+
+def test_a_captured_commit_has_not_run_yet():
+    L = layer(2)
+    state, starts, _ = drafted(L)
+    before, count, graph = state.clone(), i32([3]), torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        L.commit(state, starts, count, max_count=6)
+    assert torch.equal(state, before)
+    L.commit(state, starts, count, max_count=6)  # this one does
+    once = state.clone()
+    state.copy_(before)
+    graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(state, once) and not torch.equal(once, before)
+
+
+def test_a_refused_forward_leaves_nothing_to_commit():
+    L = layer(2)
+    state, starts, run = drafted(L)
+    with pytest.raises(SxError, match="mask must be"):
+        run(mask=torch.ones(6, 1, dtype=torch.int32, device="cuda"))
+    with pytest.raises(SxError, match="no drafted tokens"):
+        L.commit(state, starts, i32([3]), max_count=6)
