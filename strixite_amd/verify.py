@@ -200,8 +200,8 @@ class VerifyDelta:
         vars(self).update(self._buffers[key])
 
     def forward(self, x, residual, state, starts, max_len, mask=None, slots=None, stream=None):
-        """x, residual (None in the first layer) BF16 [T, d]; state, starts, slots and, for drafted tokens, mask as gated_delta_verify
-        takes them, at most max_len tokens a sequence. Returns (y [T, d], the residual stream). Runs on the layer's device, whichever is
+        """x, residual (None in the first layer, which has no block before it: x is the stream, without a post norm) BF16 [T, d]; state,
+        starts, slots and, for drafted tokens, mask as gated_delta_verify takes them, at most max_len tokens a sequence. Returns (y [T, d], the residual stream). Runs on the layer's device, whichever is
         current."""
         if self.norm_w.is_cuda and self._dev.index != torch.cuda.current_device():
             with torch.cuda.device(self._dev):
@@ -211,7 +211,7 @@ class VerifyDelta:
         self.drafted = False  # until all of it has been taken
         self._buffers_for(stream)
         res = None if residual is None else self.residual[:T]
-        kx.block_norm_int8(x, post=self.post_w, residual=residual, pre=self.norm_w, eps=self.eps, residual_scale=self.residual_scale,
+        kx.block_norm_int8(x, post=None if residual is None else self.post_w, residual=residual, pre=self.norm_w, eps=self.eps, residual_scale=self.residual_scale,
                            residual_out=res, q=self.q8[:T], scale=self.scale[:T], stream=stream)
         rows = kx.linear_int8(self.q8[:T], self.scale[:T], self.proj, y=self.rows[:T], stream=stream)
         q, k, v, z, a, b = rows[:, :2 * Hk * Dk + 2 * Hv * Dv + 2 * Hv].split([Hk * Dk, Hk * Dk, Hv * Dv, Hv * Dv, Hv, Hv], dim=1)

@@ -1,5 +1,5 @@
 """What VerifyDelta keeps from call to call on cuda:0: a forward's drafted tokens are committed once, a forward that was refused
-leaves nothing to commit."""
+leaves nothing to commit, the first layer has no block behind it."""
 import pytest
 import torch
 
@@ -79,3 +79,12 @@ def test_a_refused_forward_leaves_nothing_to_commit():
         run(mask=torch.ones(6, 1, dtype=torch.int32, device="cuda"))
     with pytest.raises(SxError, match="no drafted tokens"):
         L.commit(state, starts, i32([3]), max_count=6)
+
+
+def test_the_first_layer_has_no_block_behind_it():
+    """Without a residual the stream is x itself: the post norm is of the block before, and there is none."""
+    L, plain = layer(3, post_w=(1 + 0.2 * torch.randn(d, device="cuda", generator=gen(9))).to(BF)), layer(3)
+    x, states = torch.randn(5, d, device="cuda", generator=gen(4)).to(BF), torch.zeros(2, 1, Hv, Dk, Dv, device="cuda")
+    y, res = L.forward(x, None, states[0], i32([0, 5]), 5)
+    want, _ = plain.forward(x, None, states[1], i32([0, 5]), 5)
+    assert torch.equal(y, want) and res is x and torch.equal(states[0], states[1])
