@@ -173,8 +173,9 @@ class VerifyDelta:
     with the BF16 views q, k [T, Hk, Dk] and v [T, Hv, Dv] after the projection (a short convolution), forward's stream being the
     current one. Drafted tokens (a mask) leave the states as they are until commit takes the accepted path of the last forward;
     without a mask (prompts, decoding) forward updates them. A forward is committed once; one in a captured graph once behind every replay,
-    which is the caller's to see to. Buffers are kept for every stream that forward is called on; k, u and decay, residual and y are
-    the last forward's."""
+    which is the caller's to see to. Buffers are kept for every stream that forward is called on, and, from its first prompt on, a
+    workspace for prompts of max_tokens in all (28 KB a token with Hk = 16, Hv = 32, Dk = 128); k, u and decay, residual and y are the
+    last forward's."""
 
     def __init__(self, norm_w, proj, A_log, dt_bias, head_w, out_w, Hk, Hv, Dk, Dv, max_tokens, post_w=None, eps=1e-6, residual_scale=1.0,
                  mix=None):
@@ -185,10 +186,10 @@ class VerifyDelta:
         self._dev = norm_w.device
         self.err = torch.zeros(4, dtype=torch.int32, device=self._dev)
         self.k, self.drafted, self._replayed = None, False, False
-        self._buffers = {}
+        self._buffers, self._ws, self._captured_ws = {}, {}, []
 
     def _buffers_for(self, stream):
-        """The stream's buffers become the layer's."""
+        """The stream's buffers become the layer's. Returns the stream's key."""
         key = (stream or torch.cuda.current_stream(self._dev)).cuda_stream
         if key not in self._buffers:
             M, d, Hv, Dv = self.M, self.proj.K, self.Hv, self.Dv
@@ -198,18 +199,33 @@ class VerifyDelta:
                 self._buffers[key] = dict(residual=e(bf, M, d), q8=e(i8, M, d), scale=e(f32, M), rows=e(bf, M, self.proj.N), out=e(bf, M, Hv, Dv),
                                           u=e(f32, M, Hv, Dv), decay=e(f32, M, Hv), o8=e(i8, M, Hv * Dv), o_scale=e(f32, M), y=e(bf, M, d))
         vars(self).update(self._buffers[key])
+        return key
+
+    def _ws_for(self, key, B, stream):
+        """The stream's workspace for prompts: of max_tokens and as many sequences as a call has had. A larger one takes its place, but one
+        that a graph has captured stays."""
+        n = (kx.gated_delta_workspace_bytes(self.M, B, self.Hk, self.Hv, self.Dk, 17) + 7) // 8  # any limit over a step's
+        ws, captured = self._ws.get(key, (None, False))
+        if ws is None or ws.numel() < n:
+            if captured:
+                self._captured_ws.append(ws)
+            captured = False
+            with torch.cuda.device(self._dev), torch.cuda.stream(stream):  # from the stream's pool (None: the current one's)
+                ws = torch.empty(n, dtype=torch.int64, device=self._dev)
+        self._ws[key] = ws, captured or torch.cuda.is_current_stream_capturing()
+        return ws
 
     def forward(self, x, residual, state, starts, max_len, mask=None, slots=None, stream=None):
         """x, residual (None in the first layer, which has no block before it: x is the stream, without a post norm) BF16 [T, d]; state,
-        starts, slots and, for drafted tokens, mask as gated_delta_verify takes them, at most max_len tokens a sequence. Returns (y [T, d], the residual stream). Runs on the layer's device, whichever is
-        current."""
+        starts, slots and, for drafted tokens, mask as gated_delta_verify takes them, at most max_len tokens a sequence. Returns
+        (y [T, d], the residual stream). Runs on the layer's device, whichever is current."""
         if self.norm_w.is_cuda and self._dev.index != torch.cuda.current_device():
             with torch.cuda.device(self._dev):
                 return self.forward(x, residual, state, starts, max_len, mask, slots, stream)
         T, Hk, Hv, Dk, Dv = x.shape[0], self.Hk, self.Hv, self.Dk, self.Dv
         assert T <= self.M
         self.drafted = False  # until all of it has been taken
-        self._buffers_for(stream)
+        key = self._buffers_for(stream)
         res = None if residual is None else self.residual[:T]
         kx.block_norm_int8(x, post=None if residual is None else self.post_w, residual=residual, pre=self.norm_w, eps=self.eps, residual_scale=self.residual_scale,
                            residual_out=res, q=self.q8[:T], scale=self.scale[:T], stream=stream)
@@ -221,7 +237,7 @@ class VerifyDelta:
                 self.mix(q, self.k, v)
         args, kw = (q, self.k, v, a, b, state, starts), dict(slots=slots, A_log=self.A_log, dt_bias=self.dt_bias, out=self.out[:T], err=self.err, stream=stream)
         if mask is None:
-            kx.gated_delta(*args, max_len, **kw)
+            kx.gated_delta(*args, max_len, ws=self._ws_for(key, starts.numel() - 1, stream) if max_len > 16 else None, **kw)
         else:
             kx.gated_delta_verify(*args, mask, max_len, u=self.u[:T], decay=self.decay[:T], **kw)
         kx.block_norm_int8(self.out[:T].view(T, Hv * Dv), post=self.head_w, gate=z, group=Dv, gate_act="silu", eps=self.eps, q=self.o8[:T],

@@ -1,5 +1,5 @@
 """What VerifyDelta keeps from call to call on cuda:0: a forward's drafted tokens are committed once, a forward that was refused
-leaves nothing to commit, the first layer has no block behind it."""
+leaves nothing to commit, the first layer has no block behind it, prompts allocate nothing."""
 import pytest
 import torch
 
@@ -88,3 +88,45 @@ def test_the_first_layer_has_no_block_behind_it():
     y, res = L.forward(x, None, states[0], i32([0, 5]), 5)
     want, _ = plain.forward(x, None, states[1], i32([0, 5]), 5)
     assert torch.equal(y, want) and res is x and torch.equal(states[0], states[1])
+
+
+def test_prompts_allocate_nothing():
+    L = layer(4, max_tokens=400)
+    x, state = torch.randn(400, d, device="cuda", generator=gen(1)).to(BF), torch.zeros(4, Hv, Dk, Dv, device="cuda")
+    calls = [(400, i32([0, 400]), 400), (300, i32([0, 100, 300]), 200), (60, i32([0, 20, 40, 60]), 20)]
+    for T, starts, most in calls:
+        L.forward(x[:T], None, state, starts, most)
+    torch.cuda.synchronize()
+    before = torch.cuda.memory_stats()["allocation.all.allocated"]
+    for T, starts, most in calls:
+        L.forward(x[:T], None, state, starts, most)
+    assert torch.cuda.memory_stats()["allocation.all.allocated"] == before
+
+
+def test_a_larger_workspace_leaves_a_captured_ones_alone():
+    """A graph of a prompt keeps its workspace when a call of more sequences needs a larger one."""
+    L = layer(4, max_tokens=400)
+    x = torch.randn(400, d, device="cuda", generator=gen(1)).to(BF)
+    state, starts = torch.zeros(1, Hv, Dk, Dv, device="cuda"), i32([0, 40])
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    L.forward(x[:40], None, state, starts, 40, stream=s)
+    s.synchronize()
+    state.zero_()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=s):
+        y, _ = L.forward(x[:40], None, state, starts, 40)
+    many = i32([0] + [360 * (i + 1) // 300 for i in range(300)])
+    other = torch.zeros(300, Hv, Dk, Dv, device="cuda")
+    ref_state = torch.zeros_like(state)
+    ref = layer(4, max_tokens=400).forward(x[:40], None, ref_state, starts, 40)[0]
+    for _ in range(3):
+        L.forward(x[:360], None, other, many, 40, stream=s)
+        with torch.cuda.stream(s):
+            fill = [torch.full((1 << 18,), 1e30, device="cuda") for _ in range(200)]  # over whatever was given back
+        s.synchronize()
+        state.zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(y, ref) and torch.equal(state, ref_state)
+        del fill
