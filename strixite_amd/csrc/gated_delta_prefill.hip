@@ -17,8 +17,8 @@
 // FP32 values enter as three BF16 terms, which together are the value; of a product of two such values the six largest of the nine
 // products are taken (what is left is under 2^-22 of it).
 //
-// Tokens that are no numbers: a triangular product would carry them to the tokens before them in the chunk. They are taken
-// out and everything from them on (a value's: in its column) is NaN, as the rule has it.
+// Tokens that are no numbers, and corrections too large for one: a triangular product would carry them to the tokens before them in
+// the chunk. They are taken out and everything from them on (a value's or a correction's: in its column) is NaN, as the rule has it.
 #include "gated_delta.hpp"
 
 #include <type_traits>
@@ -424,21 +424,20 @@ __global__ void __launch_bounds__(512) delta_scan_kernel(const Args a, const Wor
             lds_barrier();
             // this wave's 16 tokens: what the state does not explain of them
             const f32x4 x = (xs[0][wave][lane] + xs[1][wave][lane]) + (xs[2][wave][lane] + xs[3][wave][lane]);
-            float r[4], v[4];
+            float r[4];
             bool odd = now.bad < kC;
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
-                v[j] = bf16_to_f32(now.v[j]);
-                odd |= !finite(v[j]);
-                r[j] = v[j] - now.in[j] * x[j];
+                r[j] = bf16_to_f32(now.v[j]) - now.in[j] * x[j];
+                odd |= !finite(r[j]);
             }
             if (now.use != ~0ull || __any(odd)) {
                 int at = now.bad;
 #pragma unroll
                 for (int j = 3; j >= 0; --j) {
                     const bool use = now.use >> (mine + j) & 1;
-                    if (use && !finite(v[j])) at = min(at, mine + j);
-                    r[j] = !use ? 0.f : finite(v[j]) ? r[j] : -now.in[j] * x[j];
+                    if (use && !finite(r[j])) at = min(at, mine + j);
+                    r[j] = use && finite(r[j]) ? r[j] : 0.f;
                 }
                 if (at < kC) atomicMin(&poison[n16], c * kC + at);
             }
@@ -460,8 +459,17 @@ __global__ void __launch_bounds__(512) delta_scan_kernel(const Args a, const Wor
             fetch_t(c + 1, now);
             u += u2;
             float uu[4], uk[4];
+            odd = false;
 #pragma unroll
-            for (int j = 0; j < 4; ++j) uu[j] = u[j], uk[j] = u[j] * keep[j];
+            for (int j = 0; j < 4; ++j) uu[j] = u[j], uk[j] = u[j] * keep[j], odd |= !finite(uu[j]);
+            if (__any(odd)) {  // too large for FP32
+#pragma unroll
+                for (int j = 3; j >= 0; --j) {
+                    if (finite(uu[j])) continue;
+                    atomicMin(&poison[n16], c * kC + mine + j);
+                    uu[j] = uk[j] = 0.f;
+                }
+            }
 #pragma unroll
             for (int i = 0; i < 3; ++i) put(ks, i, uk);
 #pragma unroll

@@ -182,3 +182,23 @@ def test_a_query_whose_squares_overflow_is_its_own_rows_loss(form, n, at):
     assert out[at, :2].isnan().all() and torch.equal(got, refs) and torch.equal(out[at, 2:], ref[at, 2:])
     rest = [i for i in range(n + 2) if i != at]
     assert torch.equal(out[rest], ref[rest])
+
+
+# ---------------- sums that overflow ----------------
+
+@pytest.mark.parametrize("form,n,at", [("steps", 12, 5), ("prompt", 12, 5), ("prompt", 100, 40), ("prompt", 100, 70), ("verify", 12, 5), ("verify", 50, 20)])
+def test_a_correction_too_large_for_fp32_reaches_only_what_is_behind_it(form, n, at):
+    """A value of 3e38 under the key that the token before gave -3e38: the correction is not in FP32's range. Rows before it, other
+    columns, heads and sequences are as they are without the second value."""
+    x = Tokens([n, 3], Hk=1, Hv=2, Dk=64, Dv=64, raw=True, f32=True, seed=n + at)
+    x.a.zero_(), x.b.fill_(1.0)
+    x.k[at] = x.k[at - 1]
+    ref, refs = through(x, form)
+    x.v[at - 1, 0, 7], x.v[at, 0, 7] = -3e38, 3e38
+    out, got = through(x, form)
+    near = lambda a, b: torch.equal(a, b) or form == "verify" and (a.double() - b.double()).norm() <= 2 * U16 * b.double().norm()  # products of tokens in FP32 there
+    assert near(out[:at - 1, 0, 7], ref[:at - 1, 0, 7]) and torch.isfinite(out[at - 1, 0, 7])
+    assert not torch.isfinite(out[at:n, 0, 7]).any() and not torch.isfinite(got[x.slot(0), 0, :, 7]).any()
+    for o, r in ((out[:, 0, :7], ref[:, 0, :7]), (out[:, 0, 8:], ref[:, 0, 8:]), (out[:, 1], ref[:, 1]), (out[n:], ref[n:])):
+        assert near(o, r)
+    assert torch.equal(got[x.slot(1)], refs[x.slot(1)]) and torch.equal(got[x.slot(0), 1], refs[x.slot(0), 1])
