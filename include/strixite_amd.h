@@ -370,7 +370,8 @@ int sx_moe_router_scored(const void *logits, int64_t ld, int64_t M, int64_t E, i
  * n_draft <= n_valid (the rest of the vocabulary: probability 0). With p, q the softmax of a row of each over temperature[b] and u
  * [T, 2] FP64 in [0, 1): draft d of row t stays if u[t, 0] q(d) < p(d). At the first that does not, a token from max(p - q, 0), behind the
  * last draft one from p: the first place at which the running sum passes u[t, 1] times the total. temperature 0 or less: a draft
- * stays if it is the row's largest logit (ties: the lowest place), which is the token otherwise. Probabilities and sums are FP64.
+ * stays if it is the row's largest logit (ties: the lowest place), which is the token otherwise. Probabilities and sums are FP64,
+ * exponentials good to 1e-14 of themselves.
  * tokens [batch, max_rows]: the drafts that stay, the token, then -1; count: how many; status 0. A row that counts and holds NaN or
  * no finite largest logit, a draft outside the vocabulary or a temperature that is not finite: status 1 + the row, count and tokens
  * the drafts before it. Impossible starts (negative, over max_rows, outside T, or behind a start that is below the one before it):
@@ -389,10 +390,11 @@ int sx_mtp_accept_sampled(const void *logits, int64_t ld, int64_t T, int64_t n_v
  *   r = residual_scale * residual + branch_scale * h    rounded to act and stored to residual_out; residual null: branch_scale * h
  *   y = r / sqrt(mean(r^2) + eps) * (pre + w_add)       pre null: y = r
  * Outputs: residual_out (with a residual), y (nullable) [M, K] in act, q (nullable) [M, K] int8 codes of y with scale [M] FP32 =
- * amax(|y|) / 127, the activations sx_linear_int8 takes. A code is the nearest one, ties to even, of y / scale as the formulas give it
- * in FP64, in their order (a mean is the sum times the rounded
- * 1 / K; only the order in which squares are added is open). A row of zeros has scale 0 and codes 0, one that holds NaN or an infinity scale NaN and
- * codes 0. post has post_len values: K (0 says so too) or the group's. K a multiple of 8, up to 16384. residual_out and y may be x,
+ * amax(|y|) / 127, the activations sx_linear_int8 takes. A code is the nearest whole number, ties to even, to 127 t / amax(|t|) with
+ * t = r (pre + w_add) (the second root is in both and cancels; pre null: t = r), where r is as the formulas give it in FP64, in their
+ * order: a mean is the sum times the rounded 1 / K, root and quotient are the nearest, and only the order in which squares are
+ * added is open. silu and sigmoid are good to 1e-14. A row of zeros has scale 0 and codes 0, one that holds NaN or an infinity scale
+ * NaN and codes 0. post has post_len values: K (0 says so too) or the group's. K a multiple of 8, up to 16384. residual_out and y may be x,
  * the residual or the gate, row for row. No reference counterpart. */
 enum sx_gate_act { SX_GATE_NONE = 0, SX_GATE_SILU = 1, SX_GATE_SIGMOID = 2 };
 typedef struct sx_block_norm {
