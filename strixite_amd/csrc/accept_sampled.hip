@@ -8,8 +8,8 @@
 // place and its sum of exponentials. Then a wave combines a row's chunks, the rows of a sequence at once, which tells the last row that
 // counts; that one's chunks of max(p - q, 0) are summed where there are draft logits, and one block a sequence finds the chunk,
 // and in it the token, at which the running sum passes u times the total (second launch). Sums are taken in one order, whatever
-// the schedule. 16 sequences of up to 6 rows of 151,936 logits with draft logits: 24 + 5.7 + 17 us, the first the VALU's (an FP64
-// exponential a logit, 0.65 of its cycles); one sequence without: 5.4 + 8.7, latencies.
+// the schedule. 16 sequences of up to 6 rows of 151,936 logits with draft logits: 25 + 5.6 + 17 us, the first the VALU's (an FP64
+// exponential a logit, 0.66 of its cycles); one sequence without: 5.5 + 8.7, latencies.
 #include "common.hpp"
 
 #include <cmath>

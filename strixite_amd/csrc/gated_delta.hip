@@ -6,7 +6,7 @@
 // Step: the cost is the state, read and written once (2 x 64 KB a head at 128 x 128), so it goes through registers: a wave
 // has 16 columns of one state, a lane four of them in Dk / 16 rows. Columns do not need each other, so waves never meet. Both
 // sums over Dk, S^T k and S^T q, are taken of the state before the token (o = e^g S^T q + (k . q) u), one reduction. One token each
-// of 48 sequences, 32 heads of 128: 43 us, 4.7 TB/s; of one sequence: 6.
+// of 48 sequences, 32 heads of 128: 44 us, 4.6 TB/s; of one sequence: 6.
 //
 // Verify: the drafted tokens are a tree, the state must not change before the accepted path is known, and token i needs
 // the state behind its ancestors only. With G the sum of g along a token's path and A_ij = beta_i e^(G_i - G_j) k_i . k_j for
@@ -14,8 +14,8 @@
 //   (I + A) U = beta (V - e^G K S),   o_i = e^G_i S^T q_i + sum_j e^(G_i - G_j) (q_i . k_j) u_j   (j: ancestors and i),
 // so the state is read once for all tokens, by the matrix unit, and no token's state is ever formed. U is what is left to
 // write: the commit adds k_j u_j^T along the accepted path to the state, for all layers in one launch. 32 heads of 128: 24 trees of
-// up to 24 25 us (a block's chain: waits 0.46 of its time, VALU 0.51) and 20 for the commit (5.1 TB/s, the states both ways); one
-// chain of 6: 8.4 and 6.
+// up to 24 26 us (a block's chain: waits 0.45 of its time, VALU 0.53) and 20 for the commit (5.1 TB/s, the states both ways); one
+// chain of 6: 9.0 and 6.6.
 #include "gated_delta.hpp"
 
 #include "kv_cache.hpp"

@@ -8,7 +8,7 @@
 // 32 heads of 128) and its four waves share a chunk: wave w holds a quarter of the state's rows in registers, multiplies K
 // and Q with them for all 64 tokens, and has a quarter of the tokens after that. What passes between the waves (sums of K S
 // and Q S, V - e^G K S, U) goes through LDS, three barriers a chunk. The latency of that chain is what bounds one
-// sequence: 8192 tokens, 32 heads of 128: 96 + 254 us, 2.0 us a chunk (the matrix unit busy 0.16 of it; 1.2 us without any loads,
+// sequence: 8192 tokens, 32 heads of 128: 99 + 259 us, 2.0 us a chunk (the matrix unit busy 0.18 of it; 1.2 us without any loads,
 // which are 100 KB a chunk and compute unit).
 //
 // Operands: a result of the matrix unit has four consecutive rows a lane, an operand eight consecutive values of a row. The
