@@ -451,7 +451,7 @@ typedef struct sx_delta {
 /* Tokens through the states, which are updated in place; out [T, heads, dim] BF16. max_len bounds a sequence's tokens: up to 16
  * they go one by one, in one launch without a workspace (sx_gated_delta_workspace_bytes says 0; ws may be null); above in chunks
  * of 64, two launches, ws 16-byte aligned, its contents never read before they are written, one per stream. A token that is no
- * number makes the rows from it on NaN (a value: its column of them), and the state. */
+ * number makes the rows from it on NaN (a value, or a correction too large for FP32: its column of them), and the state. */
 int sx_gated_delta_workspace_bytes(int64_t T, int64_t B, int64_t Hk, int64_t Hv, int64_t Dk, int64_t max_len, size_t *bytes);
 int sx_gated_delta(const sx_delta *d, int64_t max_len, const sx_head_rows *out, void *ws, size_t ws_bytes, uint32_t *err,
                    sx_stream stream);

@@ -4,9 +4,9 @@
 // logits q is all on the draft (a head that proposes its best token).
 //
 // The results are whole numbers that a border decides, and a token is picked out of sums over a vocabulary: probabilities and sums
-// are FP64 (exponentials good to 6e-15). All logits are read once, by as many blocks as they need: rows in chunks of 4096, a chunk's largest value, its
-// place and its sum of exponentials. Then a wave combines a row's chunks, the rows of a sequence at once, which tells the last row that
-// counts; that one's chunks of max(p - q, 0) are summed where there are draft logits, and one block a sequence finds the chunk,
+// are FP64 (exponentials good to 6e-15). All logits are read once, by as many blocks as they need: rows in chunks of 4096, a chunk's
+// largest value, its place and its sum of exponentials. Then a wave combines a row's chunks, the rows of a sequence at once, which tells
+// the last row that counts; that one's chunks of max(p - q, 0) are summed where there are draft logits, and one block a sequence finds the chunk,
 // and in it the token, at which the running sum passes u times the total (second launch). Sums are taken in one order, whatever
 // the schedule. 16 sequences of up to 6 rows of 151,936 logits with draft logits: 25 + 5.6 + 17 us, the first the VALU's (an FP64
 // exponential a logit, 0.66 of its cycles); one sequence without: 5.5 + 8.7, latencies.

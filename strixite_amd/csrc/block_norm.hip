@@ -8,11 +8,11 @@
 // A row is read once into registers (8 features a 16-byte load) and written from there. A code is a whole number that a border
 // decides, so it has to be that of the exact value: all is computed in FP64, which runs at FP32's rate here. Where a product of BF16
 // values lies on the border itself, the rounding of x / root decides, so mean, root and quotient are FP64's nearest and the code is
-// the formula's in 64 bits, but for silu and sigmoid, which are good to 6e-15 (40 instructions of 744 a wave; with a reciprocal root three calls in a hundred, without a residual, had a
-// code on the border's other side). The second norm's root cancels in the codes, which come from t = r (pre + w_add) alone. The VALU's
-// work bounds it where there is a gate (2048 rows of 4096, heads of 128: 24.8 us a call; a launch by itself 28.2, 0.74 of the VALU's cycles). In FP32 with a
-// bound on what that is off, and FP64 for what the bound leaves open (one code in two thousand, the row's largest value), it was as
-// slow: 820 instructions.
+// the formula's in 64 bits, but for silu and sigmoid, which are good to 6e-15 (40 instructions of 744 a wave; with a reciprocal root
+// three calls in a hundred, without a residual, had a code on the border's other side). The second norm's root cancels in the codes,
+// which come from t = r (pre + w_add) alone. The VALU's work bounds it where there is a gate (2048 rows of 4096, heads of 128: 24.8 us a
+// call; a launch by itself 28.2, 0.74 of the VALU's cycles). In FP32 with a bound on what that is off, and FP64 for what the bound
+// leaves open (one code in two thousand, the row's largest value), it was as slow: 820 instructions.
 #include "common.hpp"
 
 #include <cmath>

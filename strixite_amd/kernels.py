@@ -913,8 +913,8 @@ def gated_delta(q, k, v, a, b, state, starts, max_len, slots=None, A_log=None, d
     q, k [T, Hk, Dk] and v [T, Hv, Dv] BF16 (any token and head strides; Hv a multiple of Hk), divided by their lengths first
     (normalize), q times scale (1 / sqrt(Dk) unless given). Gates a, b [T, Hv] in BF16 or FP32: with A_log and dt_bias (FP32 [Hv])
     g = -exp(A_log) softplus(a + dt_bias), beta = sigmoid(b), else g = a and beta = b (g of -1e4 and less: a full reset). starts int32
-    [B + 1], not falling: sequence b's tokens are rows starts[b] .. starts[b + 1] - 1, at most max_len; state FP32 [states, Hv, Dk, Dv], number slots[b] (int32 [B]; None: b)
-    its own, updated in place (zeros: a new sequence). Up to 16 tokens a sequence go one by one, more in chunks. ws:
+    [B + 1], not falling: sequence b's tokens are rows starts[b] .. starts[b + 1] - 1, at most max_len; state FP32 [states, Hv, Dk, Dv],
+    number slots[b] (int32 [B]; None: b) its own, updated in place (zeros: a new sequence). Up to 16 tokens a sequence go one by one, more in chunks. ws:
     gated_delta_workspace(), made for the call unless given. Returns (out [T, Hv, Dv] BF16, err)."""
     dev = q.get_device()
     _together(dev, (k, v, a, b, state, starts, slots, A_log, dt_bias, out, ws, err))
